@@ -26,6 +26,16 @@ class GemmFusedArgs(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    """``bxl_linear_args`` of include/basedxl_b200.h."""
+
+    _fields_ = [
+        ("x", _vp), ("ldx", _ll), ("weight", _vp), ("ldw", _ll), ("bias", _vp), ("residual", _vp), ("ldr", _ll), ("y", _vp), ("ldy", _ll),
+        ("pre", _vp), ("ldp", _ll), ("dy", _vp), ("lddy", _ll), ("dx", _vp), ("lddx", _ll), ("dweight", _vp), ("lddw", _ll), ("dbias", _vp),
+        ("workspace", _vp), ("workspace_bytes", _ll), ("M", _i), ("N", _i), ("K", _i), ("dtype", _i), ("act", _i),
+    ]
+
+
 # name -> (restype, argtypes); mirrors include/basedxl_b200.h one to one
 SIGNATURES = {
     "bxl_init": (_i, []),
@@ -47,6 +57,10 @@ SIGNATURES = {
     "bxl_gemm_split_f32": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _ll, _vp]),
     "bxl_gemm_ragged_workspace_bytes": (_ll, [_i, _i, _i]),
     "bxl_gemm_ragged_f16": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _ll, _vp, _ll, _i, _i, _i, _vp, _ll, _vp]),
+    "bxl_linear_act_fwd_workspace_bytes": (_ll, [C.POINTER(LinearArgs)]),
+    "bxl_linear_act_fwd": (_i, [C.POINTER(LinearArgs), C.POINTER(_i), _vp]),
+    "bxl_linear_act_bwd_workspace_bytes": (_ll, [C.POINTER(LinearArgs)]),
+    "bxl_linear_act_bwd": (_i, [C.POINTER(LinearArgs), C.POINTER(_i), _vp]),
     "bxl_conv_weight_pack_f16": (_i, [_vp, _vp, _i, _i, _vp]),
     "bxl_conv3x3_halo_f16": (_i, [_vp, _ll, _vp, _vp, _ll, _vp, _vp, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "bxl_conv3x3_direct_f16": (_i, [_vp, _ll, _vp, _vp, _ll, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
@@ -65,6 +79,9 @@ SIGNATURES = {
     "bxl_comm_exchange": (_i, [_vp, C.POINTER(_vp), _ll, _vp, C.POINTER(_vp), _i, _i, _i, C.c_double, _vp]),
     "bxl_upsample2x_f16": (_i, [_vp, _vp, _i, _i, _i, _i, _vp]),
     "bxl_layernorm_f16": (_i, [_vp, _vp, _vp, _vp, _ll, _i, _f, _vp]),
+    "bxl_layernorm_fwd": (_i, [_vp, _ll, _vp, _vp, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _f, _vp]),
+    "bxl_layernorm_bwd_workspace_bytes": (_ll, [_ll, _i]),
+    "bxl_layernorm_bwd": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _vp, _ll, _vp]),
     "bxl_geglu_f16": (_i, [_vp, _vp, _ll, _i, _vp]),
     "bxl_cfg_euler_step": (_i, [_vp, _vp, _vp, _ll, _f, _f, _f, _vp]),
 }

@@ -337,6 +337,8 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int m, int n, int a_mn_maj
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+constexpr uint32_t kIdescBf16 = (1u << 7) | (1u << 10);   // added to it: bf16 A and B
+
 // D[tmem] (+)= A[smem] * B[smem]; issued by ONE thread.
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {

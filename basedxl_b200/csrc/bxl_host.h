@@ -68,6 +68,38 @@ int launch_kernel(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 bl
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...), what);
 }
 
+// ---- products and helpers that several entry points share --------------------------
+// C[M,N] = act(A * B + bias) + residual on the tensor cores (gemm_conv.cu), fp16 or bf16 in and out.  A is [M,K] (a_mn: [K,M]),
+// B is [N,K] (b_kn: [K,N]); their rows are 16-byte aligned (repack_rows), those of the rest may lie anywhere.
+struct LinearProduct {
+  const void* A;
+  long long lda;
+  int a_mn;
+  const void* B;
+  long long ldb;
+  int b_kn, b_is_weight;
+  const void* bias;
+  const void* residual;
+  long long ldr;
+  void* C;
+  long long ldc;
+  void* pre;                // also receives A * B + bias, or null
+  long long ldp;
+  int act, bf16, M, N, K;
+};
+int linear_product(const LinearProduct& q, cudaStream_t stream);
+// Copies the rows of up to two 16-bit matrices to rows ld_dst (a multiple of 8) apart; dst null = nothing to copy.
+struct RowCopy {
+  const void* src;
+  void* dst;
+  long long ld, ld_dst;
+  int rows, cols;
+};
+int repack_rows(const RowCopy& a, const RowCopy& b, cudaStream_t stream);
+// out0[c] = sum over i < count of part[i * pitch + c], out1[c] the same of part[i * pitch + C + c] (either may be null), in a
+// fixed order; `dtype` of the results (layernorm.cu).
+int sum_partials(const float* part, int count, long long pitch, int C, void* out0, void* out1, int dtype, cudaStream_t stream);
+
 // Clusters of `width` CTAs that can be resident at one time, for a kernel of which an SM holds one CTA.  Fewer than
 // SMs / width: a cluster stays inside one GPC, whose SM count need not be a multiple of the width.  Asked of the
 // runtime once per device and width (`cache`: one count per width up to 4, per device; threads that ask at the same

@@ -38,8 +38,12 @@
 // Roofline: tensor cores.  Algorithmic FLOPs per tile = 2*128*BN*K.
 #include <math.h>
 
+#include <type_traits>
+
+#include "bxl_act.cuh"
 #include "bxl_common.cuh"
 #include "bxl_host.h"
+#include "bxl_types.cuh"
 #include "../../include/basedxl_b200.h"
 
 namespace bxl {
@@ -110,6 +114,11 @@ struct alignas(64) GemmParams {
   int tiles_x, tiles_y;        // tiles per image
   int has_top, has_bot;
   int* dev_status;
+  // linear layers with an activation (fp16 or bf16: `bias`, `residual` and C are of that type)
+  int a_mn;                    // A given as [K,M] row-major (MN-major operand): the weight's gradient
+  int act;                     // BXL_ACT_*, applied after the bias and before the residual
+  void* pre;                   // [M][ldp]: also store the value before the activation; or null
+  long long ldp;
 };
 
 // Split-K exchange buffer of one CTA: for each of the (split-1) peers, the fp32
@@ -285,6 +294,91 @@ __device__ __forceinline__ void store_chunk_ragged(const GemmParams& p, const fl
   }
 }
 
+// Epilogue of the linear layers (T: fp16 or bf16): bias, the value before the activation where a backward pass will want it,
+// activation in fp32, residual.  `f` holds 32 consecutive columns of one row.
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  Vec<T, 2> h;
+  h.v[0] = from_f32<T>(a), h.v[1] = from_f32<T>(b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+__device__ __forceinline__ void store_row_chunk(T* to, const float (&f)[32], bool fullw, int left) {
+  if (fullw) {
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack2<T>(f[2 * j], f[2 * j + 1]);
+    if ((reinterpret_cast<uintptr_t>(to) & 31u) == 0) {
+      st_global_v8(to, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+      st_global_v8(to + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(to + q * 8) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) to[j] = from_f32<T>(f[j]);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_chunk_act(const GemmParams& p, float (&f)[32], long long out_row, int nb, const float* sbias,
+                                                const ResidualChunk& res) {
+  const bool fullw = (nb + 32 <= p.N);
+  if (sbias) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 b4 = *reinterpret_cast<const float4*>(sbias + 4 * q);
+      f[4 * q] += b4.x, f[4 * q + 1] += b4.y, f[4 * q + 2] += b4.z, f[4 * q + 3] += b4.w;
+    }
+  }
+  if (p.pre) store_row_chunk<T>(static_cast<T*>(p.pre) + out_row * p.ldp + nb, f, fullw, p.N - nb);
+  with_act(p.act, [&](auto act) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f[j] = act_value<decltype(act)::value>(f[j]);
+  });
+  if (p.residual) {
+    const T* rr = reinterpret_cast<const T*>(p.residual) + out_row * p.ldr + nb;
+    if (fullw) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint4 u = res.valid ? res.u[q] : *reinterpret_cast<const uint4*>(rr + q * 8);
+        const Vec<T, 8> h = *reinterpret_cast<const Vec<T, 8>*>(&u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[q * 8 + j] += to_f32(h.v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (nb + j < p.N) f[j] += to_f32(rr[j]);
+    }
+  }
+  store_row_chunk<T>(static_cast<T*>(p.C) + out_row * p.ldc + nb, f, fullw, p.N - nb);
+}
+// The same through the transposing stage, for rows that are not 16-byte aligned.
+template <class T>
+__device__ __forceinline__ void store_chunk_act_ragged(const GemmParams& p, const float (&f)[32], int row0, int nb, const float* sbias,
+                                                       float* turn, int lane) {
+  __syncwarp();   // the previous chunk has been stored
+#pragma unroll
+  for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = f[j];
+  __syncwarp();
+  const int col = nb + lane;
+  if (col >= p.N) return;
+  const float b = sbias ? sbias[lane] : 0.f;
+  const int rows = min(32, p.M - row0);
+  with_act(p.act, [&](auto act) {
+    for (int r = 0; r < rows; ++r) {
+      float v = turn[r * 33 + lane] + b;
+      const long long m = row0 + r;
+      if (p.pre) static_cast<T*>(p.pre)[m * p.ldp + col] = from_f32<T>(v);
+      v = act_value<decltype(act)::value>(v);
+      if (p.residual) v += to_f32(reinterpret_cast<const T*>(p.residual)[m * p.ldr + col]);
+      static_cast<T*>(p.C)[m * p.ldc + col] = from_f32<T>(v);
+    }
+  });
+}
+
 // Accumulators of one tile.  The tensor core truncates its fp32 sums, by an amount that follows the sum's size and the
 // number of additions to it.  The split-operand product therefore adds its two small products (hi*lo and lo*hi, 2^-11
 // of hi*hi) to an accumulator of their own, and hi*hi, where the tile is narrow enough, to three over successive parts of
@@ -294,10 +388,13 @@ __host__ __device__ inline int acc_sets(int parts, int bn) { return parts == 1 ?
 // kSplit: the K loop is split over the CTAs of a cluster (p.split of them); a separate
 // instantiation, so that each variant carries only its own epilogue (and its registers).
 // kTwo: operands in two fp16 parts (p.parts == 2); likewise separate.
-template <bool kConv, bool kPair, bool kSplit, bool kTwo>
+// kLin: linear layers with an activation, of fp16 (1) or bf16 (2) operands; 0 everywhere else.
+template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin = 0>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid_constant__ GemmParams p) {
   static_assert(!(kPair && kSplit), "a CTA pair walks the whole K range");
   static_assert(!(kConv && kTwo), "convolutions have fp16 operands");
+  static_assert(!kLin || !(kConv || kTwo), "an epilogue of plain products");
+  using LinT = std::conditional_t<kLin == 2, __nv_bfloat16, __half>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -468,6 +565,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
                   load_5d(dst, src, c0, par, x0 + xoff, r_src, img);
                 }
               }
+            } else if (kLin && p.a_mn) {
+              // A[K,M]: one 64(m) x 64(k) box per 64 rows of the tile
+              for (int j = 0; j < kBM / 64; ++j) load_2d(a_dst + j * 8192, &p.a_map[0], tm * kBM + j * 64, kb * kBK);
             } else {
               load_2d(a_dst, &p.a_map[0], kb * kBK, tm * kBM);
               if (parts == 2) load_2d(a_dst + kABytes, &p.a_map[1], kb * kBK, tm * kBM);
@@ -505,7 +605,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
     if (kPair && crank != 0) {
       // odd CTA of a pair: the leader issues the MMAs for both
     } else if (elect_one()) {
-      const uint32_t idesc = make_idesc_f16(kBM * kWidth, BN, 0, (!kConv && p.b_kn) ? 1 : 0);
+      const bool a_mn = kLin && p.a_mn;
+      const uint32_t idesc = make_idesc_f16(kBM * kWidth, BN, a_mn ? 1 : 0, (!kConv && p.b_kn) ? 1 : 0) | (kLin == 2 ? kIdescBf16 : 0u);
+      const uint32_t a_step = a_mn ? 128u : 2u;   // kUmmaK further along K, in 16-byte units: 16 rows of 128 bytes, or 32 bytes of a row
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
@@ -528,7 +630,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
           tc_fence_after_sync();
           const uint32_t a_addr = smem_base + stage * stage_bytes;
           const uint32_t b_addr = a_addr + parts * kABytes;
-          const uint64_t adesc = make_smem_desc_sw128(a_addr, 16, 1024);
+          // MN-major A: two 64-row halves 8 KB apart (LBO), 8-deep k-groups 1 KB apart (SBO)
+          const uint64_t adesc = make_smem_desc_sw128(a_addr, a_mn ? 8192 : 16, 1024);
           const uint32_t first = (kb == kb_begin) ? 0u : 1u;
           if (!kConv && p.b_kn) {
             // MN-major B: 64-column chunks 8 KB apart (LBO), 8-row k-groups 1 KB apart (SBO)
@@ -546,16 +649,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
               const uint32_t add = t == 0 ? fresh : t == 1 ? first : 1u;
 #pragma unroll
               for (int k = 0; k < kBK / kUmmaK; ++k) {
-                if (kPair) umma_f16_pair(d, ad + 2u * k, bd + 128u * k, idesc, add | k);
-                else umma_f16(d, ad + 2u * k, bd + 128u * k, idesc, add | k);
+                if (kPair) umma_f16_pair(d, ad + a_step * k, bd + 128u * k, idesc, add | k);
+                else umma_f16(d, ad + a_step * k, bd + 128u * k, idesc, add | k);
               }
             }
           } else {
             const uint64_t bdesc = make_smem_desc_sw128(b_addr, 16, 1024);
 #pragma unroll
             for (int k = 0; k < kBK / kUmmaK; ++k) {
-              if (kPair) umma_f16_pair(d_tmem, adesc + 2u * k, bdesc + 2u * k, idesc, first | k);
-              else umma_f16(d_tmem, adesc + 2u * k, bdesc + 2u * k, idesc, first | k);
+              if (kPair) umma_f16_pair(d_tmem, adesc + a_step * k, bdesc + 2u * k, idesc, first | k);
+              else umma_f16(d_tmem, adesc + a_step * k, bdesc + 2u * k, idesc, first | k);
             }
           }
           // frees the stage (in both CTAs of a pair) once these MMAs have read it
@@ -619,7 +722,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
           float b = 0.f, cs = 0.f;
           if (n0 + j < p.N) {
             if (p.bias_f32) b += p.bias_f32[n0 + j];
-            else if (p.bias) b += __half2float(p.bias[n0 + j]);
+            else if (p.bias) b += to_f32(reinterpret_cast<const LinT*>(p.bias)[n0 + j]);
             if (kConv && p.bias_rows && img < p.cB) b += __half2float(p.bias_rows[static_cast<long long>(img) * p.ld_bias_rows + n0 + j]);
             if (has_ln) cs = p.ln_colsum[n0 + j];
           }
@@ -681,12 +784,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
             float f[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-            store_chunk_ragged(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
+            if constexpr (kLin != 0)
+              store_chunk_act_ragged<LinT>(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
+            else store_chunk_ragged(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
           } else if (out_row >= 0 && nb < p.N) {
             float f[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-            store_chunk<kConv>(p, f, out_row, nb, img, has_bias ? s_bias + c * 32 : nullptr, res_cur,
+            if constexpr (kLin != 0) store_chunk_act<LinT>(p, f, out_row, nb, has_bias ? s_bias + c * 32 : nullptr, res_cur);
+            else store_chunk<kConv>(p, f, out_row, nb, img, has_bias ? s_bias + c * 32 : nullptr, res_cur,
                                has_ln ? s_colsum + c * 32 : nullptr, ln, stat);
           }
           res_cur = res_next;
@@ -749,7 +855,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
             }
           }
           const int nb = n0 + c * 32;
-          if (!kConv && p.ragged)
+          if constexpr (kLin != 0) {
+            if (p.ragged)
+              store_chunk_act_ragged<LinT>(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
+            else if (out_row >= 0 && nb < p.N) store_chunk_act<LinT>(p, f, out_row, nb, has_bias ? s_bias + c * 32 : nullptr, res_cur);
+          } else if (!kConv && p.ragged)
             store_chunk_ragged(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
           else if (out_row >= 0 && nb < p.N)
             store_chunk<kConv>(p, f, out_row, nb, img, has_bias ? s_bias + c * 32 : nullptr, res_cur,
@@ -868,7 +978,7 @@ static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int fo
   return best;
 }
 
-template <bool kConv, bool kPair, bool kSplit, bool kTwo>
+template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin>
 static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   const int b_rows = kPair ? p.bn / 2 : p.bn;
   const int smem = p.stages * p.parts * (kABytes + b_rows * 128) + recv_bytes(p.bn, kSplit ? p.split : 1) + kSmemMisc +
@@ -877,7 +987,7 @@ static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(gemm_conv_kernel<kConv, kPair, kSplit, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget),
+    if (int rc = check_cuda(cudaFuncSetAttribute(gemm_conv_kernel<kConv, kPair, kSplit, kTwo, kLin>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget),
                             "cudaFuncSetAttribute(gemm)"))
       return rc;
     configured[dev] = true;
@@ -889,16 +999,16 @@ static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   int clusters = p.clusters;
   if (clusters > num_units) clusters = num_units;
   if (clusters < 1) clusters = 1;
-  return launch_kernel("gemm_conv_kernel launch", gemm_conv_kernel<kConv, kPair, kSplit, kTwo>, dim3(clusters * width), dim3(kGemmThreads), smem,
+  return launch_kernel("gemm_conv_kernel launch", gemm_conv_kernel<kConv, kPair, kSplit, kTwo, kLin>, dim3(clusters * width), dim3(kGemmThreads), smem,
                        stream, width, p);
 }
 
 // tiles_m: 128-row tiles along M; tiles_n: tiles along N
-template <bool kConv, bool kTwo = false>
+template <bool kConv, bool kTwo = false, int kLin = 0>
 static int launch(const GemmParams& p, int tiles_m, int tiles_n, cudaStream_t stream) {
-  if (p.pair) return launch_one<kConv, true, false, kTwo>(p, ((tiles_m + 1) / 2) * tiles_n, stream);
-  if (p.split > 1) return launch_one<kConv, false, true, kTwo>(p, tiles_m * tiles_n, stream);
-  return launch_one<kConv, false, false, kTwo>(p, tiles_m * tiles_n, stream);
+  if (p.pair) return launch_one<kConv, true, false, kTwo, kLin>(p, ((tiles_m + 1) / 2) * tiles_n, stream);
+  if (p.split > 1) return launch_one<kConv, false, true, kTwo, kLin>(p, tiles_m * tiles_n, stream);
+  return launch_one<kConv, false, false, kTwo, kLin>(p, tiles_m * tiles_n, stream);
 }
 
 static int aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -1077,6 +1187,52 @@ extern "C" int bxl_gemm_ragged_f16(const void* A, long long lda, const void* B, 
   p.dev_status = st;
   return launch<false>(p, tiles_m, (N + tc.bn - 1) / tc.bn, s);
 }
+
+// ---- linear layers with an activation (entry points in linear.cu) --------------------
+namespace bxl {
+int repack_rows(const RowCopy& a, const RowCopy& b, cudaStream_t s) {
+  const long long vecs = (a.dst ? a.rows * (a.ld_dst / 8) : 0) + (b.dst ? b.rows * (b.ld_dst / 8) : 0);
+  if (vecs <= 0) return kOk;
+  const long long blocks = (vecs + 255) / 256, most = sm_count() * 8;
+  const RepackOperand oa{static_cast<const __half*>(a.src), static_cast<__half*>(a.dst), a.ld, a.ld_dst, a.rows, a.cols};
+  const RepackOperand ob{static_cast<const __half*>(b.src), static_cast<__half*>(b.dst), b.ld, b.ld_dst, b.rows, b.cols};
+  return launch_kernel("repack_rows_kernel launch", repack_rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, oa, ob);
+}
+
+int linear_product(const LinearProduct& q, cudaStream_t stream) {
+  int* st = device_status_ptr();
+  if (!st) return fail(kErrCuda, "linear layer: no device status word");
+  GemmParams p;
+  memset(&p, 0, sizeof(p));
+  auto rows16 = [](const void* base, long long ld) { return aligned16(base) && ld % 8 == 0; };
+  const bool ragged = q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && !rows16(q.residual, q.ldr)) || (q.pre && !rows16(q.pre, q.ldp));
+  const int tiles_m = (int)(((long long)q.M + kBM - 1) / kBM);
+  const TileConfig tc = choose_tiles(tiles_m, q.N, (int)(((long long)q.K + kBK - 1) / kBK), q.b_kn != 0, g_force_bn, g_force_split, g_force_pair < 0 ? kDefaultPair : g_force_pair,
+                                     0.0, ragged ? kSmemRaggedExtra : 0, 1, ragged || q.residual || q.pre);
+  {
+    // [M,K], or [K,M] in boxes of 64 by 64
+    uint64_t dims[2] = {(uint64_t)(q.a_mn ? q.M : q.K), (uint64_t)(q.a_mn ? q.K : q.M)};
+    uint64_t str[1] = {(uint64_t)q.lda * 2};
+    uint32_t box[2] = {kBK, (uint32_t)(q.a_mn ? kBK : kBM)};
+    if (int rc = encode_tmap_f16(&p.a_map[0], q.A, 2, dims, str, box)) return rc;
+  }
+  {
+    uint64_t dims[2] = {(uint64_t)(q.b_kn ? q.N : q.K), (uint64_t)(q.b_kn ? q.K : q.N)};
+    uint64_t str[1] = {(uint64_t)q.ldb * 2};
+    uint32_t box[2] = {kBK, (uint32_t)(q.b_kn ? kBK : tc.pair ? tc.bn / 2 : tc.bn)};
+    if (int rc = encode_tmap_f16(&p.b_map[0], q.B, 2, dims, str, box)) return rc;
+  }
+  p.M = q.M, p.N = q.N, p.K = q.K, p.parts = 1, p.b_kn = q.b_kn, p.a_mn = q.a_mn;
+  p.bn = tc.bn, p.split = tc.split, p.stages = tc.stages, p.pair = tc.pair, p.clusters = tc.clusters;
+  p.b_static = (static_weights() && q.b_is_weight) ? 1 : 0;
+  p.n_fastest = linear_tile_order(q.M, q.N, q.K, tc.bn);
+  p.bias = static_cast<const __half*>(q.bias), p.residual = static_cast<const __half*>(q.residual), p.ldr = q.ldr;
+  p.C = q.C, p.ldc = q.ldc, p.pre = q.pre, p.ldp = q.ldp, p.act = q.act, p.ragged = ragged ? 1 : 0;
+  p.dev_status = st;
+  const int tiles_n = (q.N + tc.bn - 1) / tc.bn;
+  return q.bf16 ? launch<false, false, 2>(p, tiles_m, tiles_n, stream) : launch<false, false, 1>(p, tiles_m, tiles_n, stream);
+}
+}  // namespace bxl
 
 extern "C" int bxl_gemm_dual_f16(const void* A, long long lda, const void* B, long long ldb, const void* bias, void* C1,
                                  long long ldc1, int n1, void* C2, long long ldc2, int M, int N, int K, void* stream) {

@@ -33,6 +33,22 @@ def _f16_cuda(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: expected a CUDA fp16 tensor, got {t.device} {t.dtype}")
 
 
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # BXL_F16, BXL_BF16, BXL_F32
+
+
+def _on_current_device(name: str, *tensors) -> None:
+    """The kernels run on the current device's current stream: every operand has to live there."""
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == torch.cuda.current_device()):
+            raise ValueError(f"{name}: expected tensors of the current CUDA device, got {t.device}")
+
+
+def _rows(t):
+    """``t`` as a matrix of rows with unit-stride columns (a view where its strides allow one)."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return t2 if t2.shape[1] == 1 or t2.stride(1) == 1 else t2.contiguous()
+
+
 # --------------------------------------------------------------------------- matmul
 def gemm(a, b, bias=None, residual=None, out=None, b_is_kn=False, out_f32=False):
     """``a[M,K] @ B`` with ``b`` given as [N,K] (default) or [K,N] (``b_is_kn``)."""
@@ -250,6 +266,76 @@ def gemm_split_f32(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# BXL_ACT_*; gelu takes erf, gelu_tanh its tanh form, quick_gelu is z sigmoid(1.702 z)
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "quick_gelu": 5}
+
+
+def _linear_operands(name, x, weight, activation, like_y):
+    """Checked operands: ``x`` and the ``[..., N]`` tensors of ``like_y`` (or None) as matrices of rows."""
+    _on_current_device(name, x, weight, *like_y)
+    _req(x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1 and weight.dim() == 2, f"{name}: fp16 or bf16 x [..., K] and weight [N, K]")
+    _req(weight.dtype == x.dtype and weight.shape[1] == x.shape[-1] and weight.numel() > 0, f"{name}: weight must be [N, K] in the type of x")
+    _req(activation in ACTIVATIONS, f"{name}: unknown activation {activation!r}")
+    shape = (*x.shape[:-1], weight.shape[0])
+    for t in like_y:
+        _req(t is None or (t.shape == shape and t.dtype == x.dtype), f"{name}: expected {list(shape)} in the type of x")
+    return _rows(x), _rows(weight), [None if t is None else _rows(t) for t in like_y]
+
+
+def linear_act(x, weight, bias=None, activation=None, residual=None, out=None, want_pre: bool = False):
+    """``act(x[..., K] @ weight[N, K]^T + bias) + residual`` in one product, fp16 or bf16, any extents; ``activation`` is one of
+    ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``) receives the result.  ``want_pre`` also returns the value
+    before the activation, rounded to the type of ``x``: the input of :func:`linear_act_bwd`."""
+    x2, w2, (r2,) = _linear_operands("linear_act", x, weight, activation, (residual,))
+    _on_current_device("linear_act", bias, out)
+    (m, k), n = x2.shape, w2.shape[0]
+    _req(bias is None or (bias.shape == (n,) and bias.dtype == x.dtype and bias.is_contiguous()), "linear_act: bias must be a contiguous [N] vector in the type of x")
+    shape = (*x.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+    _req(out.shape == shape and out.dtype == x.dtype and out.is_contiguous(), "linear_act: out must be contiguous, [..., N] in the type of x")
+    pre = torch.empty(shape, device=x.device, dtype=x.dtype) if want_pre else None
+    if m:
+        l = _lib.lib()
+        args = _lib.LinearArgs(_p(x2), x2.stride(0), _p(w2), w2.stride(0), _p(bias), _p(r2), 0 if r2 is None else r2.stride(0), _p(out), n, _p(pre), n)
+        args.M, args.N, args.K, args.dtype, args.act = m, n, k, _TYPES[x.dtype], ACTIVATIONS[activation]
+        nbytes = l.bxl_linear_act_fwd_workspace_bytes(C.byref(args))
+        if nbytes:
+            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            args.workspace, args.workspace_bytes = _p(ws), nbytes
+        count = C.c_int(0)
+        rc = l.bxl_linear_act_fwd(C.byref(args), C.byref(count), _stream())
+        _lib.check(rc, l, kernels=count.value)
+    return (out, pre) if want_pre else out
+
+
+def linear_act_bwd(dy, x, weight, pre=None, activation=None, want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`linear_act`, given that of its result and, where it has an activation, the
+    ``pre`` it returned; ``None`` for those that are not wanted.  The gradient of its residual is ``dy`` itself.  All have
+    the type of ``x``; sums are fp32, ``dy * act'(pre)`` is rounded to that type between the products."""
+    x2, w2, (dy2, pre2) = _linear_operands("linear_act_bwd", x, weight, activation, (dy, pre))
+    act = ACTIVATIONS[activation]
+    _req(act == 0 or pre is not None, "linear_act_bwd: an activation needs the value before it (pre)")
+    (m, k), n = x2.shape, w2.shape[0]
+    new = torch.empty if m else torch.zeros
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_dx else None
+    dweight = new((n, k), device=x.device, dtype=x.dtype) if want_dweight else None
+    dbias = new(n, device=x.device, dtype=x.dtype) if want_dbias else None
+    if m and (want_dx or want_dweight or want_dbias):
+        l = _lib.lib()
+        args = _lib.LinearArgs(_p(x2), x2.stride(0), _p(w2), w2.stride(0), None, None, 0, None, 0, _p(pre2), 0 if pre2 is None else pre2.stride(0),
+                               _p(dy2), dy2.stride(0), _p(dx), k, _p(dweight), k, _p(dbias))
+        args.M, args.N, args.K, args.dtype, args.act = m, n, k, _TYPES[x.dtype], act
+        nbytes = l.bxl_linear_act_bwd_workspace_bytes(C.byref(args))
+        if nbytes:
+            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+            args.workspace, args.workspace_bytes = _p(ws), nbytes
+        count = C.c_int(0)
+        rc = l.bxl_linear_act_bwd(C.byref(args), C.byref(count), _stream())
+        _lib.check(rc, l, kernels=count.value)
+    return dx, dweight, dbias
+
+
 # --------------------------------------------------------------------------- convolution
 def conv_weight_pack(w_oihw: torch.Tensor) -> torch.Tensor:
     _f16_cuda(w_oihw, "weight")
@@ -457,6 +543,72 @@ def layernorm(x, gamma, beta, eps):
     l = _lib.lib()
     _lib.check(l.bxl_layernorm_f16(_p(x), _p(out), _p(gamma), _p(beta), x.numel() // Ci, Ci, float(eps), _stream()), l)
     return out
+
+
+def _norm_operands(name, x, weight, bias, *like_x):
+    _on_current_device(name, x, weight, bias, *like_x)
+    _req(x.dtype in _TYPES and x.dim() >= 1 and x.shape[-1] >= 1, f"{name}: fp16, bf16 or fp32 rows of at least one element")
+    for t in like_x:
+        _req(t.shape == x.shape and t.dtype == x.dtype, f"{name}: dy must have the shape and type of x")
+    pt = x.dtype
+    for t in (weight, bias):
+        if t is not None:
+            pt = t.dtype
+            _req(t.shape == x.shape[-1:] and t.is_contiguous() and pt in (x.dtype, torch.float32),
+                 f"{name}: weight and bias must be contiguous [C] vectors in the type of x or in fp32")
+    _req(weight is None or bias is None or weight.dtype == bias.dtype, f"{name}: weight and bias must share a type")
+    return pt
+
+
+def layernorm_fwd(x, weight=None, bias=None, eps: float = 1e-5, out=None, want_stats: bool = False):
+    """LayerNorm over the last axis of ``x`` (fp16, bf16 or fp32, any width); ``weight`` and ``bias`` in its type or in
+    fp32, either may be absent.  ``out`` (which may be ``x``) receives the result.  ``want_stats`` also returns the
+    rows' fp32 ``mean`` and ``rstd``, the input of :func:`layernorm_bwd`."""
+    pt = _norm_operands("layernorm_fwd", x, weight, bias)
+    c = x.shape[-1]
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    else:
+        _on_current_device("layernorm_fwd", out)
+        _req(out.shape == x.shape and out.dtype == x.dtype and out.is_contiguous(), "layernorm_fwd: out must be contiguous, in the shape and type of x")
+    rows = x.numel() // c
+    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32) if want_stats else None
+    if rows:
+        x2 = _rows(x)
+        l = _lib.lib()
+        _lib.check(
+            l.bxl_layernorm_fwd(_p(x2), x2.stride(0), _p(weight), _p(bias), _p(out), c, _p(stats), stats.data_ptr() + 4 * rows if want_stats else None,
+                                rows, c, _TYPES[x.dtype], _TYPES[pt], float(eps), _stream()),
+            l,
+        )
+    return (out, stats[0], stats[1]) if want_stats else out
+
+
+def layernorm_bwd(dy, x, mean, rstd, weight=None, want_dweight: bool = True, want_dbias: bool = True):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`layernorm_fwd`, given that of its result and the ``mean`` and ``rstd``
+    it returned.  ``dweight`` and ``dbias`` have the type of ``weight`` (that of ``x`` without one) and are ``None`` where
+    they are not wanted; ``dweight`` is ``None`` without a ``weight``."""
+    pt = _norm_operands("layernorm_bwd", x, weight, None, dy)
+    _on_current_device("layernorm_bwd", mean, rstd)
+    for t in (mean, rstd):
+        _req(t.dtype == torch.float32 and t.shape == x.shape[:-1] and t.is_contiguous(), "layernorm_bwd: mean and rstd must be contiguous fp32, one value per row of x")
+    c = x.shape[-1]
+    rows = x.numel() // c
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    new = torch.empty if rows else torch.zeros
+    dweight = new(c, device=x.device, dtype=pt) if want_dweight and weight is not None else None
+    dbias = new(c, device=x.device, dtype=pt) if want_dbias else None
+    if rows:
+        dy2, x2 = _rows(dy), _rows(x)
+        l = _lib.lib()
+        params = dweight is not None or dbias is not None
+        ws = torch.empty(l.bxl_layernorm_bwd_workspace_bytes(rows, c), device=x.device, dtype=torch.uint8) if params else None
+        _lib.check(
+            l.bxl_layernorm_bwd(_p(dy2), dy2.stride(0), _p(x2), x2.stride(0), _p(mean), _p(rstd), _p(weight), _p(dx), c, _p(dweight), _p(dbias),
+                                rows, c, _TYPES[x.dtype], _TYPES[pt], _p(ws), ws.numel() if params else 0, _stream()),
+            l, kernels=2 if params else 1,
+        )
+    return dx, dweight, dbias
 
 
 def geglu(h):

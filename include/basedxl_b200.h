@@ -24,6 +24,9 @@
 extern "C" {
 #endif
 
+/* Element types of the entry points that take more than fp16 (`dtype`, `param_dtype`). */
+enum { BXL_F16 = 0, BXL_BF16 = 1, BXL_F32 = 2 };
+
 /* ---- library ------------------------------------------------------------ */
 
 /* Sets up the per-device status word and the TMA descriptor encoder for the
@@ -158,6 +161,37 @@ long long bxl_gemm_ragged_workspace_bytes(int M, int N, int K);
 int bxl_gemm_ragged_f16(const void* A, long long lda, const void* B, long long ldb, const void* bias, const void* residual,
                         long long ldr, void* C, long long ldc, int M, int N, int K, void* workspace, long long workspace_bytes,
                         void* stream);
+
+/* Linear layer with bias, activation and residual, fp16 or bf16 (`dtype`), accumulated in fp32:
+ *   forward:  z = x W^T + bias, y = act(z) + residual; z is also stored (rounded to `dtype`) where `pre` is set
+ *   backward: dz = dy act'(z), dx = dz W, dweight = dz^T x, dbias = sum over rows of dz; results whose pointers are NULL
+ *             are not formed.  The residual's gradient is dy itself.
+ * x [M,K], weight [N,K], bias [N], residual, y, pre, dy [M,N]; any alignment that suits the element, rows any distance apart
+ * (written ones apart).  Operands of the tensor cores that the copy engine cannot read (rows not 16-byte aligned) are first
+ * copied to the workspace.  dz is rounded to `dtype` between its two products; sums have a fixed order.
+ * Written operands overlap nothing else of the call, except that y may be the residual.
+ * bxl_linear_act_*_workspace_bytes reads all fields but the workspace.  *launches (or NULL): kernels enqueued.
+ * The forward pass replaces bxl_gemm_f16 and the activation around it; no counterpart of the backward pass in the
+ * reference, which only runs inference. */
+enum { BXL_ACT_NONE = 0, BXL_ACT_RELU = 1, BXL_ACT_SILU = 2, BXL_ACT_GELU = 3 /* erf */, BXL_ACT_GELU_TANH = 4, BXL_ACT_QUICK_GELU = 5 };
+typedef struct bxl_linear_args {
+  const void* x; long long ldx;
+  const void* weight; long long ldw;
+  const void* bias;
+  const void* residual; long long ldr;
+  void* y; long long ldy;
+  void* pre; long long ldp;
+  const void* dy; long long lddy;
+  void* dx; long long lddx;
+  void* dweight; long long lddw;
+  void* dbias;
+  void* workspace; long long workspace_bytes;
+  int M, N, K, dtype, act;
+} bxl_linear_args;
+long long bxl_linear_act_fwd_workspace_bytes(const bxl_linear_args* args);
+int bxl_linear_act_fwd(const bxl_linear_args* args, int* launches, void* stream);
+long long bxl_linear_act_bwd_workspace_bytes(const bxl_linear_args* args);
+int bxl_linear_act_bwd(const bxl_linear_args* args, int* launches, void* stream);
 
 /* ---- convolution ---------------------------------------------------------- */
 
@@ -308,6 +342,22 @@ int bxl_upsample2x_f16(const void* x, void* y, int B, int H, int W, int C, void*
 /* LayerNorm over the last axis of x[rows,C]. */
 int bxl_layernorm_f16(const void* x, void* y, const void* gamma, const void* beta, long long rows, int C, float eps,
                       void* stream);
+/* LayerNorm over the last axis with any row length C >= 1, and what its backward pass needs:
+ *   mean = sum(x) / C, rstd = 1 / sqrt(sum((x - mean)^2) / C + eps), y = (x - mean) rstd weight + bias.
+ * x, y: rows ldx / ldy elements apart, of type `dtype`; weight, bias [C] of type `param_dtype`, which is `dtype` or BXL_F32;
+ * either may be NULL (1 and 0).  mean, rstd: [rows] fp32, both or neither.  y may be x.  Any alignment that suits the
+ * element; rows of whole 16-byte vectors at 16-byte aligned addresses are read as such.
+ * No counterpart in the reference (its LayerNorms are the host UNet's, for inference). */
+int bxl_layernorm_fwd(const void* x, long long ldx, const void* weight, const void* bias, void* y, long long ldy, float* mean,
+                      float* rstd, long long rows, int C, int dtype, int param_dtype, float eps, void* stream);
+/* Its gradients, given those of y: with h = (x - mean) rstd and g = dy weight,
+ *   dx = rstd (g - mean(g) - h mean(g h)),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
+ * dweight, dbias [C] of type `param_dtype`, either may be NULL; with both NULL the workspace may be too.  The sums are
+ * formed in fp32 in a fixed order: the same call gives the same bits.  dx overlaps neither x nor dy. */
+long long bxl_layernorm_bwd_workspace_bytes(long long rows, int C);
+int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
+                      const void* weight, void* dx, long long lddx, void* dweight, void* dbias, long long rows, int C, int dtype,
+                      int param_dtype, void* workspace, long long workspace_bytes, void* stream);
 /* out[rows,F] = h[:, :F] * gelu(h[:, F:]) for h[rows,2F] (exact erf GELU). */
 int bxl_geglu_f16(const void* h, void* out, long long rows, int F, void* stream);
 

@@ -1,0 +1,231 @@
+"""Refusals and launch arguments of the training operators, with the library replaced by a recorder (no GPU), and what the
+C entry points refuse before any CUDA call."""
+import ctypes as C
+
+import pytest
+import torch
+
+from basedxl_b200 import _lib, ops
+
+
+class _Recorder:
+    """Stands for the loaded library: remembers the launches."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name.endswith("_bytes"):
+            return lambda *a: 1024
+
+        def call(*args):
+            if name.startswith("bxl_linear"):
+                a = args[0]._obj
+                args = {f: getattr(a, f) for f, _ in a._fields_}
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    rec = _Recorder()
+    monkeypatch.setattr(_lib, "lib", lambda: rec)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+
+    def on_cpu(name, *tensors):
+        ops._req(all(t is None or t.device.type == "cpu" for t in tensors), f"{name}: another device")
+
+    monkeypatch.setattr(ops, "_on_current_device", on_cpu)
+    return rec
+
+
+def _z(*shape, dtype=torch.float16, device="cpu"):
+    return torch.zeros(*shape, dtype=dtype, device=device)
+
+
+META = {"device": "meta"}
+
+
+@pytest.mark.parametrize(
+    "kw",
+    [
+        {"x": _z(5, 8, dtype=torch.float64)},
+        {"x": _z(5, 8, dtype=torch.int32)},
+        {"x": _z(5, 0)},
+        {"x": torch.zeros((), dtype=torch.float16)},
+        {"x": _z(5, 8, **META)},
+        {"weight": _z(7)},
+        {"weight": _z(1, 8)},
+        {"weight": _z(16)[::2]},
+        {"weight": _z(8, dtype=torch.bfloat16)},
+        {"weight": _z(8, **META)},
+        {"bias": _z(9)},
+        {"bias": _z(8, dtype=torch.float32)},        # not the weight's type
+        {"out": _z(5, 9)},
+        {"out": _z(8, 5).t()},
+        {"out": _z(5, 8, dtype=torch.float32)},
+        {"out": _z(5, 8, **META)},
+    ],
+)
+def test_layernorm_fwd_refuses(recorder, kw):
+    args = {"x": _z(5, 8), "weight": _z(8), "bias": _z(8), **kw}
+    with pytest.raises(ValueError):
+        ops.layernorm_fwd(args.pop("x"), args.pop("weight"), args.pop("bias"), **args)
+    assert not recorder.calls
+
+
+@pytest.mark.parametrize(
+    "kw",
+    [
+        {"dy": _z(5, 9)},
+        {"dy": _z(8)},
+        {"dy": _z(5, 8, dtype=torch.float32)},
+        {"dy": _z(5, 8, **META)},
+        {"mean": _z(4, dtype=torch.float32)},
+        {"mean": _z(5)},
+        {"rstd": _z(10, dtype=torch.float32)[::2]},
+        {"rstd": _z(5, 1, dtype=torch.float32)},
+        {"mean": _z(5, dtype=torch.float32, **META)},
+        {"weight": _z(5)},
+        {"weight": _z(8, dtype=torch.bfloat16)},
+    ],
+)
+def test_layernorm_bwd_refuses(recorder, kw):
+    args = {"dy": _z(5, 8), "x": _z(5, 8), "mean": _z(5, dtype=torch.float32), "rstd": _z(5, dtype=torch.float32), "weight": _z(8), **kw}
+    with pytest.raises(ValueError):
+        ops.layernorm_bwd(**args)
+    assert not recorder.calls
+
+
+@pytest.mark.parametrize(
+    "kw",
+    [
+        {"x": _z(5, 8, dtype=torch.float32), "weight": _z(6, 8, dtype=torch.float32)},
+        {"x": _z(5, 8, dtype=torch.bfloat16)},
+        {"x": _z(5, 9)},
+        {"x": _z(5, 8, **META)},
+        {"weight": _z(8)},
+        {"weight": _z(0, 8)},
+        {"weight": _z(1, 6, 8)},
+        {"weight": _z(6, 8, **META)},
+        {"bias": _z(5)},
+        {"bias": _z(1, 6)},
+        {"bias": _z(12)[::2]},
+        {"bias": _z(6, dtype=torch.float32)},
+        {"bias": _z(6, **META)},
+        {"residual": _z(6)},
+        {"residual": _z(5, 6, dtype=torch.float32)},
+        {"residual": _z(5, 6, **META)},
+        {"activation": "swish"},
+        {"activation": 3},
+        {"out": _z(5, 7)},
+        {"out": _z(6, 5).t()},
+        {"out": _z(5, 6, dtype=torch.float32)},
+        {"out": _z(5, 6, **META)},
+    ],
+)
+def test_linear_act_refuses(recorder, kw):
+    with pytest.raises(ValueError):
+        ops.linear_act(**{"x": _z(5, 8), "weight": _z(6, 8), **kw})
+    assert not recorder.calls
+
+
+@pytest.mark.parametrize(
+    "kw",
+    [
+        {"pre": None},
+        {"pre": _z(5, 7)},
+        {"pre": _z(5, 6, dtype=torch.float32)},
+        {"pre": _z(5, 6, **META)},
+        {"dy": _z(5, 8)},
+        {"dy": _z(5, 6, dtype=torch.bfloat16)},
+        {"dy": _z(5, 6, **META)},
+        {"x": _z(4, 8)},
+        {"activation": "tanh"},
+    ],
+)
+def test_linear_act_bwd_refuses(recorder, kw):
+    with pytest.raises(ValueError):
+        ops.linear_act_bwd(**{"dy": _z(5, 6), "x": _z(5, 8), "weight": _z(6, 8), "pre": _z(5, 6), "activation": "gelu", **kw})
+    assert not recorder.calls
+
+
+def test_empty_batches_launch_nothing(recorder):
+    y, mean, rstd = ops.layernorm_fwd(_z(0, 8), _z(8), want_stats=True)
+    dx, dw, db = ops.layernorm_bwd(_z(0, 8), _z(0, 8), mean, rstd, _z(8))
+    assert y.shape == dx.shape == (0, 8) and mean.shape == (0,) and not dw.any() and not db.any()
+    y, pre = ops.linear_act(_z(2, 0, 8), _z(6, 8), want_pre=True)
+    dx, dw, db = ops.linear_act_bwd(_z(2, 0, 6), _z(2, 0, 8), _z(6, 8))
+    assert y.shape == pre.shape == (2, 0, 6) and dx.shape == (2, 0, 8) and not dw.any() and not db.any()
+    assert not recorder.calls
+
+
+def test_strides_reach_the_kernel(recorder):
+    """Rows any distance apart are passed on as they lie; columns that are not next to one another are copied first."""
+    ops.layernorm_fwd(_z(5, 20)[:, 3:11], _z(8), want_stats=True)
+    ops.layernorm_fwd(_z(8, 5).t())
+    ops.layernorm_bwd(_z(1, 8).expand(5, 8), _z(5, 9)[:, :8], _z(5, dtype=torch.float32), _z(5, dtype=torch.float32))
+    (_, a), (_, b), (_, c) = recorder.calls
+    assert (a[1], a[5], a[8:12]) == (20, 8, (5, 8, 0, 0)) and b[1] == 8 and (c[1], c[3], c[8], c[9]) == (0, 9, 8, None)
+    recorder.calls.clear()
+    ops.linear_act(_z(5, 20)[:, 3:11], _z(6, 8), residual=_z(1, 6).expand(5, 6), activation="silu")
+    ops.linear_act_bwd(_z(5, 7)[:, :6], _z(5, 8), _z(6, 12)[:, :8], pre=_z(5, 6), activation="gelu", want_dweight=False)
+    (_, a), (_, b) = recorder.calls
+    assert (a["ldx"], a["ldw"], a["ldr"], a["ldy"], a["M"], a["N"], a["K"], a["act"]) == (20, 8, 0, 6, 5, 6, 8, 2) and a["pre"] is None
+    assert (b["lddy"], b["ldw"], b["ldp"], b["lddx"], b["act"], b["dweight"]) == (7, 12, 6, 8, 3, None) and b["workspace_bytes"] == 1024
+
+
+# ---- the C entry points: refused before any CUDA call --------------------------------------------
+P = 0x1000  # stands for an address; nothing reads it
+
+
+def _norm_fwd(**kw):
+    a = {"x": P, "ldx": 64, "w": P, "b": P, "y": P, "ldy": 64, "mean": P, "rstd": P, "rows": 4, "C": 64, "dtype": 0, "pt": 0, "eps": 1e-5, **kw}
+    return _lib.load().bxl_layernorm_fwd(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw", [{"x": None}, {"y": None}, {"rows": 0}, {"rows": -1}, {"C": 0}, {"C": (1 << 30) + 1}, {"ldy": 63}, {"ldx": -1}, {"mean": None}, {"rstd": None},
+                                {"dtype": 3}, {"dtype": 2}, {"pt": 1}, {"eps": -1.0}, {"eps": float("nan")}, {"x": P + 1}, {"w": P + 1}, {"mean": P + 2}])
+def test_c_layernorm_fwd_refuses(kw):
+    assert _norm_fwd(**kw) < 0 and b"bxl_layernorm_fwd" in _lib.load().bxl_last_error()
+
+
+@pytest.mark.parametrize("kw", [{"dy": None}, {"x": None}, {"mean": None}, {"rstd": None}, {"dx": None}, {"rows": 0}, {"C": -8}, {"lddx": 8}, {"lddy": -64}, {"pt": 1},
+                                {"dtype": -1}, {"dw": P + 1}, {"dx": P + 1}, {"ws": None}, {"ws": P + 8}, {"ws_bytes": 16}])
+def test_c_layernorm_bwd_refuses(kw):
+    a = {"dy": P, "lddy": 64, "x": P, "ldx": 64, "mean": P, "rstd": P, "w": P, "dx": P, "lddx": 64, "dw": P, "db": P, "rows": 4, "C": 64, "dtype": 0, "pt": 0,
+         "ws": P, "ws_bytes": 1 << 20, **kw}
+    assert _lib.load().bxl_layernorm_bwd(*a.values(), None) < 0 and b"bxl_layernorm_bwd" in _lib.load().bxl_last_error()
+
+
+def _linear(**kw):
+    a = _lib.LinearArgs()
+    base = {"x": P, "ldx": 64, "weight": P, "ldw": 64, "y": P, "ldy": 64, "dy": P, "lddy": 64, "dx": P, "lddx": 64, "dweight": P, "lddw": 64, "dbias": P,
+            "M": 32, "N": 64, "K": 64, "dtype": 0, "act": 0, "workspace": P, "workspace_bytes": 1 << 20}
+    for k, v in {**base, **kw}.items():
+        setattr(a, k, v)
+    return C.byref(a)
+
+
+BOTH = [{"x": None}, {"weight": None}, {"M": 0}, {"N": -1}, {"K": 0}, {"M": (1 << 30) + 1}, {"dtype": 2}, {"dtype": 7}, {"act": 6}, {"act": -1}, {"x": P + 1}, {"bias": P + 1}, {"ldx": -1}]
+
+
+@pytest.mark.parametrize("kw", BOTH + [{"y": None}, {"ldy": 63}, {"pre": P, "ldp": 8}, {"ldx": 65, "workspace": None}, {"ldx": 65, "workspace_bytes": 64}])
+def test_c_linear_act_fwd_refuses(kw):
+    l = _lib.load()
+    assert l.bxl_linear_act_fwd(_linear(**kw), None, None) < 0 and b"bxl_linear_act_fwd" in l.bxl_last_error()
+
+
+@pytest.mark.parametrize("kw", BOTH + [{"dy": None}, {"act": 3}, {"lddx": 63}, {"lddw": 0}, {"lddy": -1}, {"workspace": None}, {"workspace": P + 4}, {"workspace_bytes": 8}])
+def test_c_linear_act_bwd_refuses(kw):
+    l = _lib.load()
+    assert l.bxl_linear_act_bwd(_linear(**kw), None, None) < 0 and b"bxl_linear_act_bwd" in l.bxl_last_error()
+
+
+@pytest.mark.parametrize("kw,nbytes", [({}, 0), ({"ldx": 68}, 32 * 64 * 2), ({"ldw": 65}, 64 * 64 * 2), ({"x": P + 2, "ldx": 0}, 32 * 64 * 2), ({"M": 8, "ldx": 65}, 0),
+                                       ({"K": 63}, 0), ({"K": 63, "ldx": 63}, 32 * 64 * 2)])
+def test_workspace_of_the_forward_pass(kw, nbytes):
+    """Copies only of operands whose rows are not 16-byte aligned, and none for a few rows."""
+    assert _lib.load().bxl_linear_act_fwd_workspace_bytes(_linear(**kw)) == nbytes
