@@ -58,7 +58,7 @@ SIGNATURES = {
     "bxl_gemm_ragged_workspace_bytes": (_ll, [_i, _i, _i]),
     "bxl_gemm_ragged_f16": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _ll, _vp, _ll, _i, _i, _i, _vp, _ll, _vp]),
     "bxl_linear_act_fwd_workspace_bytes": (_ll, [C.POINTER(LinearArgs)]),
-    "bxl_linear_act_fwd": (_i, [C.POINTER(LinearArgs), C.POINTER(_i), _vp]),
+    "bxl_linear_act_fwd": (_i, [C.POINTER(LinearArgs), _vp]),
     "bxl_linear_act_bwd_workspace_bytes": (_ll, [C.POINTER(LinearArgs)]),
     "bxl_linear_act_bwd": (_i, [C.POINTER(LinearArgs), C.POINTER(_i), _vp]),
     "bxl_conv_weight_pack_f16": (_i, [_vp, _vp, _i, _i, _vp]),
@@ -119,6 +119,8 @@ def lib() -> C.CDLL:
     """The loaded library, initialised for the current CUDA device."""
     import torch
 
+    if _inited_devices and torch._C._cuda_getDevice() in _inited_devices:
+        return _lib
     l = load()
     if not torch.cuda.is_available():
         raise BxlError("basedxl_b200 needs a CUDA device (sm_100a); none is available and there is no CPU path")

@@ -4,11 +4,14 @@
 //   backward  h = (x - m) r,  g = dy w:  dx = r (g - mean(g) - h mean(g h)),
 //             dw = sum over rows of dy h,  db = sum over rows of dy
 //
-// Bound by memory: the forward pass reads x and writes y once, the backward pass reads dy and x and writes dx once.  A row
-// therefore stays in registers (as loaded, not widened) between its reduction and its result: one warp holds a short
-// row, a block a long one, and only rows longer than a block's registers are read again.  Sums are fp32; the variance is
-// taken of the differences from the mean.  dw and db: every thread keeps the sums of its own columns over all rows that it
-// meets, a block adds those of its warps, and a second launch adds the blocks' in a fixed order (no atomics).
+// Memory bounds it in principle: the forward pass reads x and writes y once, the backward pass reads dy and x and writes dx
+// once.  At 8 bytes a cycle and SM and 16-bit values that leaves some 20 (forward) and 30 (backward) instructions for a
+// value, so issue slots come close: arithmetic is on pairs (F2), and a value is widened once and kept.  Sums are fp32; the
+// variance is taken of the differences from the mean.  dw and db: every thread keeps the sums of its own columns over
+// all rows that it meets, a block adds those of its threads, and a second launch adds the blocks' in a fixed order (no
+// atomics).
+#include <stdlib.h>
+
 #include "bxl_common.cuh"
 #include "bxl_host.h"
 #include "bxl_types.cuh"
@@ -36,73 +39,101 @@ __device__ __forceinline__ float warp_sum(float v) {
 // so that one barrier each is enough.
 __device__ __forceinline__ float block_sum(float v, float* slot) {
   v = warp_sum(v);
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (lane == 0) slot[threadIdx.x >> 5] = v;
   __syncthreads();
-  return warp_sum(lane < static_cast<int>(blockDim.x >> 5) ? slot[lane] : 0.f);
+  if (warps > 4) return warp_sum(lane < warps ? slot[lane] : 0.f);
+  v = slot[0];
+  for (int i = 1; i < warps; ++i) v += slot[i];
+  return v;
 }
-
-constexpr int kLnWarps = 8;   // rows in flight in a block of the warp-per-row form
-
-// kWarp: a warp per row, kLnWarps rows per block.  Otherwise a block per row.  NV vectors of VEC elements per thread.
-template <class T, int VEC, int NV, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? kLnWarps * 32 : 1024) ln_fwd_kernel(const LnArgs a) {
-  pdl_launch_dependents();
-  __shared__ float red[2][32];
-  const int tid = kWarp ? (threadIdx.x & 31) : threadIdx.x;
-  const int step = kWarp ? 32 : blockDim.x;
-  const int n = a.C / VEC;
-  const Param<T> w{a.weight, a.param_f32}, b{a.bias, a.param_f32};
-  const long long first = kWarp ? blockIdx.x * (long long)kLnWarps + (threadIdx.x >> 5) : blockIdx.x;
-  const long long stride = kWarp ? gridDim.x * (long long)kLnWarps : gridDim.x;
-  pdl_wait();
-  for (long long r = first; r < a.rows; r += stride) {
-    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
-    Vec<T, VEC> raw[NV];
+// Sum over LANES neighbouring lanes (8, 16 or 32), or over the block (0).
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* slot) {
+  if constexpr (LANES == 0) {
+    return block_sum(v, slot);
+  } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * step < n) raw[i] = load_vec<T, VEC>(xr + (tid + i * step) * VEC);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * step < n) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += to_f32(raw[i].v[j]);
-      }
-    const float mean = (kWarp ? warp_sum(s) : block_sum(s, red[0])) / a.C;   // a division: the mean of equal values is their value
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * step < n) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = to_f32(raw[i].v[j]) - mean;
-          q = fmaf(d, d, q);
-        }
-      }
-    const float rstd = rsqrtf((kWarp ? warp_sum(q) : block_sum(q, red[1])) * a.inv_c + a.eps);
-    T* yr = static_cast<T*>(a.y) + r * a.ldy;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (tid + i * step) * VEC;
-      if (tid + i * step < n) {
-        float wv[VEC], bv[VEC];
-        if (w.p) w.template get<VEC>(c, wv);
-        if (b.p) b.template get<VEC>(c, bv);
-        Vec<T, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float h = (to_f32(raw[i].v[j]) - mean) * rstd;
-          o.v[j] = from_f32<T>(fmaf(h, w.p ? wv[j] : 1.f, b.p ? bv[j] : 0.f));
-        }
-        store_vec<T, VEC>(yr + c, o);
-      }
-    }
-    if (a.mean && tid == 0) a.mean[r] = mean, a.rstd[r] = rstd;
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   }
 }
 
-// Rows longer than a block's registers: three passes over the row, the second and third mostly from L2.
+// ---- forward: a row in registers -------------------------------------------------------------
+// LANES lanes per row (0: a block per row), NV vectors of VEC elements each.  The next row is on its way while the present
+// one is reduced.
+constexpr int kLnWarps = 8;   // warps of a block that holds several rows
+template <class T, int VEC, int NV, int LANES, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) ln_fwd_kernel(const LnArgs a) {
+  pdl_launch_dependents();
+  using F = typename Lanes<VEC>::F;
+  constexpr int N = Lanes<VEC>::N;
+  __shared__ float red[2][32];
+  constexpr int kRows = LANES ? kLnWarps * 32 / LANES : 1;   // rows of a block
+  constexpr int kTogether = LANES ? 32 / LANES : 1;          // rows of a warp
+  const int tid = LANES ? threadIdx.x % LANES : threadIdx.x;
+  const int step = LANES ? LANES : blockDim.x;
+  const int n = a.C / VEC;
+  const Param<T> w{a.weight, a.param_f32}, b{a.bias, a.param_f32};
+  const long long stride = gridDim.x * (long long)kRows;
+  long long r = blockIdx.x * (long long)kRows + (LANES ? threadIdx.x / LANES : 0);
+  Vec<T, VEC> next[NV];
+  auto fetch = [&](long long row) {
+    if (row >= a.rows) return;
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * step < n) next[i] = load_vec<T, VEC>(xr + (tid + i * step) * VEC);
+  };
+  pdl_wait();
+  fetch(r);
+  // the lanes of a warp stay together: those of rows past the last one take part in the sums
+  const long long last = (a.rows + kTogether - 1) / kTogether * kTogether;
+  for (; r < last; r += stride) {
+    F x[NV][N];
+    F s = splat<F>(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * step < n) {
+        widen<T, VEC>(next[i], x[i]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) s = add(s, x[i][j]);
+      }
+    fetch(r + stride);
+    const float mean = row_sum<LANES>(total(s), red[0]) / a.C;   // a division: the mean of equal values is their value
+    const F minus = splat<F>(-mean);
+    F q = splat<F>(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * step < n) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          x[i][j] = add(x[i][j], minus);
+          q = fma(x[i][j], x[i][j], q);
+        }
+      }
+    const float rstd = rsqrtf(row_sum<LANES>(total(q), red[1]) * a.inv_c + a.eps);
+    if (r < a.rows) {
+      T* yr = static_cast<T*>(a.y) + r * a.ldy;
+      const F scale = splat<F>(rstd);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (tid + i * step) * VEC;
+        if (tid + i * step < n) {
+          F wv[N], bv[N];
+          w.template get<VEC>(c, 1.f, wv);
+          b.template get<VEC>(c, 0.f, bv);
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[i][j] = fma(mul(x[i][j], scale), wv[j], bv[j]);
+          store_vec<T, VEC>(yr + c, narrow<T, VEC>(x[i]));
+        }
+      }
+      if (a.mean && tid == 0) a.mean[r] = mean, a.rstd[r] = rstd;
+    }
+  }
+}
+
+// Rows of any length that nothing else takes: three passes over the row, the second and third mostly from L2.
 template <class T>
 __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const LnArgs a) {
   pdl_launch_dependents();
@@ -127,121 +158,440 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const LnArgs a) {
   }
 }
 
-// ---- backward ------------------------------------------------------------------------------
-// The next row of dy and x is on its way while the present one is reduced.
-template <class T, int VEC, int NV, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? kLnWarps * 32 : (NV * VEC > 8 ? 512 : 1024)) ln_bwd_kernel(const LnArgs a) {
-  pdl_launch_dependents();
-  extern __shared__ float4 dyn[];                       // weight [C]; afterwards the warps' column sums
-  float* sw = reinterpret_cast<float*>(dyn);
-  __shared__ float red[2][2][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tid = kWarp ? lane : threadIdx.x;
-  const int step = kWarp ? 32 : blockDim.x;
-  const int n = a.C / VEC;
-  const Param<T> w{a.weight, a.param_f32};
-  pdl_wait();
-  for (int c = threadIdx.x; c < a.C; c += blockDim.x) sw[c] = w.p ? w.at(c) : 1.f;
-  __syncthreads();
-  const long long first = kWarp ? blockIdx.x * (long long)kLnWarps + warp : blockIdx.x;
-  const long long stride = kWarp ? gridDim.x * (long long)kLnWarps : gridDim.x;
-  float dw[NV * VEC], db[NV * VEC];
+// ---- many rows: teams ------------------------------------------------------------------------
+// A team of TL threads (8 to a whole block) takes one row at a time and keeps it in registers between its sums and its result;
+// thread `i` of a team has the columns i, i + TL, ... of every row, so that the parameters (forward) and the column sums
+// (backward) stay in registers over all rows.  Rows come through a ring of stages of their own per team, filled by the bulk
+// copy engine: the bytes in flight depend neither on registers nor on occupancy.  Teams below a warp share the warp's stage.
+//
+// Rows of whole 16-byte vectors are copied one by one.  Rows of other lengths can be copied where they lie back to back from an
+// aligned address on: the span is then widened to 16-byte boundaries (what it touches beside the row belongs to its
+// neighbours), and what lies behind the tensor's last boundary is copied by hand.
+struct LnTeams {
+  int TL, rows, stages;     // threads of a team; rows and copies in flight of a ring
+  long long units;          // a.rows in steps of `rows`
+  int one_copy;             // a unit's rows lie back to back
+  int mat_bytes;            // a stage's room for one matrix
+  unsigned long long ceiling;    // elements of x and dy before their last 16-byte boundary
+  int off_w, off_red, off_bar;   // shared-memory offsets: weight, partial sums, barriers (the rings come first)
+  int* dev_status;
+};
+constexpr int kTeamThreads = 512, kTeamWarps = kTeamThreads / 32;
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// Where a stage's first element lies in its room.
+template <class T, int VEC>
+__device__ __forceinline__ uint32_t stage_shift(long long row0, int C) {
+  return VEC == 1 ? (static_cast<uint32_t>(row0) * static_cast<uint32_t>(C)) & (16 / sizeof(T) - 1) : 0;
+}
+// Called by all lanes of one warp: rows [row0, row0 + n) of the given matrices, each to its room of the stage.
+template <class T, int VEC, int MATS>
+__device__ __forceinline__ void load_stage(const T* const (&src)[MATS], const long long (&ld)[MATS], const LnArgs& a, const LnTeams& t, long long row0, int n,
+                                           uint8_t* stage, uint32_t bar) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (VEC == 1) {
+    constexpr unsigned long long kUnit = 16 / sizeof(T);
+    if (lane == 0) {
+      const unsigned long long begin = static_cast<unsigned long long>(row0) * a.C, first = begin & ~(kUnit - 1), end = begin + static_cast<uint32_t>(n * a.C);
+      unsigned long long stop = (end + kUnit - 1) & ~(kUnit - 1);
+      if (stop > t.ceiling) {
+        stop = t.ceiling > first ? t.ceiling : first;
 #pragma unroll
-  for (int i = 0; i < NV * VEC; ++i) dw[i] = db[i] = 0.f;
-  Vec<T, VEC> x[NV], dy[NV], xn[NV], dyn_[NV];
-  float mean = 0.f, rstd = 0.f, mean_n = 0.f, rstd_n = 0.f;
-  auto fetch = [&](long long r, Vec<T, VEC>(&xv)[NV], Vec<T, VEC>(&dv)[NV], float& m, float& s) {
-    if (r >= a.rows) return;
-    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
-    const T* dr = static_cast<const T*>(a.dy) + r * a.lddy;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * step < n) {
-        xv[i] = load_vec<T, VEC>(xr + (tid + i * step) * VEC);
-        dv[i] = load_vec<T, VEC>(dr + (tid + i * step) * VEC);
+        for (int m = 0; m < MATS; ++m)
+          for (unsigned long long i = stop; i < end; ++i) reinterpret_cast<T*>(stage + m * t.mat_bytes)[i - first] = src[m][i];
       }
-    m = a.mean[r], s = a.rstd[r];
-  };
-  fetch(first, x, dy, mean, rstd);
-  int it = 0;
-  for (long long r = first; r < a.rows; r += stride, it ^= 1) {
-    fetch(r + stride, xn, dyn_, mean_n, rstd_n);
-    float s1 = 0.f, s2 = 0.f;
+      const uint32_t bytes = static_cast<uint32_t>(stop - first) * sizeof(T);
+      mbar_arrive_expect_tx(bar, MATS * bytes);
+      if (bytes) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * step < n) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float d = to_f32(dy[i].v[j]), h = (to_f32(x[i].v[j]) - mean) * rstd;
-          const float g = d * sw[(tid + i * step) * VEC + j];
-          s1 += g;
-          s2 = fmaf(g, h, s2);
-          db[i * VEC + j] += d;
-          dw[i * VEC + j] = fmaf(d, h, dw[i * VEC + j]);
-        }
+        for (int m = 0; m < MATS; ++m) bulk_load(smem_u32(stage + m * t.mat_bytes), src[m] + first, bytes, bar);
       }
-    s1 = warp_sum(s1), s2 = warp_sum(s2);
-    if (!kWarp) {
-      if (lane == 0) red[it][0][warp] = s1, red[it][1][warp] = s2;
-      __syncthreads();
-      const bool in = lane < static_cast<int>(blockDim.x >> 5);
-      s1 = warp_sum(in ? red[it][0][lane] : 0.f), s2 = warp_sum(in ? red[it][1][lane] : 0.f);
     }
-    s1 *= a.inv_c, s2 *= a.inv_c;
-    T* out = static_cast<T*>(a.y) + r * a.ldy;
+  } else {
+    const uint32_t row_bytes = a.C * sizeof(T);
+    if (t.one_copy) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, MATS * n * row_bytes);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (tid + i * step < n) {
-        Vec<T, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float h = (to_f32(x[i].v[j]) - mean) * rstd;
-          const float g = to_f32(dy[i].v[j]) * sw[(tid + i * step) * VEC + j];
-          o.v[j] = from_f32<T>(rstd * (g - s1 - h * s2));
-        }
-        store_vec<T, VEC>(out + (tid + i * step) * VEC, o);
+        for (int m = 0; m < MATS; ++m) bulk_load(smem_u32(stage + m * t.mat_bytes), src[m] + row0 * ld[m], n * row_bytes, bar);
       }
+    } else {
+      if (lane == 0) mbar_arrive_expect_tx(bar, MATS * n * row_bytes);
+      __syncwarp();
+      if (lane < n) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = xn[i], dy[i] = dyn_[i];
-    mean = mean_n, rstd = rstd_n;
+        for (int m = 0; m < MATS; ++m) bulk_load(smem_u32(stage + m * t.mat_bytes) + lane * row_bytes, src[m] + (row0 + lane) * ld[m], row_bytes, bar);
+      }
+    }
   }
-  if (!a.part) return;
-  float* pw = a.part + blockIdx.x * 2ll * a.C;
-  if (kWarp) {
-    // the warps' sums, added pairwise through shared memory
-    for (int half = kLnWarps / 2; half > 0; half >>= 1) {
-      __syncthreads();
-      if (warp >= half && warp < 2 * half) {
-        float* to = sw + (warp - half) * 2ll * a.C;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (tid + i * step < n) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) to[(tid + i * step) * VEC + j] = dw[i * VEC + j], to[a.C + (tid + i * step) * VEC + j] = db[i * VEC + j];
-          }
-      }
-      __syncthreads();
-      if (warp < half) {
-        const float* from = sw + warp * 2ll * a.C;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (tid + i * step < n) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) dw[i * VEC + j] += from[(tid + i * step) * VEC + j], db[i * VEC + j] += from[a.C + (tid + i * step) * VEC + j];
-          }
-      }
-    }
-    if (warp != 0) return;
+}
+// After a wait that gave up: copies that may still be in flight land before the block's shared memory is released.
+__device__ __forceinline__ void let_copies_land() {
+  const unsigned long long t0 = global_timer_ns();
+  while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+// Barrier of the `threads` threads of one team; whether any of them raised `flag`.
+__device__ __forceinline__ bool team_barrier(int id, int threads, bool flag) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(flag))
+      : "memory");
+  return any != 0;
+}
+// What a thread is in its team.
+struct TeamRole {
+  int lane;                // in the team
+  int warps, warp;         // warps of the team, and which of them
+  int team, teams;         // of the block (a warp's teams count as one)
+  int sub;                 // which of a warp's rows
+  __device__ __forceinline__ explicit TeamRole(int TL) {
+    lane = threadIdx.x % TL;
+    warps = TL > 32 ? TL / 32 : 1, warp = threadIdx.x / 32 % warps;
+    team = threadIdx.x / (32 * warps), teams = kTeamWarps / warps;
+    sub = TL < 32 ? (threadIdx.x & 31) / TL : 0;
   }
+};
+// Sums over a team of two values at once.  Teams of several warps meet at a barrier, once: partial sums take turns between
+// two slots.  Returns whether a wait has failed.
+template <int K>
+__device__ __forceinline__ void add_lanes(float (&v)[K], int o) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (tid + i * step < n) {
+  for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+}
+template <int K>
+__device__ __forceinline__ bool team_sum(float (&v)[K], const LnTeams& t, const TeamRole& me, float* slots, int turn, bool failed) {
+  if (t.TL > 16) add_lanes<K>(v, 16);
+  if (t.TL > 8) add_lanes<K>(v, 8);
+  add_lanes<K>(v, 4);
+  add_lanes<K>(v, 2);
+  add_lanes<K>(v, 1);
+  if (me.warps == 1) return failed;
+  float* s = slots + (me.team * 2 + turn) * me.warps * K;
+  if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) pw[(tid + i * step) * VEC + j] = dw[i * VEC + j], pw[a.C + (tid + i * step) * VEC + j] = db[i * VEC + j];
+    for (int k = 0; k < K; ++k) s[me.warp * K + k] = v[k];
+  }
+  failed = team_barrier(1 + me.team, 32 * me.warps, failed);
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = s[(threadIdx.x & (me.warps - 1)) * K + k];
+  if (me.warps > 8) add_lanes<K>(v, 8);
+  if (me.warps > 4) add_lanes<K>(v, 4);
+  if (me.warps > 2) add_lanes<K>(v, 2);
+  add_lanes<K>(v, 1);
+  return failed;
+}
+// s / C, exact where the quotient is (equal values have that value as their mean): a product and one correction.
+__device__ __forceinline__ float mean_of(float s, const LnArgs& a) {
+  const float m = s * a.inv_c;
+  return fmaf(fmaf(-m, static_cast<float>(a.C), s), a.inv_c, m);
+}
+// A vector of fp32 parameters in shared memory: quarters of 16 bytes of neighbouring vectors lie side by side (two
+// planes for VEC = 8), so that a warp's reads meet no bank twice.
+template <int VEC>
+__device__ __forceinline__ void shared_param(const float* s, int n, int v, typename Lanes<VEC>::F (&out)[Lanes<VEC>::N]) {
+  if constexpr (VEC == 1) {
+    out[0] = s[v];
+  } else {
+#pragma unroll
+    for (int q = 0; q < VEC / 4; ++q) {
+      const float4 u = *reinterpret_cast<const float4*>(s + (q * n + v) * 4);
+      out[2 * q] = f2(u.x, u.y), out[2 * q + 1] = f2(u.z, u.w);
     }
+  }
+}
+template <int VEC>
+__device__ __forceinline__ int shared_param_index(int n, int c) {
+  if constexpr (VEC == 1) return c;
+  else return ((c % VEC / 4) * n + c / VEC) * 4 + c % 4;
+}
+// Which of a thread's NV vectors may lie behind the row's end: the host picks NV so that only the last one does (the last four
+// single elements).
+template <int VEC, int NV>
+__device__ __forceinline__ bool has_vector(int i, int v, int n) {
+  return i < NV - (VEC == 1 ? 4 : 1) || v < n;
 }
 
-// Rows longer than a block's registers: dx alone, two passes over the row.
+// The ring of a team: what its first warp fills and all of it waits on.
+template <class T, int VEC, int MATS>
+struct TeamRing {
+  const LnArgs& a;
+  const LnTeams& t;
+  const T* src[MATS];
+  long long ld[MATS];
+  uint8_t* base;
+  uint32_t bars;
+  volatile int* abort_flag;
+  long long step;           // units that the grid's teams take at a time
+  int stage;
+  uint32_t phase;
+  __device__ __forceinline__ TeamRing(const LnArgs& a_, const LnTeams& t_, uint8_t* smem, const TeamRole& me) : a(a_), t(t_) {
+    src[0] = static_cast<const T*>(a.x), ld[0] = a.ldx;
+    if constexpr (MATS == 2) src[1] = static_cast<const T*>(a.dy), ld[1] = a.lddy;
+    base = smem + me.team * t.stages * MATS * t.mat_bytes;
+    bars = smem_u32(smem + t.off_bar) + 8 * me.team * t.stages;
+    abort_flag = reinterpret_cast<volatile int*>(smem + t.off_bar + 8 * t.stages * me.teams);
+    step = gridDim.x * (long long)me.teams;
+    stage = 0, phase = 0;
+    if (me.warp == 0 && (threadIdx.x & 31) == 0)
+      for (int i = 0; i < t.stages; ++i) mbar_init(bars + 8 * i, 1);
+    if (threadIdx.x == 0) *abort_flag = 0;
+    if ((threadIdx.x & 31) == 0) mbar_fence_init();
+    __syncthreads();
+  }
+  __device__ __forceinline__ void load(long long unit, int st) {
+    if (unit >= t.units) return;
+    const long long row0 = unit * t.rows;
+    load_stage<T, VEC, MATS>(src, ld, a, t, row0, (int)min((long long)t.rows, a.rows - row0), base + st * MATS * t.mat_bytes, bars + 8 * st);
+  }
+  __device__ __forceinline__ bool wait(int site) { return mbar_wait_warp(bars + 8 * stage, phase, abort_flag, t.dev_status, site); }
+  __device__ __forceinline__ const T* mat(int m, long long row0) const {
+    return reinterpret_cast<const T*>(base + (stage * MATS + m) * t.mat_bytes) + stage_shift<T, VEC>(row0, a.C);
+  }
+  // after the team has read the stage: called by its first warp
+  __device__ __forceinline__ void refill(long long unit) { load(unit + t.stages * step, stage); }
+  __device__ __forceinline__ void next() {
+    if (++stage == t.stages) stage = 0, phase ^= 1u;
+  }
+};
+
+template <class T, int VEC, int NV>
+__global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_teams_kernel(const LnArgs a, const LnTeams t) {
+  pdl_launch_dependents();
+  using F = typename Lanes<VEC>::F;
+  constexpr int N = Lanes<VEC>::N;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const TeamRole me(t.TL);
+  TeamRing<T, VEC, 1> ring(a, t, smem, me);
+  float* slots = reinterpret_cast<float*>(smem + t.off_red);
+  const int n = a.C / VEC;
+  const long long first = blockIdx.x * (long long)me.teams + me.team;
+  pdl_wait();
+  if (me.warp == 0)
+    for (int i = 0; i < t.stages; ++i) ring.load(first + i * ring.step, i);
+  F w[NV][N], b[NV][N];
+  {
+    const Param<T> pw{a.weight, a.param_f32}, pb{a.bias, a.param_f32};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = min(me.lane + i * t.TL, n - 1);
+      pw.template get<VEC>((long long)v * VEC, 1.f, w[i]);
+      pb.template get<VEC>((long long)v * VEC, 0.f, b[i]);
+    }
+  }
+  bool failed = false;
+  for (long long unit = first; unit < t.units; unit += ring.step) {
+    const long long row0 = unit * t.rows, row = row0 + me.sub;
+    const bool in = row < a.rows;
+    failed = !ring.wait(700);
+    if (failed && me.warps == 1) break;
+    const T* xs = ring.mat(0, row0) + me.sub * a.C;
+    F x[NV][N];
+    F s[2] = {splat<F>(0.f), splat<F>(0.f)};   // two chains of additions
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = me.lane + i * t.TL;
+      if (in && has_vector<VEC, NV>(i, v, n)) {
+        widen<T, VEC>(load_vec<T, VEC>(xs + v * VEC), x[i]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) s[(i * N + j) % 2] = add(s[(i * N + j) % 2], x[i][j]);
+      }
+    }
+    float sum[1] = {total(add(s[0], s[1]))};
+    failed = team_sum<1>(sum, t, me, slots, 0, failed);
+    if (failed) break;
+    // the stage has been read by the whole team
+    __syncwarp();
+    if (me.warp == 0) ring.refill(unit);
+    ring.next();
+    const float mean = mean_of(sum[0], a);
+    const F minus = splat<F>(-mean);
+    s[0] = s[1] = splat<F>(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (has_vector<VEC, NV>(i, me.lane + i * t.TL, n)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          x[i][j] = add(x[i][j], minus);
+          s[(i * N + j) % 2] = fma(x[i][j], x[i][j], s[(i * N + j) % 2]);
+        }
+      }
+    }
+    sum[0] = total(add(s[0], s[1]));
+    team_sum<1>(sum, t, me, slots, 1, false);
+    const float rstd = rsqrtf(sum[0] * a.inv_c + a.eps);
+    if (in) {
+      const F scale = splat<F>(rstd);
+      T* yr = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = me.lane + i * t.TL;
+        if (has_vector<VEC, NV>(i, v, n)) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[i][j] = fma(mul(x[i][j], scale), w[i][j], b[i][j]);
+          store_vec<T, VEC>(yr + v * VEC, narrow<T, VEC>(x[i]));
+        }
+      }
+      if (a.mean && me.lane == 0) a.mean[row] = mean, a.rstd[row] = rstd;
+    }
+  }
+  if (__syncthreads_or(failed)) let_copies_land();
+}
+
+// ---- backward --------------------------------------------------------------------------------
+template <class T, int VEC, int NV>
+__global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnArgs a, const LnTeams t) {
+  pdl_launch_dependents();
+  using F = typename Lanes<VEC>::F;
+  constexpr int N = Lanes<VEC>::N;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const TeamRole me(t.TL);
+  TeamRing<T, VEC, 2> ring(a, t, smem, me);
+  float* slots = reinterpret_cast<float*>(smem + t.off_red);
+  float* sw = reinterpret_cast<float*>(smem + t.off_w);
+  const int n = a.C / VEC;
+  const long long first = blockIdx.x * (long long)me.teams + me.team;
+  pdl_wait();
+  if (me.warp == 0)
+    for (int i = 0; i < t.stages; ++i) ring.load(first + i * ring.step, i);
+  {
+    const Param<T> w{a.weight, a.param_f32};
+    for (int c = threadIdx.x; c < a.C; c += kTeamThreads) sw[shared_param_index<VEC>(n, c)] = w.p ? w.at(c) : 1.f;
+  }
+  F dw[NV][N], db[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) dw[i][j] = db[i][j] = splat<F>(0.f);
+  float mean_next = 0.f, rstd_next = 0.f;
+  auto moments = [&](long long row) {
+    if (row < a.rows) mean_next = a.mean[row], rstd_next = a.rstd[row];
+  };
+  moments(first * t.rows + me.sub);
+  __syncthreads();
+  bool failed = false;
+  int turn = 0;
+  for (long long unit = first; unit < t.units; unit += ring.step, turn ^= 1) {
+    const long long row0 = unit * t.rows, row = row0 + me.sub;
+    const bool in = row < a.rows;
+    failed = !ring.wait(701);
+    if (failed && me.warps == 1) break;
+    const T* xs = ring.mat(0, row0) + me.sub * a.C;
+    const T* ds = ring.mat(1, row0) + me.sub * a.C;
+    F x[NV][N];                          // x - mean
+    Vec<T, VEC> raw[NV];                 // dy, as loaded: widened twice, at half the registers
+    const float mean = mean_next, rstd = rstd_next;
+    moments((unit + ring.step) * t.rows + me.sub);
+    F s1 = splat<F>(0.f), s2 = s1;       // sum(g), sum(g (x - mean))
+    const F minus = splat<F>(-mean);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = me.lane + i * t.TL;
+      if (in && has_vector<VEC, NV>(i, v, n)) {
+        F w[N], d[N];
+        widen<T, VEC>(load_vec<T, VEC>(xs + v * VEC), x[i]);
+        raw[i] = load_vec<T, VEC>(ds + v * VEC);
+        widen<T, VEC>(raw[i], d);
+        shared_param<VEC>(sw, n, v, w);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const F g = mul(d[j], w[j]);
+          x[i][j] = add(x[i][j], minus);
+          s1 = add(s1, g);
+          s2 = fma(g, x[i][j], s2);
+        }
+      }
+    }
+    float sum[2] = {total(s1), total(s2)};
+    failed = team_sum<2>(sum, t, me, slots, turn, failed);
+    if (failed) break;
+    __syncwarp();
+    if (me.warp == 0) ring.refill(unit);   // the stage has been read by the whole team
+    ring.next();
+    const F r = splat<F>(rstd), c1 = splat<F>(-rstd * (sum[0] * a.inv_c)), c2 = splat<F>(-rstd * (rstd * (sum[1] * a.inv_c)));
+    if (in) {
+      T* out = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = me.lane + i * t.TL;
+        if (has_vector<VEC, NV>(i, v, n)) {
+          F w[N], d[N];
+          widen<T, VEC>(raw[i], d);
+          shared_param<VEC>(sw, n, v, w);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            // dx = dy (w r) + h c2 + c1
+            const F h = mul(x[i][j], r);
+            dw[i][j] = fma(d[j], h, dw[i][j]);
+            db[i][j] = add(db[i][j], d[j]);
+            x[i][j] = fma(d[j], mul(w[j], r), fma(h, c2, c1));
+          }
+          store_vec<T, VEC>(out + v * VEC, narrow<T, VEC>(x[i]));
+        }
+      }
+    }
+  }
+  if (__syncthreads_or(failed)) {
+    let_copies_land();
+    return;
+  }
+  if (!a.part) return;
+  // Column sums of the block: over the rows of a warp by shuffles, over teams through shared memory (the rings are empty by
+  // now), half of them at a time.
+  if (t.TL < 32) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        for (int o = t.TL; o < 32; o <<= 1) {
+          if constexpr (VEC == 1) {
+            dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], o), db[i][j] += __shfl_xor_sync(0xffffffffu, db[i][j], o);
+          } else {
+            dw[i][j] = add(dw[i][j], F2{__shfl_xor_sync(0xffffffffu, dw[i][j].v, o)});
+            db[i][j] = add(db[i][j], F2{__shfl_xor_sync(0xffffffffu, db[i][j].v, o)});
+          }
+        }
+  }
+  float* buf = reinterpret_cast<float*>(smem);
+  float* out = a.part + blockIdx.x * 2ll * a.C;
+  for (int half = me.teams / 2;; half /= 2) {
+    float* to = half ? buf + (me.team - half) * 2 * a.C : out;
+    if ((half ? me.team >= half && me.team < 2 * half : me.team == 0) && me.sub == 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = me.lane + i * t.TL;
+        if (has_vector<VEC, NV>(i, v, n)) {
+          *reinterpret_cast<Vec<F, N>*>(to + v * VEC) = *reinterpret_cast<const Vec<F, N>*>(&dw[i]);
+          *reinterpret_cast<Vec<F, N>*>(to + a.C + v * VEC) = *reinterpret_cast<const Vec<F, N>*>(&db[i]);
+        }
+      }
+    }
+    if (half == 0) break;
+    __syncthreads();
+    if (me.team < half && me.sub == 0) {
+      const float* from = buf + me.team * 2 * a.C;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = me.lane + i * t.TL;
+        if (has_vector<VEC, NV>(i, v, n)) {
+          const Vec<F, N> p = *reinterpret_cast<const Vec<F, N>*>(from + v * VEC), q = *reinterpret_cast<const Vec<F, N>*>(from + a.C + v * VEC);
+#pragma unroll
+          for (int j = 0; j < N; ++j) dw[i][j] = add(dw[i][j], p.v[j]), db[i][j] = add(db[i][j], q.v[j]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Rows that the teams do not take: dx alone, two passes over the row.
 template <class T>
 __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(const LnArgs a) {
   pdl_launch_dependents();
@@ -316,86 +666,181 @@ int sum_partials(const float* part, int count, long long pitch, int C, void* out
 // ---- host side -----------------------------------------------------------------------------
 static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Once per kernel and device: more dynamic shared memory than the default.
+template <auto kernel>
+static int allow_smem(int bytes) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "cudaFuncSetAttribute(layernorm)")) return rc;
+    configured[dev] = true;
+  }
+  return kOk;
+}
 constexpr int kLnMaxC = 1 << 30;   // column indices, and a step past the last one, are ints
-constexpr int kLnBlocksPerSm = 4;
-// Blocks of the backward pass, each of which leaves one row of column sums: at most four an SM, and no more than one for
-// sixteen rows unless that leaves SMs idle (the sums are 16 bytes a column and block, written and read again).
+// Blocks of the backward pass, at most: each leaves one row of column sums.
 static long long ln_bwd_blocks(long long rows) {
-  const long long sms = sm_count();
-  long long g = rows / 16 > sms ? rows / 16 : sms;
-  if (g > sms * kLnBlocksPerSm) g = sms * kLnBlocksPerSm;
-  return g < rows ? g : rows;
+  const long long most = sm_count() * 2ll;
+  return rows < most ? rows : most;
 }
 
-template <class T, int VEC, int NV, bool kWarp>
+// Whether rows of `base` lie back to back from a 16-byte aligned address on.
+static bool back_to_back(const void* base, long long ld, int C) { return al16(base) && ld == C; }
+
+constexpr long long kSmemSm = 227 * 1024, kSmemHalf = kSmemSm / 2 - 1024;   // of an SM; a block's where two share one
+// Fills `t` for rows of `mats` matrices and threads of at most `most` vectors; false where rows of this size do not fit.
+// `params`: bytes of shared memory for the parameters; `sums`: whether the block's column sums meet in the rings at the end;
+// `room`: shared memory of a block.  NV of the kernel: t.nv.
+static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats, int most, long long params, bool sums, long long room, int& nv, int& smem) {
+  const long long row = a.C * (long long)elem, n = a.C / vec;
+  int TL = 8;
+  while (TL < kTeamThreads && n > (long long)most * TL) TL *= 2;
+  if (n > (long long)most * TL) return false;
+  nv = (int)((n + TL - 1) / TL);
+  if (vec == 1) nv = (nv + 3) / 4 * 4;
+  const int warps = TL > 32 ? TL / 32 : 1, teams = kTeamWarps / warps;
+  t.ceiling = (unsigned long long)a.rows * a.C / (16 / elem) * (16 / elem);
+  t.TL = TL, t.rows = TL < 32 ? 32 / TL : 1, t.units = (a.rows + t.rows - 1) / t.rows;
+  t.mat_bytes = (int)((t.rows * row + 15) / 16 * 16 + (vec == 1 ? 32 : 0));   // a widened span begins and ends up to 15 bytes further out
+  const long long slots = 2ll * kTeamWarps * mats * 4, rest = params + slots + teams * 8 * 8 + 512;
+  const long long scratch = sums ? teams / 2 * 2ll * a.C * 4 : 0;
+  long long stages = (room - rest) / ((long long)teams * mats * t.mat_bytes);
+  if (stages > 8) stages = 8;
+  if (stages < 2 || scratch > room - rest) return false;
+  t.stages = (int)stages;
+  long long ring = stages * teams * mats * t.mat_bytes;
+  if (ring < scratch) ring = scratch;
+  t.off_w = (int)((ring + 127) / 128 * 128);
+  t.off_red = (int)((t.off_w + params + 15) / 16 * 16);
+  t.off_bar = (int)(t.off_red + slots);
+  smem = t.off_bar + 8 * t.stages * teams + 16;
+  return smem <= room;
+}
+static int team_blocks(const LnTeams& t, int per_sm) {
+  const long long teams = kTeamWarps / (t.TL > 32 ? t.TL / 32 : 1), need = (t.units + teams - 1) / teams, most = (long long)sm_count() * per_sm;
+  return (int)(need < most ? need : most);
+}
+
+template <class T, int VEC, int NV>
+static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
+  if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV>>(kSmemSm)) return rc;
+  return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
+}
+template <class T, int VEC>
+static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
+  LnTeams t = {};
+  int nv = 0, smem = 0;
+  const bool close = back_to_back(a.x, a.ldx, a.C);
+  const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 6, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
+  done = (VEC > 1 || close) &&
+         (plan_teams(t, a, sizeof(T), VEC, 1, most, 0, false, kSmemSm, nv, smem) || plan_teams(t, a, sizeof(T), VEC, 1, wide, 0, false, kSmemSm, nv, smem));
+  if (done && nv * VEC <= 8) plan_teams(t, a, sizeof(T), VEC, 1, most, 0, false, kSmemHalf, nv, smem);   // two blocks an SM
+  if (!done) return kOk;
+  t.one_copy = close || t.rows == 1;
+  if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_fwd: no device status word");
+  if constexpr (VEC == 1) {
+    if (nv <= 4) return ln_fwd_teams_launch<T, 1, 4>(a, t, smem, s);
+    if (nv <= 8) return ln_fwd_teams_launch<T, 1, 8>(a, t, smem, s);
+    if (nv <= 12) return ln_fwd_teams_launch<T, 1, 12>(a, t, smem, s);
+    return ln_fwd_teams_launch<T, 1, 16>(a, t, smem, s);
+  } else {
+    if (nv == 1) return ln_fwd_teams_launch<T, VEC, 1>(a, t, smem, s);
+    if (nv == 2) return ln_fwd_teams_launch<T, VEC, 2>(a, t, smem, s);
+    if (nv == 3) return ln_fwd_teams_launch<T, VEC, 3>(a, t, smem, s);
+    if (nv == 4) return ln_fwd_teams_launch<T, VEC, 4>(a, t, smem, s);
+    if constexpr (VEC == 4) {
+      if (nv == 5) return ln_fwd_teams_launch<T, VEC, 5>(a, t, smem, s);
+      if (nv == 6) return ln_fwd_teams_launch<T, VEC, 6>(a, t, smem, s);
+      if (nv == 7) return ln_fwd_teams_launch<T, VEC, 7>(a, t, smem, s);
+      return ln_fwd_teams_launch<T, VEC, 8>(a, t, smem, s);
+    }
+    return fail(kErrUnsupported, "bxl_layernorm_fwd: no kernel for %d vectors a thread", nv);
+  }
+}
+
+template <class T, int VEC, int NV, int LANES, int kMaxThreads = LANES ? kLnWarps * 32 : 512>
 static int ln_fwd_launch(const LnArgs& a, int threads, cudaStream_t s) {
-  const long long need = kWarp ? (a.rows + kLnWarps - 1) / kLnWarps : a.rows, most = (long long)sm_count() * 16;
-  return launch_kernel("ln_fwd_kernel launch", ln_fwd_kernel<T, VEC, NV, kWarp>, dim3((unsigned)(need < most ? need : most)), dim3(threads), 0, s, 1, a);
+  constexpr int kRows = LANES ? kLnWarps * 32 / LANES : 1;
+  const long long need = (a.rows + kRows - 1) / kRows, most = sm_count() * (2048ll / threads);
+  return launch_kernel("ln_fwd_kernel launch", ln_fwd_kernel<T, VEC, NV, LANES, kMaxThreads>, dim3((unsigned)(need < most ? need : most)), dim3(threads), 0, s, 1, a);
 }
 template <class T>
 static int ln_fwd(const LnArgs& a, bool vec, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), W = kLnWarps * 32;
+  const char* e = getenv("LN_FEW");
+  const long long few = e ? atoll(e) : 2048;
+  if (a.rows > few) {
+    bool done = false;
+    if (int rc = vec ? ln_fwd_teams<T, V>(a, done, s) : ln_fwd_teams<T, 1>(a, done, s)) return rc;
+    if (done) return kOk;
+  }
   if (vec) {
     const int n = a.C / V;
-    if (n <= 32) return ln_fwd_launch<T, V, 1, true>(a, kLnWarps * 32, s);
-    if (n <= 64) return ln_fwd_launch<T, V, 2, true>(a, kLnWarps * 32, s);
-    if (n <= 96) return ln_fwd_launch<T, V, 3, true>(a, kLnWarps * 32, s);
-    if (n <= 160) return ln_fwd_launch<T, V, 5, true>(a, kLnWarps * 32, s);
-    if (n <= 512) return ln_fwd_launch<T, V, 2, false>(a, 256, s);
-    if (n <= 1024) return ln_fwd_launch<T, V, 2, false>(a, 512, s);
-    if (n <= 2048) return ln_fwd_launch<T, V, 4, false>(a, 512, s);
-    if (n <= 8192) return ln_fwd_launch<T, V, 8, false>(a, 1024, s);
+    if (n <= 32) return ln_fwd_launch<T, V, 1, 32>(a, W, s);
+    if (n <= 64) return ln_fwd_launch<T, V, 2, 32>(a, W, s);
+    if (n <= 96) return ln_fwd_launch<T, V, 3, 32>(a, W, s);
+    for (int threads = 64; threads <= 512; threads *= 2)
+      if (n <= 2 * threads) return ln_fwd_launch<T, V, 2, 0>(a, threads, s);
+    if (n <= 2048) return ln_fwd_launch<T, V, 4, 0>(a, 512, s);
+    if (n <= 4096) return ln_fwd_launch<T, V, 4, 0, 1024>(a, 1024, s);
   } else {
-    if (a.C <= 64) return ln_fwd_launch<T, 1, 2, true>(a, kLnWarps * 32, s);
-    if (a.C <= 256) return ln_fwd_launch<T, 1, 8, true>(a, kLnWarps * 32, s);
-    if (a.C <= 2048) return ln_fwd_launch<T, 1, 8, false>(a, 256, s);
-    if (a.C <= 8192) return ln_fwd_launch<T, 1, 8, false>(a, 1024, s);
-    if (a.C <= 16384) return ln_fwd_launch<T, 1, 16, false>(a, 1024, s);
+    if (a.C <= 256) return ln_fwd_launch<T, 1, 8, 32>(a, W, s);
+    if (a.C <= 2048) return ln_fwd_launch<T, 1, 8, 0>(a, 256, s);
+    if (a.C <= 8192) return ln_fwd_launch<T, 1, 8, 0, 1024>(a, 1024, s);
   }
   const long long most = (long long)sm_count() * 2;
   return launch_kernel("ln_fwd_long_kernel launch", ln_fwd_long_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, s, 1, a);
 }
 
-template <class T, int VEC, int NV, bool kWarp>
-static int ln_bwd_launch(const LnArgs& a, int threads, int& blocks, cudaStream_t s) {
-  const long long most = ln_bwd_blocks(a.rows), need = kWarp ? (a.rows + kLnWarps - 1) / kLnWarps : a.rows;
-  blocks = (int)(need < most ? need : most);
-  size_t smem = sizeof(float) * a.C;
-  if (kWarp && a.part) smem *= kLnWarps;   // half of the warps' two sums
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(ln_bwd_kernel<T, VEC, NV, kWarp>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024),
-                            "cudaFuncSetAttribute(layernorm)"))
-      return rc;
-    configured[dev] = true;
-  }
-  return launch_kernel("ln_bwd_kernel launch", ln_bwd_kernel<T, VEC, NV, kWarp>, dim3(blocks), dim3(threads), smem, s, 1, a);
+template <class T, int VEC, int NV>
+static int ln_bwd_teams_launch(const LnArgs& a, const LnTeams& t, int blocks, int smem, cudaStream_t s) {
+  if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV>>(kSmemSm)) return rc;
+  return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
 }
+template <class T, int VEC>
+static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s) {
+  LnTeams t = {};
+  int nv = 0, smem = 0;
+  const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
+  const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 6, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
+  done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
+                                         plan_teams(t, a, sizeof(T), VEC, 2, wide, 4ll * a.C, true, kSmemSm, nv, smem));
+  if (!done) return kOk;
+  t.one_copy = close || t.rows == 1;
+  if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_bwd: no device status word");
+  blocks = team_blocks(t, 1);
+  if constexpr (VEC == 1) {
+    if (nv <= 4) return ln_bwd_teams_launch<T, 1, 4>(a, t, blocks, smem, s);
+    if (nv <= 8) return ln_bwd_teams_launch<T, 1, 8>(a, t, blocks, smem, s);
+    if (nv <= 12) return ln_bwd_teams_launch<T, 1, 12>(a, t, blocks, smem, s);
+    return ln_bwd_teams_launch<T, 1, 16>(a, t, blocks, smem, s);
+  } else {
+    if (nv == 1) return ln_bwd_teams_launch<T, VEC, 1>(a, t, blocks, smem, s);
+    if (nv == 2) return ln_bwd_teams_launch<T, VEC, 2>(a, t, blocks, smem, s);
+    if (nv == 3) return ln_bwd_teams_launch<T, VEC, 3>(a, t, blocks, smem, s);
+    if (nv == 4) return ln_bwd_teams_launch<T, VEC, 4>(a, t, blocks, smem, s);
+    if constexpr (VEC == 4) {
+      if (nv == 5) return ln_bwd_teams_launch<T, VEC, 5>(a, t, blocks, smem, s);
+      if (nv == 6) return ln_bwd_teams_launch<T, VEC, 6>(a, t, blocks, smem, s);
+      if (nv == 7) return ln_bwd_teams_launch<T, VEC, 7>(a, t, blocks, smem, s);
+      return ln_bwd_teams_launch<T, VEC, 8>(a, t, blocks, smem, s);
+    }
+    return fail(kErrUnsupported, "bxl_layernorm_bwd: no kernel for %d vectors a thread", nv);
+  }
+}
+
 template <class T>
 static int ln_bwd(const LnArgs& a, bool vec, int& blocks, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  if (vec) {
-    const int n = a.C / V;
-    if (n <= 32) return ln_bwd_launch<T, V, 1, true>(a, kLnWarps * 32, blocks, s);
-    if (n <= 64) return ln_bwd_launch<T, V, 2, true>(a, kLnWarps * 32, blocks, s);
-    if (n <= 96) return ln_bwd_launch<T, V, 3, true>(a, kLnWarps * 32, blocks, s);
-    if (n <= 256) return ln_bwd_launch<T, V, 1, false>(a, 256, blocks, s);
-    if (n <= 512) return ln_bwd_launch<T, V, 1, false>(a, 512, blocks, s);
-    if (n <= 1024) return ln_bwd_launch<T, V, 2, false>(a, 512, blocks, s);
-    if (n <= 2048) return ln_bwd_launch<T, V, 4, false>(a, 512, blocks, s);
-  } else {
-    if (a.C <= 64) return ln_bwd_launch<T, 1, 2, true>(a, kLnWarps * 32, blocks, s);
-    if (a.C <= 256) return ln_bwd_launch<T, 1, 8, true>(a, kLnWarps * 32, blocks, s);
-    if (a.C <= 2048) return ln_bwd_launch<T, 1, 8, false>(a, 256, blocks, s);
-    if (a.C <= 8192) return ln_bwd_launch<T, 1, 8, false>(a, 1024, blocks, s);
-  }
+  bool done = false;
+  if (int rc = vec ? ln_bwd_teams<T, V>(a, done, blocks, s) : ln_bwd_teams<T, 1>(a, done, blocks, s)) return rc;
+  if (done) return kOk;
   const long long most = (long long)sm_count() * 2;
   if (int rc = launch_kernel("ln_bwd_long_kernel launch", ln_bwd_long_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, s, 1, a))
     return rc;
   if (!a.part) return kOk;
-  const long long shares = ln_bwd_blocks(a.rows) < 64 ? ln_bwd_blocks(a.rows) : 64;
+  const long long shares = a.rows < 64 ? a.rows : 64;
   blocks = (int)shares;
   return launch_kernel("ln_bwd_columns_kernel launch", ln_bwd_columns_kernel<T>, dim3((a.C + 255) / 256, (unsigned)shares), dim3(256), 0, s, 1, a);
 }

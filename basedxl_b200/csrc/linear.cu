@@ -220,7 +220,7 @@ using namespace bxl;
 
 extern "C" long long bxl_linear_act_fwd_workspace_bytes(const bxl_linear_args* a) { return check_linear("bxl_linear_act_fwd", a) ? 0 : fwd_workspace(a); }
 
-extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, int* launches, void* stream) {
+extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, void* stream) {
   const char* who = "bxl_linear_act_fwd";
   if (int rc = check_linear(who, a)) return rc;
   if (!a->y) return fail(kErrInvalidArg, "%s: null operand", who);
@@ -228,7 +228,6 @@ extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, int* launches, void*
   if (int rc = check_workspace(who, a, fwd_workspace(a))) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   const int bf16 = a->dtype == BXL_BF16;
-  if (launches) *launches = fwd_workspace(a) > 0 ? 2 : 1;
   if (a->M <= kFewRows) {
     const FewRows p{a->x, a->weight, a->bias, a->residual, a->y, a->pre, a->ldx, a->ldw, a->ldr, a->ldy, a->ldp, a->M, a->N, a->K, a->act};
     const bool vec = a->K % 8 == 0 && al(a->x, 16) && al(a->weight, 16) && a->ldx % 8 == 0 && a->ldw % 8 == 0;

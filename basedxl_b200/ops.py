@@ -16,7 +16,8 @@ _vp = C.c_void_p
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle, without the ``Stream`` object that ``torch.cuda.current_stream`` builds (3.2 -> 0.3 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _p(t: torch.Tensor | None) -> int | None:
@@ -34,19 +35,25 @@ def _f16_cuda(t: torch.Tensor, name: str) -> None:
 
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # BXL_F16, BXL_BF16, BXL_F32
+_HALF_TYPES = (torch.float16, torch.bfloat16)
 
 
-def _on_current_device(name: str, *tensors) -> None:
-    """The kernels run on the current device's current stream: every operand has to live there."""
-    for t in tensors:
-        if t is not None and not (t.is_cuda and t.device.index == torch.cuda.current_device()):
-            raise ValueError(f"{name}: expected tensors of the current CUDA device, got {t.device}")
+def _device() -> int:
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1   # no tensor of a device exists before
+
+
+def _here(name: str, x: torch.Tensor) -> torch.device:
+    """The device of ``x``, which has to be the current one: the kernels run on its current stream."""
+    dev = x.device
+    if dev.index != _device():
+        raise ValueError(f"{name}: expected tensors of the current CUDA device, got {dev}")
+    return dev
 
 
 def _rows(t):
     """``t`` as a matrix of rows with unit-stride columns (a view where its strides allow one)."""
     t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return t2 if t2.shape[1] == 1 or t2.stride(1) == 1 else t2.contiguous()
+    return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
 
 
 # --------------------------------------------------------------------------- matmul
@@ -270,42 +277,54 @@ def gemm_split_f32(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "quick_gelu": 5}
 
 
-def _linear_operands(name, x, weight, activation, like_y):
-    """Checked operands: ``x`` and the ``[..., N]`` tensors of ``like_y`` (or None) as matrices of rows."""
-    _on_current_device(name, x, weight, *like_y)
-    _req(x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1 and weight.dim() == 2, f"{name}: fp16 or bf16 x [..., K] and weight [N, K]")
-    _req(weight.dtype == x.dtype and weight.shape[1] == x.shape[-1] and weight.numel() > 0, f"{name}: weight must be [N, K] in the type of x")
-    _req(activation in ACTIVATIONS, f"{name}: unknown activation {activation!r}")
-    shape = (*x.shape[:-1], weight.shape[0])
-    for t in like_y:
-        _req(t is None or (t.shape == shape and t.dtype == x.dtype), f"{name}: expected {list(shape)} in the type of x")
-    return _rows(x), _rows(weight), [None if t is None else _rows(t) for t in like_y]
+def _linear_operands(name, x, weight, activation):
+    """Checks what the two passes share; returns device, type, ``x`` and ``weight`` as rows, and the shape of the result."""
+    dev, dt, shape, ws = _here(name, x), x.dtype, x.shape, weight.shape
+    if dt not in _HALF_TYPES or len(shape) < 1 or len(ws) != 2 or weight.dtype != dt or ws[1] != shape[-1] or ws[0] < 1 or ws[1] < 1:
+        raise ValueError(f"{name}: expected fp16 or bf16 x [..., K] and weight [N, K], got {x.dtype} {list(shape)} and {weight.dtype} {list(ws)}")
+    if weight.device != dev:
+        raise ValueError(f"{name}: weight is on {weight.device}, x on {dev}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{name}: unknown activation {activation!r}")
+    return dev, dt, _rows(x), _rows(weight), (*shape[:-1], ws[0])
+
+
+def _like(name, t, what, shape, dt, dev):
+    if t.shape != shape or t.dtype != dt or t.device != dev:
+        raise ValueError(f"{name}: {what} must be {list(shape)} in the type and on the device of x, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def linear_act(x, weight, bias=None, activation=None, residual=None, out=None, want_pre: bool = False):
     """``act(x[..., K] @ weight[N, K]^T + bias) + residual`` in one product, fp16 or bf16, any extents; ``activation`` is one of
     ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``) receives the result.  ``want_pre`` also returns the value
     before the activation, rounded to the type of ``x``: the input of :func:`linear_act_bwd`."""
-    x2, w2, (r2,) = _linear_operands("linear_act", x, weight, activation, (residual,))
-    _on_current_device("linear_act", bias, out)
-    (m, k), n = x2.shape, w2.shape[0]
-    _req(bias is None or (bias.shape == (n,) and bias.dtype == x.dtype and bias.is_contiguous()), "linear_act: bias must be a contiguous [N] vector in the type of x")
-    shape = (*x.shape[:-1], n)
+    dev, dt, x2, w2, shape = _linear_operands("linear_act", x, weight, activation)
+    (m, k), n = x2.shape, shape[-1]
+    r2 = pre = None
+    if bias is not None:
+        _like("linear_act", bias, "bias", (n,), dt, dev)
+        _req(bias.is_contiguous(), "linear_act: bias must be contiguous")
+    if residual is not None:
+        _like("linear_act", residual, "residual", shape, dt, dev)
+        r2 = _rows(residual)
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=x.dtype)
-    _req(out.shape == shape and out.dtype == x.dtype and out.is_contiguous(), "linear_act: out must be contiguous, [..., N] in the type of x")
-    pre = torch.empty(shape, device=x.device, dtype=x.dtype) if want_pre else None
+        out = x.new_empty(shape)
+    else:
+        _like("linear_act", out, "out", shape, dt, dev)
+        _req(out.is_contiguous(), "linear_act: out must be contiguous")
+    if want_pre:
+        pre = torch.empty_like(out)
     if m:
         l = _lib.lib()
-        args = _lib.LinearArgs(_p(x2), x2.stride(0), _p(w2), w2.stride(0), _p(bias), _p(r2), 0 if r2 is None else r2.stride(0), _p(out), n, _p(pre), n)
-        args.M, args.N, args.K, args.dtype, args.act = m, n, k, _TYPES[x.dtype], ACTIVATIONS[activation]
-        nbytes = l.bxl_linear_act_fwd_workspace_bytes(C.byref(args))
+        args = _lib.LinearArgs(
+            x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _p(bias), _p(r2), 0 if r2 is None else r2.stride(0), out.data_ptr(), n, _p(pre), n,
+            None, 0, None, 0, None, 0, None, None, 0, m, n, k, _TYPES[dt], ACTIVATIONS[activation])
+        ref = C.byref(args)
+        nbytes = l.bxl_linear_act_fwd_workspace_bytes(ref)
         if nbytes:
-            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-            args.workspace, args.workspace_bytes = _p(ws), nbytes
-        count = C.c_int(0)
-        rc = l.bxl_linear_act_fwd(C.byref(args), C.byref(count), _stream())
-        _lib.check(rc, l, kernels=count.value)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+        _lib.check(l.bxl_linear_act_fwd(ref, _stream()), l, kernels=2 if nbytes else 1)
     return (out, pre) if want_pre else out
 
 
@@ -313,26 +332,35 @@ def linear_act_bwd(dy, x, weight, pre=None, activation=None, want_dx: bool = Tru
     """Gradients ``(dx, dweight, dbias)`` of :func:`linear_act`, given that of its result and, where it has an activation, the
     ``pre`` it returned; ``None`` for those that are not wanted.  The gradient of its residual is ``dy`` itself.  All have
     the type of ``x``; sums are fp32, ``dy * act'(pre)`` is rounded to that type between the products."""
-    x2, w2, (dy2, pre2) = _linear_operands("linear_act_bwd", x, weight, activation, (dy, pre))
-    act = ACTIVATIONS[activation]
+    dev, dt, x2, w2, shape = _linear_operands("linear_act_bwd", x, weight, activation)
+    act, (m, k), n = ACTIVATIONS[activation], x2.shape, shape[-1]
+    _like("linear_act_bwd", dy, "dy", shape, dt, dev)
+    pre2 = None
+    if pre is not None:
+        _like("linear_act_bwd", pre, "pre", shape, dt, dev)
+        pre2 = _rows(pre)
     _req(act == 0 or pre is not None, "linear_act_bwd: an activation needs the value before it (pre)")
-    (m, k), n = x2.shape, w2.shape[0]
-    new = torch.empty if m else torch.zeros
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if want_dx else None
-    dweight = new((n, k), device=x.device, dtype=x.dtype) if want_dweight else None
-    dbias = new(n, device=x.device, dtype=x.dtype) if want_dbias else None
-    if m and (want_dx or want_dweight or want_dbias):
+    dx = x.new_empty(x.shape) if want_dx else None
+    dweight = x.new_empty((n, k)) if want_dweight else None
+    dbias = x.new_empty(n) if want_dbias else None
+    if not m:
+        for t in (dweight, dbias):
+            if t is not None:
+                t.zero_()
+    elif want_dx or want_dweight or want_dbias:
+        dy2 = _rows(dy)
         l = _lib.lib()
-        args = _lib.LinearArgs(_p(x2), x2.stride(0), _p(w2), w2.stride(0), None, None, 0, None, 0, _p(pre2), 0 if pre2 is None else pre2.stride(0),
-                               _p(dy2), dy2.stride(0), _p(dx), k, _p(dweight), k, _p(dbias))
-        args.M, args.N, args.K, args.dtype, args.act = m, n, k, _TYPES[x.dtype], act
-        nbytes = l.bxl_linear_act_bwd_workspace_bytes(C.byref(args))
+        args = _lib.LinearArgs(
+            x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, 0, None, 0, _p(pre2), 0 if pre2 is None else pre2.stride(0),
+            dy2.data_ptr(), dy2.stride(0), _p(dx), k, _p(dweight), k, _p(dbias), None, 0, m, n, k, _TYPES[dt], act)
+        ref = C.byref(args)
+        nbytes = l.bxl_linear_act_bwd_workspace_bytes(ref)
         if nbytes:
-            ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-            args.workspace, args.workspace_bytes = _p(ws), nbytes
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
         count = C.c_int(0)
-        rc = l.bxl_linear_act_bwd(C.byref(args), C.byref(count), _stream())
-        _lib.check(rc, l, kernels=count.value)
+        _lib.check(l.bxl_linear_act_bwd(ref, C.byref(count), _stream()), l, kernels=0)
+        _lib.launches += count.value
     return dx, dweight, dbias
 
 
@@ -545,18 +573,18 @@ def layernorm(x, gamma, beta, eps):
     return out
 
 
-def _norm_operands(name, x, weight, bias, *like_x):
-    _on_current_device(name, x, weight, bias, *like_x)
-    _req(x.dtype in _TYPES and x.dim() >= 1 and x.shape[-1] >= 1, f"{name}: fp16, bf16 or fp32 rows of at least one element")
-    for t in like_x:
-        _req(t.shape == x.shape and t.dtype == x.dtype, f"{name}: dy must have the shape and type of x")
-    pt = x.dtype
-    for t in (weight, bias):
-        if t is not None:
-            pt = t.dtype
-            _req(t.shape == x.shape[-1:] and t.is_contiguous() and pt in (x.dtype, torch.float32),
-                 f"{name}: weight and bias must be contiguous [C] vectors in the type of x or in fp32")
-    _req(weight is None or bias is None or weight.dtype == bias.dtype, f"{name}: weight and bias must share a type")
+def _norm_operands(name, x):
+    dev, shape = _here(name, x), x.shape
+    if x.dtype not in _TYPES or len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"{name}: expected fp16, bf16 or fp32 rows of at least one element, got {x.dtype} {list(shape)}")
+    return dev, x.dtype, shape, shape[-1]
+
+
+def _norm_param(name, t, c, dt, dev):
+    """The type of a weight or bias vector, which is that of x or fp32."""
+    pt = t.dtype
+    if t.shape != (c,) or not t.is_contiguous() or (pt != dt and pt != torch.float32) or t.device != dev:
+        raise ValueError(f"{name}: weight and bias must be contiguous [{c}] vectors in the type of x or in fp32, on its device")
     return pt
 
 
@@ -564,50 +592,67 @@ def layernorm_fwd(x, weight=None, bias=None, eps: float = 1e-5, out=None, want_s
     """LayerNorm over the last axis of ``x`` (fp16, bf16 or fp32, any width); ``weight`` and ``bias`` in its type or in
     fp32, either may be absent.  ``out`` (which may be ``x``) receives the result.  ``want_stats`` also returns the
     rows' fp32 ``mean`` and ``rstd``, the input of :func:`layernorm_bwd`."""
-    pt = _norm_operands("layernorm_fwd", x, weight, bias)
-    c = x.shape[-1]
+    dev, dt, shape, c = _norm_operands("layernorm_fwd", x)
+    pt = dt
+    if weight is not None:
+        pt = _norm_param("layernorm_fwd", weight, c, dt, dev)
+    if bias is not None:
+        bt = _norm_param("layernorm_fwd", bias, c, dt, dev)
+        _req(weight is None or bt == pt, "layernorm_fwd: weight and bias must share a type")
+        pt = bt
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
-        _on_current_device("layernorm_fwd", out)
-        _req(out.shape == x.shape and out.dtype == x.dtype and out.is_contiguous(), "layernorm_fwd: out must be contiguous, in the shape and type of x")
+        _like("layernorm_fwd", out, "out", shape, dt, dev)
+        _req(out.is_contiguous(), "layernorm_fwd: out must be contiguous")
     rows = x.numel() // c
-    stats = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32) if want_stats else None
+    mean = rstd = None
+    if want_stats:
+        mean = x.new_empty(shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     if rows:
         x2 = _rows(x)
         l = _lib.lib()
         _lib.check(
-            l.bxl_layernorm_fwd(_p(x2), x2.stride(0), _p(weight), _p(bias), _p(out), c, _p(stats), stats.data_ptr() + 4 * rows if want_stats else None,
-                                rows, c, _TYPES[x.dtype], _TYPES[pt], float(eps), _stream()),
+            l.bxl_layernorm_fwd(x2.data_ptr(), x2.stride(0), _p(weight), _p(bias), out.data_ptr(), c, _p(mean), _p(rstd), rows, c, _TYPES[dt], _TYPES[pt],
+                                eps, _stream()),
             l,
         )
-    return (out, stats[0], stats[1]) if want_stats else out
+    return (out, mean, rstd) if want_stats else out
 
 
 def layernorm_bwd(dy, x, mean, rstd, weight=None, want_dweight: bool = True, want_dbias: bool = True):
     """Gradients ``(dx, dweight, dbias)`` of :func:`layernorm_fwd`, given that of its result and the ``mean`` and ``rstd``
     it returned.  ``dweight`` and ``dbias`` have the type of ``weight`` (that of ``x`` without one) and are ``None`` where
     they are not wanted; ``dweight`` is ``None`` without a ``weight``."""
-    pt = _norm_operands("layernorm_bwd", x, weight, None, dy)
-    _on_current_device("layernorm_bwd", mean, rstd)
+    dev, dt, shape, c = _norm_operands("layernorm_bwd", x)
+    _like("layernorm_bwd", dy, "dy", shape, dt, dev)
     for t in (mean, rstd):
-        _req(t.dtype == torch.float32 and t.shape == x.shape[:-1] and t.is_contiguous(), "layernorm_bwd: mean and rstd must be contiguous fp32, one value per row of x")
-    c = x.shape[-1]
+        if t.dtype != torch.float32 or t.shape != shape[:-1] or t.device != dev or not t.is_contiguous():
+            raise ValueError("layernorm_bwd: mean and rstd must be contiguous fp32, one value per row of x, on its device")
+    pt = dt
+    if weight is not None:
+        pt = _norm_param("layernorm_bwd", weight, c, dt, dev)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dweight = torch.empty_like(weight) if want_dweight and weight is not None else None
+    dbias = (x.new_empty(c) if weight is None else torch.empty_like(weight)) if want_dbias else None
     rows = x.numel() // c
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    new = torch.empty if rows else torch.zeros
-    dweight = new(c, device=x.device, dtype=pt) if want_dweight and weight is not None else None
-    dbias = new(c, device=x.device, dtype=pt) if want_dbias else None
     if rows:
         dy2, x2 = _rows(dy), _rows(x)
         l = _lib.lib()
-        params = dweight is not None or dbias is not None
-        ws = torch.empty(l.bxl_layernorm_bwd_workspace_bytes(rows, c), device=x.device, dtype=torch.uint8) if params else None
+        ws, nbytes = None, 0
+        if dweight is not None or dbias is not None:
+            nbytes = l.bxl_layernorm_bwd_workspace_bytes(rows, c)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
         _lib.check(
-            l.bxl_layernorm_bwd(_p(dy2), dy2.stride(0), _p(x2), x2.stride(0), _p(mean), _p(rstd), _p(weight), _p(dx), c, _p(dweight), _p(dbias),
-                                rows, c, _TYPES[x.dtype], _TYPES[pt], _p(ws), ws.numel() if params else 0, _stream()),
-            l, kernels=2 if params else 1,
+            l.bxl_layernorm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), mean.data_ptr(), rstd.data_ptr(), _p(weight), dx.data_ptr(), c,
+                                _p(dweight), _p(dbias), rows, c, _TYPES[dt], _TYPES[pt], _p(ws), nbytes, _stream()),
+            l, kernels=2 if nbytes else 1,
         )
+    else:
+        for t in (dweight, dbias):
+            if t is not None:
+                t.zero_()
     return dx, dweight, dbias
 
 
