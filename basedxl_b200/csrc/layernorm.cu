@@ -10,8 +10,6 @@
 // variance is taken of the differences from the mean.  dw and db: every thread keeps the sums of its own columns over
 // all rows that it meets, a block adds those of its threads, and a second launch adds the blocks' in a fixed order (no
 // atomics).
-#include <stdlib.h>
-
 #include "bxl_common.cuh"
 #include "bxl_host.h"
 #include "bxl_types.cuh"
@@ -266,14 +264,14 @@ __device__ __forceinline__ void add_lanes(float (&v)[K], int o) {
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
 }
-template <int K>
+template <int K, bool kSub>
 __device__ __forceinline__ bool team_sum(float (&v)[K], const LnTeams& t, const TeamRole& me, float* slots, int turn, bool failed) {
-  if (t.TL > 16) add_lanes<K>(v, 16);
-  if (t.TL > 8) add_lanes<K>(v, 8);
+  if (!kSub || t.TL > 16) add_lanes<K>(v, 16);
+  if (!kSub || t.TL > 8) add_lanes<K>(v, 8);
   add_lanes<K>(v, 4);
   add_lanes<K>(v, 2);
   add_lanes<K>(v, 1);
-  if (me.warps == 1) return failed;
+  if constexpr (kSub) return failed;
   float* s = slots + (me.team * 2 + turn) * me.warps * K;
   if ((threadIdx.x & 31) == 0) {
 #pragma unroll
@@ -320,7 +318,7 @@ __device__ __forceinline__ bool has_vector(int i, int v, int n) {
 }
 
 // The ring of a team: what its first warp fills and all of it waits on.
-template <class T, int VEC, int MATS>
+template <class T, int VEC, int MATS, bool kSub>
 struct TeamRing {
   const LnArgs& a;
   const LnTeams& t;
@@ -348,8 +346,8 @@ struct TeamRing {
   }
   __device__ __forceinline__ void load(long long unit, int st) {
     if (unit >= t.units) return;
-    const long long row0 = unit * t.rows;
-    load_stage<T, VEC, MATS>(src, ld, a, t, row0, (int)min((long long)t.rows, a.rows - row0), base + st * MATS * t.mat_bytes, bars + 8 * st);
+    const long long row0 = kSub ? unit * t.rows : unit;
+    load_stage<T, VEC, MATS>(src, ld, a, t, row0, kSub ? (int)min((long long)t.rows, a.rows - row0) : 1, base + st * MATS * t.mat_bytes, bars + 8 * st);
   }
   __device__ __forceinline__ bool wait(int site) { return mbar_wait_warp(bars + 8 * stage, phase, abort_flag, t.dev_status, site); }
   __device__ __forceinline__ const T* mat(int m, long long row0) const {
@@ -362,14 +360,15 @@ struct TeamRing {
   }
 };
 
-template <class T, int VEC, int NV>
+// kSub: teams of a warp or less.
+template <class T, int VEC, int NV, bool kSub>
 __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_teams_kernel(const LnArgs a, const LnTeams t) {
   pdl_launch_dependents();
   using F = typename Lanes<VEC>::F;
   constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(128) uint8_t smem[];
   const TeamRole me(t.TL);
-  TeamRing<T, VEC, 1> ring(a, t, smem, me);
+  TeamRing<T, VEC, 1, kSub> ring(a, t, smem, me);
   float* slots = reinterpret_cast<float*>(smem + t.off_red);
   const int n = a.C / VEC;
   const long long first = blockIdx.x * (long long)me.teams + me.team;
@@ -388,11 +387,11 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
   }
   bool failed = false;
   for (long long unit = first; unit < t.units; unit += ring.step) {
-    const long long row0 = unit * t.rows, row = row0 + me.sub;
-    const bool in = row < a.rows;
+    const long long row0 = kSub ? unit * t.rows : unit, row = row0 + (kSub ? me.sub : 0);
+    const bool in = !kSub || row < a.rows;
     failed = !ring.wait(700);
-    if (failed && me.warps == 1) break;
-    const T* xs = ring.mat(0, row0) + me.sub * a.C;
+    if (kSub && failed) break;
+    const T* xs = ring.mat(0, row0) + (kSub ? me.sub * a.C : 0);
     F x[NV][N];
     F s[2] = {splat<F>(0.f), splat<F>(0.f)};   // two chains of additions
 #pragma unroll
@@ -405,7 +404,7 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
       }
     }
     float sum[1] = {total(add(s[0], s[1]))};
-    failed = team_sum<1>(sum, t, me, slots, 0, failed);
+    failed = team_sum<1, kSub>(sum, t, me, slots, 0, failed);
     if (failed) break;
     // the stage has been read by the whole team
     __syncwarp();
@@ -425,7 +424,7 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
       }
     }
     sum[0] = total(add(s[0], s[1]));
-    team_sum<1>(sum, t, me, slots, 1, false);
+    team_sum<1, kSub>(sum, t, me, slots, 1, false);
     const float rstd = rsqrtf(sum[0] * a.inv_c + a.eps);
     if (in) {
       const F scale = splat<F>(rstd);
@@ -446,14 +445,14 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
 }
 
 // ---- backward --------------------------------------------------------------------------------
-template <class T, int VEC, int NV>
+template <class T, int VEC, int NV, bool kSub>
 __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnArgs a, const LnTeams t) {
   pdl_launch_dependents();
   using F = typename Lanes<VEC>::F;
   constexpr int N = Lanes<VEC>::N;
   extern __shared__ __align__(128) uint8_t smem[];
   const TeamRole me(t.TL);
-  TeamRing<T, VEC, 2> ring(a, t, smem, me);
+  TeamRing<T, VEC, 2, kSub> ring(a, t, smem, me);
   float* slots = reinterpret_cast<float*>(smem + t.off_red);
   float* sw = reinterpret_cast<float*>(smem + t.off_w);
   const int n = a.C / VEC;
@@ -474,43 +473,40 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
   auto moments = [&](long long row) {
     if (row < a.rows) mean_next = a.mean[row], rstd_next = a.rstd[row];
   };
-  moments(first * t.rows + me.sub);
+  moments(kSub ? first * t.rows + me.sub : first);
   __syncthreads();
   bool failed = false;
   int turn = 0;
   for (long long unit = first; unit < t.units; unit += ring.step, turn ^= 1) {
-    const long long row0 = unit * t.rows, row = row0 + me.sub;
-    const bool in = row < a.rows;
+    const long long row0 = kSub ? unit * t.rows : unit, row = row0 + (kSub ? me.sub : 0);
+    const bool in = !kSub || row < a.rows;
     failed = !ring.wait(701);
-    if (failed && me.warps == 1) break;
-    const T* xs = ring.mat(0, row0) + me.sub * a.C;
-    const T* ds = ring.mat(1, row0) + me.sub * a.C;
-    F x[NV][N];                          // x - mean
-    Vec<T, VEC> raw[NV];                 // dy, as loaded: widened twice, at half the registers
+    if (kSub && failed) break;
+    const T* xs = ring.mat(0, row0) + (kSub ? me.sub * a.C : 0);
+    const T* ds = ring.mat(1, row0) + (kSub ? me.sub * a.C : 0);
+    Vec<T, VEC> rx[NV], rd[NV];          // as loaded, and widened twice: registers bound this kernel
     const float mean = mean_next, rstd = rstd_next;
-    moments((unit + ring.step) * t.rows + me.sub);
+    moments(kSub ? (unit + ring.step) * t.rows + me.sub : unit + ring.step);
     F s1 = splat<F>(0.f), s2 = s1;       // sum(g), sum(g (x - mean))
     const F minus = splat<F>(-mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = me.lane + i * t.TL;
       if (in && has_vector<VEC, NV>(i, v, n)) {
-        F w[N], d[N];
-        widen<T, VEC>(load_vec<T, VEC>(xs + v * VEC), x[i]);
-        raw[i] = load_vec<T, VEC>(ds + v * VEC);
-        widen<T, VEC>(raw[i], d);
+        F w[N], d[N], x[N];
+        rx[i] = load_vec<T, VEC>(xs + v * VEC), rd[i] = load_vec<T, VEC>(ds + v * VEC);
+        widen<T, VEC>(rx[i], x), widen<T, VEC>(rd[i], d);
         shared_param<VEC>(sw, n, v, w);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const F g = mul(d[j], w[j]);
-          x[i][j] = add(x[i][j], minus);
           s1 = add(s1, g);
-          s2 = fma(g, x[i][j], s2);
+          s2 = fma(g, add(x[j], minus), s2);
         }
       }
     }
     float sum[2] = {total(s1), total(s2)};
-    failed = team_sum<2>(sum, t, me, slots, turn, failed);
+    failed = team_sum<2, kSub>(sum, t, me, slots, turn, failed);
     if (failed) break;
     __syncwarp();
     if (me.warp == 0) ring.refill(unit);   // the stage has been read by the whole team
@@ -522,18 +518,18 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
       for (int i = 0; i < NV; ++i) {
         const int v = me.lane + i * t.TL;
         if (has_vector<VEC, NV>(i, v, n)) {
-          F w[N], d[N];
-          widen<T, VEC>(raw[i], d);
+          F w[N], d[N], x[N];
+          widen<T, VEC>(rx[i], x), widen<T, VEC>(rd[i], d);
           shared_param<VEC>(sw, n, v, w);
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             // dx = dy (w r) + h c2 + c1
-            const F h = mul(x[i][j], r);
+            const F h = mul(add(x[j], minus), r);
             dw[i][j] = fma(d[j], h, dw[i][j]);
             db[i][j] = add(db[i][j], d[j]);
-            x[i][j] = fma(d[j], mul(w[j], r), fma(h, c2, c1));
+            x[j] = fma(d[j], mul(w[j], r), fma(h, c2, c1));
           }
-          store_vec<T, VEC>(out + v * VEC, narrow<T, VEC>(x[i]));
+          store_vec<T, VEC>(out + v * VEC, narrow<T, VEC>(x));
         }
       }
     }
@@ -544,8 +540,8 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
   }
   if (!a.part) return;
   // Column sums of the block: over the rows of a warp by shuffles, over teams through shared memory (the rings are empty by
-  // now), half of them at a time.
-  if (t.TL < 32) {
+  // now).
+  if constexpr (kSub) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -559,36 +555,91 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
           }
         }
   }
-  float* buf = reinterpret_cast<float*>(smem);
   float* out = a.part + blockIdx.x * 2ll * a.C;
-  for (int half = me.teams / 2;; half /= 2) {
-    float* to = half ? buf + (me.team - half) * 2 * a.C : out;
-    if ((half ? me.team >= half && me.team < 2 * half : me.team == 0) && me.sub == 0) {
+  float* to = me.teams > 1 ? reinterpret_cast<float*>(smem) + me.team * 2 * a.C : out;
+  if (me.sub == 0) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = me.lane + i * t.TL;
-        if (has_vector<VEC, NV>(i, v, n)) {
-          *reinterpret_cast<Vec<F, N>*>(to + v * VEC) = *reinterpret_cast<const Vec<F, N>*>(&dw[i]);
-          *reinterpret_cast<Vec<F, N>*>(to + a.C + v * VEC) = *reinterpret_cast<const Vec<F, N>*>(&db[i]);
-        }
+    for (int i = 0; i < NV; ++i) {
+      const int v = me.lane + i * t.TL;
+      if (has_vector<VEC, NV>(i, v, n)) {
+        *reinterpret_cast<Vec<F, N>*>(to + v * VEC) = *reinterpret_cast<const Vec<F, N>*>(&dw[i]);
+        *reinterpret_cast<Vec<F, N>*>(to + a.C + v * VEC) = *reinterpret_cast<const Vec<F, N>*>(&db[i]);
       }
     }
-    if (half == 0) break;
-    __syncthreads();
-    if (me.team < half && me.sub == 0) {
-      const float* from = buf + me.team * 2 * a.C;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = me.lane + i * t.TL;
-        if (has_vector<VEC, NV>(i, v, n)) {
-          const Vec<F, N> p = *reinterpret_cast<const Vec<F, N>*>(from + v * VEC), q = *reinterpret_cast<const Vec<F, N>*>(from + a.C + v * VEC);
-#pragma unroll
-          for (int j = 0; j < N; ++j) dw[i][j] = add(dw[i][j], p.v[j]), db[i][j] = add(db[i][j], q.v[j]);
-        }
-      }
-    }
-    __syncthreads();
   }
+  if (me.teams == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.C; c += kTeamThreads) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < me.teams; ++k) s += reinterpret_cast<const float*>(smem)[k * 2 * a.C + c];
+    out[c] = s;
+  }
+}
+
+// Few rows, in one launch: the first `a.rows` blocks form a row of dx each, the others 32 columns of dw and db each.  Both read x
+// and dy, which by then lie in L2; no partial sums, no second launch (154 x 2048: 7.5 -> 2.8 us; 512 x 1280: 8.0 -> 7.4, 1024 x
+// 1280: 8.7 against 14.2).
+constexpr int kSmallThreads = 512, kSmallRows = 512;
+template <class T, class P, int VEC>
+__global__ void __launch_bounds__(kSmallThreads) ln_bwd_small_kernel(const LnArgs a, P* dweight, P* dbias) {
+  pdl_launch_dependents();
+  using F = typename Lanes<VEC>::F;
+  constexpr int N = Lanes<VEC>::N, kWarps = kSmallThreads / 32;
+  __shared__ float red[2][kWarps][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  if (blockIdx.x < a.rows) {
+    const long long r = blockIdx.x;
+    const Param<T> w{a.weight, a.param_f32};
+    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
+    const T* dr = static_cast<const T*>(a.dy) + r * a.lddy;
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    const F minus = splat<F>(-mean);
+    const int n = a.C / VEC;
+    F s1 = splat<F>(0.f), s2 = s1;
+    for (int v = threadIdx.x; v < n; v += kSmallThreads) {
+      F x[N], d[N], wv[N];
+      widen<T, VEC>(load_vec<T, VEC>(xr + v * VEC), x), widen<T, VEC>(load_vec<T, VEC>(dr + v * VEC), d);
+      w.template get<VEC>(v * VEC, 1.f, wv);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const F g = mul(d[j], wv[j]);
+        s1 = add(s1, g);
+        s2 = fma(g, add(x[j], minus), s2);
+      }
+    }
+    const float t1 = block_sum(total(s1), red[0][0]) * a.inv_c, t2 = block_sum(total(s2), red[1][0]) * a.inv_c;
+    const F rs = splat<F>(rstd), c1 = splat<F>(-rstd * t1), c2 = splat<F>(-rstd * (rstd * t2));
+    T* out = static_cast<T*>(a.y) + r * a.ldy;
+    for (int v = threadIdx.x; v < n; v += kSmallThreads) {
+      F x[N], d[N], wv[N];
+      widen<T, VEC>(load_vec<T, VEC>(xr + v * VEC), x), widen<T, VEC>(load_vec<T, VEC>(dr + v * VEC), d);
+      w.template get<VEC>(v * VEC, 1.f, wv);
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = fma(d[j], mul(wv[j], rs), fma(mul(add(x[j], minus), rs), c2, c1));
+      store_vec<T, VEC>(out + v * VEC, narrow<T, VEC>(x));
+    }
+    return;
+  }
+  const int c = (blockIdx.x - static_cast<int>(a.rows)) * 32 + lane;
+  float dw = 0.f, db = 0.f;
+  if (c < a.C) {
+#pragma unroll 8
+    for (int r = warp; r < a.rows; r += kWarps) {
+      const float d = to_f32(static_cast<const T*>(a.dy)[r * a.lddy + c]);
+      dw = fmaf(d, (to_f32(static_cast<const T*>(a.x)[r * a.ldx + c]) - a.mean[r]) * a.rstd[r], dw);
+      db += d;
+    }
+  }
+  red[0][warp][lane] = dw, red[1][warp][lane] = db;
+  __syncthreads();
+  P* out = warp == 0 ? dweight : dbias;
+  if (warp > 1 || c >= a.C || !out) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) v += red[warp][k][lane];
+  out[c] = from_f32<P>(v);
 }
 
 // Rows that the teams do not take: dx alone, two passes over the row.
@@ -645,6 +696,7 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* part, i
   if (!out) return;
   float v = 0.f;
   if (c < C)
+#pragma unroll 8
     for (int i = warp; i < count; i += warps) v += part[i * pitch + blockIdx.y * (long long)C + c];
   s[warp][lane] = v;
   __syncthreads();
@@ -681,6 +733,7 @@ static int allow_smem(int bytes) {
 constexpr int kLnMaxC = 1 << 30;   // column indices, and a step past the last one, are ints
 // Blocks of the backward pass, at most: each leaves one row of column sums.
 static long long ln_bwd_blocks(long long rows) {
+  if (rows <= kSmallRows) return 0;
   const long long most = sm_count() * 2ll;
   return rows < most ? rows : most;
 }
@@ -704,7 +757,7 @@ static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats,
   t.TL = TL, t.rows = TL < 32 ? 32 / TL : 1, t.units = (a.rows + t.rows - 1) / t.rows;
   t.mat_bytes = (int)((t.rows * row + 15) / 16 * 16 + (vec == 1 ? 32 : 0));   // a widened span begins and ends up to 15 bytes further out
   const long long slots = 2ll * kTeamWarps * mats * 4, rest = params + slots + teams * 8 * 8 + 512;
-  const long long scratch = sums ? teams / 2 * 2ll * a.C * 4 : 0;
+  const long long scratch = sums && teams > 1 ? teams * 2ll * a.C * 4 : 0;
   long long stages = (room - rest) / ((long long)teams * mats * t.mat_bytes);
   if (stages > 8) stages = 8;
   if (stages < 2 || scratch > room - rest) return false;
@@ -722,10 +775,12 @@ static int team_blocks(const LnTeams& t, int per_sm) {
   return (int)(need < most ? need : most);
 }
 
-template <class T, int VEC, int NV>
+template <class T, int VEC, int NV, bool kSub = false>
 static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
-  if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV>>(kSmemSm)) return rc;
-  return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
+  if constexpr (!kSub)
+    if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, true>(a, t, smem, s);
+  if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kSub>>(kSmemSm)) return rc;
+  return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV, kSub>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
 }
 template <class T, int VEC>
 static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
@@ -768,9 +823,9 @@ static int ln_fwd_launch(const LnArgs& a, int threads, cudaStream_t s) {
 template <class T>
 static int ln_fwd(const LnArgs& a, bool vec, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T), W = kLnWarps * 32;
-  const char* e = getenv("LN_FEW");
-  const long long few = e ? atoll(e) : 2048;
-  if (a.rows > few) {
+  // Few values: a block's ring costs more than it brings (1024 x 640: 3.0 us without, 3.4 with; 4096 x 320: 4.3 and 3.8).
+  const long long few = vec ? 1 << 20 : 1 << 18;
+  if (a.rows * a.C > few) {
     bool done = false;
     if (int rc = vec ? ln_fwd_teams<T, V>(a, done, s) : ln_fwd_teams<T, 1>(a, done, s)) return rc;
     if (done) return kOk;
@@ -793,17 +848,20 @@ static int ln_fwd(const LnArgs& a, bool vec, cudaStream_t s) {
   return launch_kernel("ln_fwd_long_kernel launch", ln_fwd_long_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, s, 1, a);
 }
 
-template <class T, int VEC, int NV>
+template <class T, int VEC, int NV, bool kSub = false>
 static int ln_bwd_teams_launch(const LnArgs& a, const LnTeams& t, int blocks, int smem, cudaStream_t s) {
-  if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV>>(kSmemSm)) return rc;
-  return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
+  if constexpr (!kSub)
+    if (t.TL <= 32) return ln_bwd_teams_launch<T, VEC, NV, true>(a, t, blocks, smem, s);
+  if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV, kSub>>(kSmemSm)) return rc;
+  return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV, kSub>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
 }
 template <class T, int VEC>
 static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s) {
   LnTeams t = {};
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
-  const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 6, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
+  // Vectors a thread holds: 24 values of 16 bits or 16 of fp32 (8192 x 5120: 96 us with 24, 86 with 16); wider rows spill.
+  const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 4, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
   done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
                                          plan_teams(t, a, sizeof(T), VEC, 2, wide, 4ll * a.C, true, kSmemSm, nv, smem));
   if (!done) return kOk;
@@ -830,6 +888,14 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
   }
 }
 
+template <class T, class P>
+static int ln_bwd_small(const LnArgs& a, bool vec, void* dweight, void* dbias, cudaStream_t s) {
+  const dim3 grid((unsigned)a.rows + (dweight || dbias ? (a.C + 31) / 32 : 0));
+  constexpr int V = 16 / sizeof(T);
+  P *dw = static_cast<P*>(dweight), *db = static_cast<P*>(dbias);
+  if (vec) return launch_kernel("ln_bwd_small_kernel launch", ln_bwd_small_kernel<T, P, V>, grid, dim3(kSmallThreads), 0, s, 1, a, dw, db);
+  return launch_kernel("ln_bwd_small_kernel launch", ln_bwd_small_kernel<T, P, 1>, grid, dim3(kSmallThreads), 0, s, 1, a, dw, db);
+}
 template <class T>
 static int ln_bwd(const LnArgs& a, bool vec, int& blocks, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
@@ -895,7 +961,7 @@ extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, 
       (reinterpret_cast<uintptr_t>(mean) | reinterpret_cast<uintptr_t>(rstd)) % 4)
     return fail(kErrInvalidArg, "bxl_layernorm_bwd: pointers must be aligned to their elements");
   const bool params = dweight || dbias;
-  if (params) {
+  if (params && ln_bwd_blocks(rows)) {
     if (!workspace || !al16(workspace)) return fail(kErrInvalidArg, "bxl_layernorm_bwd: workspace must be 16-byte aligned");
     if (workspace_bytes < bxl_layernorm_bwd_workspace_bytes(rows, C)) return fail(kErrTooLarge, "bxl_layernorm_bwd: workspace too small");
   }
@@ -905,6 +971,12 @@ extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, 
   a.rows = rows, a.C = C, a.param_f32 = param_dtype == BXL_F32, a.inv_c = 1.f / (float)C;
   const bool vec = rows_of_vectors(x, ldx, C, b) && rows_of_vectors(dy, lddy, C, b) && rows_of_vectors(dx, lddx, C, b) && al16(weight);
   cudaStream_t s = (cudaStream_t)stream;
+  if (!ln_bwd_blocks(rows)) {
+    a.part = nullptr;
+    if (dtype == BXL_F32) return ln_bwd_small<float, float>(a, vec, dweight, dbias, s);
+    if (dtype == BXL_F16) return param_dtype == BXL_F32 ? ln_bwd_small<__half, float>(a, vec, dweight, dbias, s) : ln_bwd_small<__half, __half>(a, vec, dweight, dbias, s);
+    return param_dtype == BXL_F32 ? ln_bwd_small<__nv_bfloat16, float>(a, vec, dweight, dbias, s) : ln_bwd_small<__nv_bfloat16, __nv_bfloat16>(a, vec, dweight, dbias, s);
+  }
   int blocks = 0, rc;
   if (dtype == BXL_F16) rc = ln_bwd<__half>(a, vec, blocks, s);
   else if (dtype == BXL_BF16) rc = ln_bwd<__nv_bfloat16>(a, vec, blocks, s);

@@ -643,7 +643,8 @@ def layernorm_bwd(dy, x, mean, rstd, weight=None, want_dweight: bool = True, wan
         ws, nbytes = None, 0
         if dweight is not None or dbias is not None:
             nbytes = l.bxl_layernorm_bwd_workspace_bytes(rows, c)
-            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            if nbytes:
+                ws = x.new_empty(nbytes, dtype=torch.uint8)
         _lib.check(
             l.bxl_layernorm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), mean.data_ptr(), rstd.data_ptr(), _p(weight), dx.data_ptr(), c,
                                 _p(dweight), _p(dbias), rows, c, _TYPES[dt], _TYPES[pt], _p(ws), nbytes, _stream()),

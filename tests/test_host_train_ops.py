@@ -190,7 +190,7 @@ def test_c_layernorm_fwd_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", [{"dy": None}, {"x": None}, {"mean": None}, {"rstd": None}, {"dx": None}, {"rows": 0}, {"C": -8}, {"lddx": 8}, {"lddy": -64}, {"pt": 1},
-                                {"dtype": -1}, {"dw": P + 1}, {"dx": P + 1}, {"ws": None}, {"ws": P + 8}, {"ws_bytes": 16}])
+                                {"dtype": -1}, {"dw": P + 1}, {"dx": P + 1}, {"ws": None, "rows": 4000}, {"ws": P + 8, "rows": 4000}, {"ws_bytes": 16, "rows": 4000}])
 def test_c_layernorm_bwd_refuses(kw):
     a = {"dy": P, "lddy": 64, "x": P, "ldx": 64, "mean": P, "rstd": P, "w": P, "dx": P, "lddx": 64, "dw": P, "db": P, "rows": 4, "C": 64, "dtype": 0, "pt": 0,
          "ws": P, "ws_bytes": 1 << 20, **kw}
