@@ -1,48 +1,123 @@
-// Activations of the linear layers and their derivatives, in fp32 on the unrounded pre-activation.
+// Activations of the linear layers and their derivatives, in fp32 on the unrounded pre-activation, one value or a pair (F2) at
+// a time.
 //
-// The sigmoid forms (silu, quick_gelu, and gelu with tanh: z (1 + tanh(u/2)) / 2 = z sigmoid(u)) take the fast exponential
-// and division, whose errors are 2^-21 of the value: far below the 2^-12 of an fp16 result.  Factors that stand beside a
-// vanishing one are clamped first, so that infinite pre-activations give the limits (0, z; derivatives 0 and 1) and not
-// 0 * inf; NaN stays NaN through the other factor.
+// silu, quick_gelu and gelu with tanh are z sigmoid(u), since (1 + tanh(u / 2)) / 2 = sigmoid(u); they take the fast
+// exponential and reciprocal, whose errors are 2^-21 of the value, far below the 2^-12 of an fp16 result.  gelu with erf takes
+// the normal distribution's tail below, to 1e-7.  Factors that stand beside a vanishing one are clamped, so that infinite
+// pre-activations give the limits (0 and z; derivatives 0 and 1) and not 0 * inf; the clamps pass NaN on.
 #pragma once
-#include "../../include/basedxl_b200.h"
+#include "bxl_types.cuh"
 
 namespace bxl {
 
-__device__ __forceinline__ float sigmoid_f32(float u) { return __fdividef(1.f, 1.f + __expf(-u)); }
-// u of gelu with tanh: 2 sqrt(2 / pi) (z + 0.044715 z^3)
-__device__ __forceinline__ float gelu_tanh_argument(float z) { return z * fmaf(0.07135481627260025f * z, z, 1.5957691216057308f); }
-
-template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  const float zc = fmaxf(z, -1e30f);   // -inf * 0
-  if constexpr (ACT == BXL_ACT_RELU) return z < 0.f ? 0.f : z;
-  else if constexpr (ACT == BXL_ACT_SILU) return __fdividef(zc, 1.f + __expf(-z));
-  else if constexpr (ACT == BXL_ACT_GELU) return 0.5f * zc * (1.f + erff(z * 0.70710678118654752f));
-  else if constexpr (ACT == BXL_ACT_GELU_TANH) return __fdividef(zc, 1.f + __expf(-gelu_tanh_argument(z)));
-  else if constexpr (ACT == BXL_ACT_QUICK_GELU) return __fdividef(zc, 1.f + __expf(-1.702f * z));
-  else return z;
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float magnitude(float a) { return fabsf(a); }
+__device__ __forceinline__ float if_negative(float z, float a, float b) { return z < 0.f ? a : b; }
+// ... and of pairs, for what has no instruction for two
+#define BXL_ON_PAIRS(name)                                             \
+  __device__ __forceinline__ F2 name(F2 a) {                           \
+    const float2 u = split(a);                                         \
+    return f2(name(u.x), name(u.y));                                   \
+  }
+BXL_ON_PAIRS(rcp_approx)
+BXL_ON_PAIRS(exp2_approx)
+BXL_ON_PAIRS(magnitude)
+#undef BXL_ON_PAIRS
+__device__ __forceinline__ F2 min_nan(F2 a, float b) {
+  const float2 u = split(a);
+  return f2(min_nan(u.x, b), min_nan(u.y, b));
+}
+__device__ __forceinline__ F2 max_nan(F2 a, float b) {
+  const float2 u = split(a);
+  return f2(max_nan(u.x, b), max_nan(u.y, b));
+}
+__device__ __forceinline__ F2 if_negative(F2 z, F2 a, F2 b) {
+  const float2 u = split(z), v = split(a), w = split(b);
+  return f2(if_negative(u.x, v.x, w.x), if_negative(u.y, v.y, w.y));
 }
 
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  const float zc = fminf(fmaxf(z, -1e3f), 1e3f);   // beyond it the factors beside it are exactly 0
-  if constexpr (ACT == BXL_ACT_RELU) {
-    return z > 0.f ? 1.f : z == z ? 0.f : z;
+// Phi(-a) of the normal distribution, a >= 0, by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: with
+// t = 1 / (1 + p y), erfc(y) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-y^2) + error, |error| <= 1.5e-7, at y = a / sqrt(2).
+// One reciprocal and one exponential, which the density takes too (`e` = exp(-a^2 / 2)).
+template <class F>
+__device__ __forceinline__ F normal_tail(F a, F& e) {
+  const F t = rcp_approx(fma(splat<F>(0.3275911f * 0.70710678118654752f), a, splat<F>(1.f)));
+  e = exp2_approx(mul(mul(a, a), splat<F>(-0.72134752044448170f)));   // log2(e) / 2
+  F p = fma(t, splat<F>(0.5f * 1.061405429f), splat<F>(0.5f * -1.453152027f));
+  p = fma(t, p, splat<F>(0.5f * 1.421413741f));
+  p = fma(t, p, splat<F>(0.5f * -0.284496736f));
+  p = fma(t, p, splat<F>(0.5f * 0.254829592f));
+  return mul(mul(p, t), e);
+}
+// exp(-u) of sigmoid(u) = 1 / (1 + exp(-u))
+template <int ACT, class F>
+__device__ __forceinline__ F exp_minus_argument(F z) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  if constexpr (ACT == BXL_ACT_SILU) return exp2_approx(mul(z, splat<F>(-kLog2e)));
+  else if constexpr (ACT == BXL_ACT_QUICK_GELU) return exp2_approx(mul(z, splat<F>(-1.702f * kLog2e)));
+  else  // gelu with tanh: u = 2 sqrt(2 / pi) (z + 0.044715 z^3)
+    return exp2_approx(mul(z, fma(mul(z, z), splat<F>(-0.07135481627260025f * kLog2e), splat<F>(-1.5957691216057308f * kLog2e))));
+}
+
+template <int ACT, class F>
+__device__ __forceinline__ F act_value(F z) {
+  if constexpr (ACT == BXL_ACT_NONE) {
+    return z;
+  } else if constexpr (ACT == BXL_ACT_RELU) {
+    return max_nan(z, 0.f);
   } else if constexpr (ACT == BXL_ACT_GELU) {
-    // Phi(z) + z phi(z)
-    return fmaf(zc, 0.3989422804014327f * __expf(-0.5f * zc * zc), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
-  } else if constexpr (ACT == BXL_ACT_SILU) {
-    const float s = sigmoid_f32(z);
-    return fmaf(zc * s, 1.f - s, s);
-  } else if constexpr (ACT == BXL_ACT_QUICK_GELU) {
-    const float s = sigmoid_f32(1.702f * z);
-    return fmaf(1.702f * zc * s, 1.f - s, s);
-  } else if constexpr (ACT == BXL_ACT_GELU_TANH) {
-    const float s = sigmoid_f32(gelu_tanh_argument(z));
-    return fmaf(zc * s * (1.f - s), fmaf(0.2140644488178008f * zc, zc, 1.5957691216057308f), s);
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|): nothing cancels on either side
+    const F a = min_nan(magnitude(z), 1e3f);
+    F e;
+    const F q = normal_tail(a, e);
+    return fma(mul(a, splat<F>(-1.f)), q, max_nan(z, 0.f));
   } else {
-    return 1.f;
+    return mul(max_nan(z, -1e30f), rcp_approx(add(exp_minus_argument<ACT>(z), splat<F>(1.f))));
+  }
+}
+
+template <int ACT, class F>
+__device__ __forceinline__ F act_slope(F z) {
+  if constexpr (ACT == BXL_ACT_NONE) {
+    return splat<F>(1.f);
+  } else if constexpr (ACT == BXL_ACT_RELU) {
+    // 0 or 1; 0 * z keeps a NaN
+    const F zero = mul(min_nan(max_nan(z, -1.f), 1.f), splat<F>(0.f));
+    return add(zero, if_negative(mul(z, splat<F>(-1.f)), splat<F>(1.f), splat<F>(0.f)));
+  } else if constexpr (ACT == BXL_ACT_GELU) {
+    // Phi(z) + z phi(z): of s = Phi(-a) - a phi(a) it is s on the left and 1 - s on the right
+    const F a = min_nan(magnitude(z), 1e3f);
+    F e;
+    const F q = normal_tail(a, e);
+    const F s = fma(mul(a, splat<F>(-0.3989422804014327f)), e, q);
+    return if_negative(z, s, fma(s, splat<F>(-1.f), splat<F>(1.f)));
+  } else {
+    // s + z s (1 - s) du/dz; beyond the clamps s (1 - s) is exactly 0
+    const F zc = min_nan(max_nan(z, -1e3f), 1e3f);
+    const F s = rcp_approx(add(exp_minus_argument<ACT>(z), splat<F>(1.f)));
+    const F rest = mul(mul(zc, s), fma(s, splat<F>(-1.f), splat<F>(1.f)));
+    if constexpr (ACT == BXL_ACT_SILU) return add(s, rest);
+    else if constexpr (ACT == BXL_ACT_QUICK_GELU) return fma(rest, splat<F>(1.702f), s);
+    else return fma(rest, fma(mul(zc, zc), splat<F>(0.2140644488178008f), splat<F>(1.5957691216057308f)), s);
   }
 }
 
@@ -51,8 +126,8 @@ template <int ACT>
 struct ActTag {
   static constexpr int value = ACT;
 };
-template <class F>
-__host__ __device__ __forceinline__ void with_act(int act, F&& f) {
+template <class Fn>
+__host__ __device__ __forceinline__ void with_act(int act, Fn&& f) {
   switch (act) {
     case BXL_ACT_RELU: f(ActTag<BXL_ACT_RELU>{}); break;
     case BXL_ACT_SILU: f(ActTag<BXL_ACT_SILU>{}); break;

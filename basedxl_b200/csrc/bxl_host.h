@@ -24,10 +24,10 @@ int fail(int code, const char* fmt, ...);          // records the message, retur
 int check_cuda(cudaError_t e, const char* what);   // kOk or kErrCuda (+ message)
 int* device_status_ptr();                          // per-device status word (3 ints), nullptr on failure
 
-// 16-bit (fp16) tiled tensor map with 128-byte swizzle and zero fill.
+// 16-bit (fp16) tiled tensor map with 128-byte swizzle (or 64) and zero fill.
 // dims/box: innermost first.  strides_bytes: rank-1 entries for dims 1..rank-1.
 int encode_tmap_f16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                    const uint32_t* box);
+                    const uint32_t* box, int swizzle = 128);
 
 int sm_count();
 

@@ -111,36 +111,52 @@ constexpr int kDzWarps = 8;
 template <class T, int VEC>
 __global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
   pdl_launch_dependents();
+  using F = typename Lanes<VEC>::F;
+  constexpr int N = Lanes<VEC>::N;
   __shared__ float sums[kDzWarps][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + lane) * VEC;
   const int per = (p.M + gridDim.y - 1) / gridDim.y;
   const long long r1 = min((long long)p.M, (blockIdx.y + 1ll) * per);
-  float acc[VEC];
+  F acc[N];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+  for (int j = 0; j < N; ++j) acc[j] = splat<F>(0.f);
   pdl_wait();
   if (c < p.N)
     with_act(p.act, [&](auto act) {
       constexpr int kAct = decltype(act)::value;
 #pragma unroll 4
       for (long long r = (long long)blockIdx.y * per + warp; r < r1; r += kDzWarps) {
-        const Vec<T, VEC> g = load_vec<T, VEC>(static_cast<const T*>(p.dy) + r * p.lddy + c);
-        Vec<T, VEC> z, o;
-        if constexpr (kAct != BXL_ACT_NONE) z = load_vec<T, VEC>(static_cast<const T*>(p.pre) + r * p.ldp + c);
+        F d[N];
+        widen<T, VEC>(load_vec<T, VEC>(static_cast<const T*>(p.dy) + r * p.lddy + c), d);
+        if constexpr (kAct != BXL_ACT_NONE) {
+          F z[N];
+          widen<T, VEC>(load_vec<T, VEC>(static_cast<const T*>(p.pre) + r * p.ldp + c), z);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float d = to_f32(g.v[j]);
-          if constexpr (kAct != BXL_ACT_NONE) d *= act_slope<kAct>(to_f32(z.v[j]));
-          acc[j] += d;
-          o.v[j] = from_f32<T>(d);
+          for (int j = 0; j < N; ++j) {
+            if constexpr (VEC == 1) {
+              d[j] *= act_slope<kAct>(z[j]);
+            } else {
+              const float2 u = split(z[j]);
+              d[j] = mul(d[j], f2(act_slope<kAct>(u.x), act_slope<kAct>(u.y)));
+            }
+          }
         }
-        if (p.dz) store_vec<T, VEC>(static_cast<T*>(p.dz) + r * p.ldz + c, o);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = add(acc[j], d[j]);
+        if (p.dz) store_vec<T, VEC>(static_cast<T*>(p.dz) + r * p.ldz + c, narrow<T, VEC>(d));
       }
     });
   if (!p.part) return;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sums[warp][lane + 32 * j] = acc[j];
+  for (int j = 0; j < N; ++j) {
+    if constexpr (VEC == 1) {
+      sums[warp][lane] = acc[j];
+    } else {
+      const float2 u = split(acc[j]);
+      sums[warp][lane + 64 * j] = u.x, sums[warp][lane + 64 * j + 32] = u.y;
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * VEC; i += kDzWarps * 32) {
     const int col = (blockIdx.x * 32 + i % 32) * VEC + i / 32;
