@@ -4,7 +4,8 @@
 // silu, quick_gelu and gelu with tanh are z sigmoid(u), since (1 + tanh(u / 2)) / 2 = sigmoid(u); they take the fast
 // exponential and reciprocal, whose errors are 2^-21 of the value, far below the 2^-12 of an fp16 result.  gelu with erf takes
 // the normal distribution's tail below, to 1e-7.  Factors that stand beside a vanishing one are clamped, so that infinite
-// pre-activations give the limits (0 and z; derivatives 0 and 1) and not 0 * inf; the clamps pass NaN on.
+// pre-activations give the limits (0 and z; derivatives 0 and 1; to 2^-50, as sigmoids end at 2^-60) and not 0 * inf; the
+// clamps pass NaN on.
 #pragma once
 #include "bxl_types.cuh"
 
@@ -38,10 +39,15 @@ __device__ __forceinline__ float if_negative(float z, float a, float b) { return
     const float2 u = split(a);                                         \
     return f2(name(u.x), name(u.y));                                   \
   }
-BXL_ON_PAIRS(rcp_approx)
 BXL_ON_PAIRS(exp2_approx)
 BXL_ON_PAIRS(magnitude)
 #undef BXL_ON_PAIRS
+// Both reciprocals of a pair from that of the product, which must not overflow: one special-function instruction instead of two.
+__device__ __forceinline__ F2 rcp_approx(F2 a) {
+  const float2 u = split(a);
+  const float r = rcp_approx(u.x * u.y);
+  return mul(f2(u.y, u.x), f2(r, r));
+}
 __device__ __forceinline__ F2 min_nan(F2 a, float b) {
   const float2 u = split(a);
   return f2(min_nan(u.x, b), min_nan(u.y, b));
@@ -68,14 +74,16 @@ __device__ __forceinline__ F normal_tail(F a, F& e) {
   p = fma(t, p, splat<F>(0.5f * 0.254829592f));
   return mul(mul(p, t), e);
 }
-// exp(-u) of sigmoid(u) = 1 / (1 + exp(-u))
+// exp(-u) of sigmoid(u) = 1 / (1 + exp(-u)), at most 2^60, so that the product of two divisors does not overflow
 template <int ACT, class F>
 __device__ __forceinline__ F exp_minus_argument(F z) {
   constexpr float kLog2e = 1.4426950408889634f;
-  if constexpr (ACT == BXL_ACT_SILU) return exp2_approx(mul(z, splat<F>(-kLog2e)));
-  else if constexpr (ACT == BXL_ACT_QUICK_GELU) return exp2_approx(mul(z, splat<F>(-1.702f * kLog2e)));
+  F u;
+  if constexpr (ACT == BXL_ACT_SILU) u = mul(z, splat<F>(-kLog2e));
+  else if constexpr (ACT == BXL_ACT_QUICK_GELU) u = mul(z, splat<F>(-1.702f * kLog2e));
   else  // gelu with tanh: u = 2 sqrt(2 / pi) (z + 0.044715 z^3)
-    return exp2_approx(mul(z, fma(mul(z, z), splat<F>(-0.07135481627260025f * kLog2e), splat<F>(-1.5957691216057308f * kLog2e))));
+    u = mul(z, fma(mul(z, z), splat<F>(-0.07135481627260025f * kLog2e), splat<F>(-1.5957691216057308f * kLog2e)));
+  return exp2_approx(min_nan(u, 60.f));
 }
 
 template <int ACT, class F>
@@ -91,7 +99,7 @@ __device__ __forceinline__ F act_value(F z) {
     const F q = normal_tail(a, e);
     return fma(mul(a, splat<F>(-1.f)), q, max_nan(z, 0.f));
   } else {
-    return mul(max_nan(z, -1e30f), rcp_approx(add(exp_minus_argument<ACT>(z), splat<F>(1.f))));
+    return mul(max_nan(z, -1e3f), rcp_approx(add(exp_minus_argument<ACT>(z), splat<F>(1.f))));
   }
 }
 
@@ -111,10 +119,11 @@ __device__ __forceinline__ F act_slope(F z) {
     const F s = fma(mul(a, splat<F>(-0.3989422804014327f)), e, q);
     return if_negative(z, s, fma(s, splat<F>(-1.f), splat<F>(1.f)));
   } else {
-    // s + z s (1 - s) du/dz; beyond the clamps s (1 - s) is exactly 0
-    const F zc = min_nan(max_nan(z, -1e3f), 1e3f);
-    const F s = rcp_approx(add(exp_minus_argument<ACT>(z), splat<F>(1.f)));
-    const F rest = mul(mul(zc, s), fma(s, splat<F>(-1.f), splat<F>(1.f)));
+    // s + z s (1 - s) du/dz with 1 - s = s exp(-u), which is exact on both sides; beyond the clamps s (1 - s) vanishes
+    constexpr float kEnd = ACT == BXL_ACT_GELU_TANH ? 12.f : 64.f;
+    const F zc = min_nan(max_nan(z, -kEnd), kEnd), e = exp_minus_argument<ACT>(z);
+    const F s = rcp_approx(add(e, splat<F>(1.f)));
+    const F rest = mul(mul(zc, s), mul(s, e));
     if constexpr (ACT == BXL_ACT_SILU) return add(s, rest);
     else if constexpr (ACT == BXL_ACT_QUICK_GELU) return fma(rest, splat<F>(1.702f), s);
     else return fma(rest, fma(mul(zc, zc), splat<F>(0.2140644488178008f), splat<F>(1.5957691216057308f)), s);

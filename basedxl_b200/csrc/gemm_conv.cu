@@ -55,9 +55,11 @@ constexpr int kUmmaK = 16;         // K of one tcgen05.mma.kind::f16
 #define BXL_EPI_SUB 2
 #endif
 constexpr int kEpiSub = BXL_EPI_SUB;            // epilogue warps per 32-row quarter of the tile
-constexpr int kEpiThreads = kEpiSub * 128;
-constexpr int kWarpA = 4 * kEpiSub, kWarpMma = kWarpA + 1, kWarpB = kWarpA + 2;   // after the epilogue warps: A loads, MMA, B loads
-constexpr int kGemmThreads = (4 * kEpiSub + 3) * 32;
+// Linear layers with an activation take twice as many: their chunks are bound by the latencies of the accumulator read, the
+// activation's exponential and reciprocal and the store, one after the other in every warp.
+constexpr int kEpiSubLin = 4;
+constexpr int epi_sub(int lin) { return lin ? kEpiSubLin : kEpiSub; }
+constexpr int gemm_threads(int lin) { return (4 * epi_sub(lin) + 3) * 32; }
 constexpr int kABytes = kBM * kBK * 2;       // 16 KB
 constexpr int kSmemBudget = 227 * 1024;      // dynamic shared memory available to one CTA
 constexpr int kSmemMisc = 3072;              // alignment slack + barriers + the tile's bias row (256 floats)
@@ -300,17 +302,11 @@ __device__ __forceinline__ void store_chunk_ragged(const GemmParams& p, const fl
 // activation in fp32, residual.  `f` holds 32 consecutive columns of one row.
 // A warp's 32 x 32 values leave through shared memory by the copy engine: a lane's stores straight to its row of C touch 32 rows
 // at a time, and took 1.8 us of a 256-column tile's 6.9 (8192 x 1280 x 5120 with the pre-activation kept: 93 us of 77 without).
-// Two buffers of 2 KB per warp take turns; rows and columns past the matrix are clipped.
+// A buffer of 2 KB per warp; rows and columns past the matrix are clipped.
 constexpr int kOutBytes = 32 * 32 * 2;
-struct OutStage {
-  uint32_t base;    // this warp's two buffers
-  int turn;
-};
 template <class T>
-__device__ __forceinline__ void store_tile_chunk(const CUtensorMap* map, const F2 (&f)[16], int row0, int nb, OutStage& out, int lane) {
-  const uint32_t buf = out.base + out.turn * kOutBytes;
-  out.turn ^= 1;
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the copy before last has read this buffer
+__device__ __forceinline__ void store_tile_chunk(const CUtensorMap* map, const F2 (&f)[16], int row0, int nb, uint32_t buf, int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the copy before has read the buffer
   __syncwarp();
 #pragma unroll
   for (int q = 0; q < 4; ++q)   // rows of 64 bytes in the 64-byte swizzled layout: 16-byte piece index XOR (row / 2 mod 4)
@@ -364,7 +360,7 @@ __device__ __forceinline__ void add_bias(const uint32_t (&acc)[32], const BiasCh
   }
 }
 template <class T>
-__device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, OutStage& out, int lane) {
+__device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, uint32_t out, int lane) {
   if (p.pre) store_tile_chunk<T>(&p.pre_map, f, row0, nb, out, lane);
   with_act(p.act, [&](auto act) {
 #pragma unroll
@@ -423,10 +419,12 @@ __host__ __device__ inline int acc_sets(int parts, int bn) { return parts == 1 ?
 // kTwo: operands in two fp16 parts (p.parts == 2); likewise separate.
 // kLin: linear layers with an activation, of fp16 (1) or bf16 (2) operands; 0 everywhere else.
 template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin = 0>
-__global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid_constant__ GemmParams p) {
+__global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const __grid_constant__ GemmParams p) {
   static_assert(!(kPair && kSplit), "a CTA pair walks the whole K range");
   static_assert(!(kConv && kTwo), "convolutions have fp16 operands");
   static_assert(!kLin || !(kConv || kTwo), "an epilogue of plain products");
+  constexpr int kSub = epi_sub(kLin), kSubThreads = kSub * 128;                       // epilogue warps of a quarter of the tile
+  constexpr int kWarpA = 4 * kSub, kWarpMma = kWarpA + 1, kWarpB = kWarpA + 2;         // after the epilogue warps: A loads, MMA, B loads
   using LinT = std::conditional_t<kLin == 2, __nv_bfloat16, __half>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -471,9 +469,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), 4 * kEpiSub * kWidth);  // one arrival per epilogue warp (of both CTAs in pair mode)
+      mbar_init(tempty_bar(a), 4 * kSub * kWidth);  // one arrival per epilogue warp (of both CTAs in pair mode)
     }
-    const uint32_t peers_threads = (S > 1) ? (S - 1) * static_cast<uint32_t>(kEpiThreads) : 1u;  // every epilogue thread of every peer
+    const uint32_t peers_threads = (S > 1) ? (S - 1) * static_cast<uint32_t>(kSubThreads) : 1u;  // every epilogue thread of every peer
     mbar_init(recv_full_bar, peers_threads);
     mbar_init(recv_free_bar, peers_threads);
     *abort_flag = 0;
@@ -719,11 +717,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
   } else {
     // ======================= epilogue (warps 0..7) =======================
     const int quarter = warp & 3;  // TMEM lane quarter this warp may access
-    const int half = warp >> 2;    // which of the quarter's kEpiSub warps: it takes the chunks c with c % kEpiSub == half
+    const int half = warp >> 2;    // which of the quarter's kSub warps: it takes the chunks c with c % kSub == half
     const int row_in_tile = quarter * 32 + lane;
     const int chunks = BN / 32;
     const int cps = chunks / S;    // 32-column chunks per owner slice
-    [[maybe_unused]] OutStage out_stage{smem_u32(s_turn) + warp * 2 * kOutBytes, 0};
+    [[maybe_unused]] const uint32_t out_stage = smem_u32(s_turn) + warp * kOutBytes;
     int it = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++it) {
       const int acc = it & 1;
@@ -750,9 +748,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
       const bool has_ln = !kConv && (p.ln_part != nullptr);
       const bool has_bias = (p.bias != nullptr) || (p.bias_f32 != nullptr) || (kConv && p.bias_rows != nullptr);
       if ((has_bias && !kLin) || has_ln) {
-        asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
-        const int et = warp * 32 + lane;   // 0..kEpiThreads-1
-        for (int j = et; j < BN; j += kEpiThreads) {
+        asm volatile("bar.sync 1, %0;" ::"n"(kSubThreads) : "memory");
+        const int et = warp * 32 + lane;   // 0..kSubThreads-1
+        for (int j = et; j < BN; j += kSubThreads) {
           float b = 0.f, cs = 0.f;
           if (n0 + j < p.N) {
             if (p.bias_f32) b += p.bias_f32[n0 + j];
@@ -763,7 +761,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
           s_bias[j] = b;
           if (has_ln) s_colsum[j] = cs;
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(kSubThreads) : "memory");
       }
       // LayerNorm fold: this row's mean and reciprocal standard deviation from the partial sums
       // the producer of A left (read while this tile's MMAs still run)
@@ -806,34 +804,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
         }
       };
       if constexpr (kLin != 0 && !kSplit) {
-        // The next chunk's accumulator is on its way while this one goes through the activation.
-        uint32_t v[32];
-        if (half < chunks) tmem_ld_32x32(t_row + half * 32, v);
 #pragma unroll 1
-        for (int c = half; c < chunks; c += kEpiSub) {
-          const int nb = n0 + c * 32;
+        for (int c = half; c < chunks; c += kSub) {
+          const int nb = n0 + c * 32, row0 = tm * kBM + quarter * 32;
+          uint32_t v[32];
+          tmem_ld_32x32(t_row + c * 32, v);
+          if (c != half) {
+            load_bias<LinT>(p, nb, bias);
+            load_residual(p, out_row, nb, res_cur);
+          }
           tmem_ld_wait();
           F2 f[16];
           add_bias<LinT>(v, bias, f);
-          if (c + kEpiSub < chunks) {
-            tmem_ld_32x32(t_row + (c + kEpiSub) * 32, v);
-            load_bias<LinT>(p, nb + kEpiSub * 32, bias);
-            load_residual(p, out_row, nb + kEpiSub * 32, res_next);
-          }
-          const int row0 = tm * kBM + quarter * 32;
           if (p.ragged) store_chunk_act_ragged<LinT>(p, f, row0, nb, s_turn + warp * kTurnFloats, lane);
           else if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, f, out_row, row0, nb, res_cur, out_stage, lane);
-          res_cur = res_next;
-          res_next.valid = false;
         }
       } else if constexpr (!kSplit) {
         // One chunk at a time per warp (measured: several accumulator loads in flight per warp do not
         // shorten the epilogue; a second warp on the same scheduler does).
 #pragma unroll 1
-        for (int c = half; c < chunks; c += kEpiSub) {
+        for (int c = half; c < chunks; c += kSub) {
           uint32_t v[32];
           tmem_ld_32x32(t_row + c * 32, v);
-          if (c + kEpiSub < chunks) load_residual(p, out_row, n0 + (c + kEpiSub) * 32, res_next);
+          if (c + kSub < chunks) load_residual(p, out_row, n0 + (c + kSub) * 32, res_next);
           tmem_ld_wait();
           add_sets(c, v);
           const int nb = n0 + c * 32;
@@ -862,7 +855,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
           const int own_lo = static_cast<int>(crank) * cps;
           const int nf = chunks - cps;                                  // chunks owned by the peers
 #pragma unroll 1
-          for (int fi = half; fi < nf; fi += kEpiSub) {
+          for (int fi = half; fi < nf; fi += kSub) {
             const int c = fi < own_lo ? fi : fi + cps;                   // fi-th chunk that is not this CTA's own
             uint32_t v[32];
             tmem_ld_32x32(t_row + c * 32, v);
@@ -886,20 +879,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
         uint32_t v[32];
         if (has_own) {
           load_residual(p, out_row, n0 + (static_cast<int>(crank) * cps + half) * 32, res_cur);
-          tmem_ld_32x32(t_row + (static_cast<int>(crank) * cps + half) * 32, v);
+          if constexpr (kLin == 0) tmem_ld_32x32(t_row + (static_cast<int>(crank) * cps + half) * 32, v);
         }
         if (!mbar_wait_cluster(recv_full_bar, it & 1u, abort_flag, p.dev_status, 302)) break;
         __syncwarp();
 #pragma unroll 1
-        for (int cc = half; cc < cps; cc += kEpiSub) {
+        for (int cc = half; cc < cps; cc += kSub) {
           const int c = crank * cps + cc;
-          if (cc + kEpiSub < cps) load_residual(p, out_row, n0 + (c + kEpiSub) * 32, res_next);
+          if constexpr (kLin != 0) {
+            tmem_ld_32x32(t_row + c * 32, v);
+            if (cc != half) {
+              load_bias<LinT>(p, n0 + c * 32, bias);
+              load_residual(p, out_row, n0 + c * 32, res_cur);
+            }
+          } else if (cc + kSub < cps) {
+            load_residual(p, out_row, n0 + (c + kSub) * 32, res_next);
+          }
           tmem_ld_wait();
           add_sets(c, v);
           float f[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-          if (cc + kEpiSub < cps) tmem_ld_32x32(t_row + (c + kEpiSub) * 32, v);   // this warp's next own chunk, in flight during the reduction
+          if (kLin == 0 && cc + kSub < cps) tmem_ld_32x32(t_row + (c + kSub) * 32, v);   // this warp's next own chunk, in flight during the reduction
           for (int slot = 0; slot < S - 1; ++slot) {
             const uint8_t* src = smem_gen + (recv_base - smem_base) + ((slot * cps + cc) * 8 * kBM + row_in_tile) * 16;
 #pragma unroll
@@ -915,7 +916,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
 #pragma unroll
             for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(f[j]);
             add_bias<LinT>(u, bias, g);
-            load_bias<LinT>(p, nb + kEpiSub * 32, bias);
             const int row0 = tm * kBM + quarter * 32;
             if (p.ragged) store_chunk_act_ragged<LinT>(p, g, row0, nb, s_turn + warp * kTurnFloats, lane);
             else if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, g, out_row, row0, nb, res_cur, out_stage, lane);
@@ -924,15 +924,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_conv_kernel(const __grid
           else if (out_row >= 0 && nb < p.N)
             store_chunk<kConv>(p, f, out_row, nb, img, has_bias ? s_bias + c * 32 : nullptr, res_cur,
                                has_ln ? s_colsum + c * 32 : nullptr, ln, stat);
-          res_cur = res_next;
-          res_next.valid = false;
+          if constexpr (kLin == 0) {
+            res_cur = res_next;
+            res_next.valid = false;
+          }
         }
         // tell the peers their pushes have been consumed
         for (uint32_t o = 0; o < static_cast<uint32_t>(S); ++o)
           if (o != crank) mbar_arrive_remote(map_to_cta(recv_free_bar, o));
       }
       if (!kConv && p.stat_out && out_row >= 0)
-        p.stat_out[out_row * p.stat_parts + (tn * S + (S > 1 ? static_cast<int>(crank) : 0)) * kEpiSub + half] = make_float2(stat.s, stat.q);
+        p.stat_out[out_row * p.stat_parts + (tn * S + (S > 1 ? static_cast<int>(crank) : 0)) * kSub + half] = make_float2(stat.s, stat.q);
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -974,9 +976,9 @@ struct TileConfig {
 };
 
 constexpr int kSmemLnExtra = 1024;           // the weight column-sum row of a GEMM with a folded LayerNorm
-constexpr int kSmemRaggedExtra = 4 * kEpiSub * kTurnFloats * 4;   // the epilogue warps' transposing stages
+constexpr int ragged_bytes(int lin) { return 4 * epi_sub(lin) * kTurnFloats * 4; }   // the epilogue warps' transposing stages
 
-constexpr int kSmemOutExtra = 4 * kEpiSub * 2 * kOutBytes;        // ... or their output buffers (linear layers)
+constexpr int kSmemOutExtra = 4 * kEpiSubLin * kOutBytes;          // ... or their output buffers (linear layers)
 
 static int stages_for(int bn, int split, int pair = 0, int extra_smem = 0, int parts = 1) {
   const int stage = parts * (kABytes + (pair ? bn * 64 : bn * 128));
@@ -1006,7 +1008,7 @@ static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int fo
   const int sms = sm_count();
   TileConfig best{128, 1, stages_for(128, 1, 0, extra_smem, parts), 0, sms};
   int at_once[5] = {0, sms, 0, 0, 0};
-  for (int w = 2; w <= 4; w *= 2) at_once[w] = resident_clusters(gemm_conv_kernel<false, false, true, false>, kGemmThreads, kSmemBudget, w, g_clusters);
+  for (int w = 2; w <= 4; w *= 2) at_once[w] = resident_clusters(gemm_conv_kernel<false, false, true, false>, gemm_threads(0), kSmemBudget, w, g_clusters);
   double best_cost = 1e30;
   for (int pair = 0; pair <= 1; ++pair) {
     if (force_pair >= 0 && pair != force_pair) continue;
@@ -1047,7 +1049,7 @@ template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin>
 static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   const int b_rows = kPair ? p.bn / 2 : p.bn;
   const int smem = p.stages * p.parts * (kABytes + b_rows * 128) + recv_bytes(p.bn, kSplit ? p.split : 1) + kSmemMisc +
-                   (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? kSmemRaggedExtra : kLin ? kSmemOutExtra : 0);
+                   (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? ragged_bytes(kLin) : kLin ? kSmemOutExtra : 0);
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1064,7 +1066,7 @@ static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   int clusters = p.clusters;
   if (clusters > num_units) clusters = num_units;
   if (clusters < 1) clusters = 1;
-  return launch_kernel("gemm_conv_kernel launch", gemm_conv_kernel<kConv, kPair, kSplit, kTwo, kLin>, dim3(clusters * width), dim3(kGemmThreads), smem,
+  return launch_kernel("gemm_conv_kernel launch", gemm_conv_kernel<kConv, kPair, kSplit, kTwo, kLin>, dim3(clusters * width), dim3(gemm_threads(kLin)), smem,
                        stream, width, p);
 }
 
@@ -1229,7 +1231,7 @@ extern "C" int bxl_gemm_ragged_f16(const void* A, long long lda, const void* B, 
   const bool ragged = !aligned16(C) || ldc % 8 || N % 8 || (residual && (!aligned16(residual) || ldr % 8));
   const int tiles_m = (M + kBM - 1) / kBM;
   const TileConfig tc = choose_tiles(tiles_m, N, (K + kBK - 1) / kBK, true, g_force_bn, g_force_split,
-                                     g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, ragged ? kSmemRaggedExtra : 0, 1, ragged || residual);
+                                     g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, ragged ? ragged_bytes(0) : 0, 1, ragged || residual);
   {
     uint64_t dims[2] = {(uint64_t)K, (uint64_t)M};
     uint64_t str[1] = {(uint64_t)a.ld_dst * 2};
@@ -1273,7 +1275,7 @@ int linear_product(const LinearProduct& q, cudaStream_t stream) {
   const bool ragged = q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && !rows16(q.residual, q.ldr)) || (q.pre && !rows16(q.pre, q.ldp));
   const int tiles_m = (int)(((long long)q.M + kBM - 1) / kBM);
   const TileConfig tc = choose_tiles(tiles_m, q.N, (int)(((long long)q.K + kBK - 1) / kBK), q.b_kn != 0, g_force_bn, g_force_split, g_force_pair < 0 ? kDefaultPair : g_force_pair,
-                                     0.0, ragged ? kSmemRaggedExtra : kSmemOutExtra, 1, ragged || q.residual || q.pre);
+                                     0.0, ragged ? ragged_bytes(1) : kSmemOutExtra, 1, ragged || q.residual || q.pre);
   {
     // [M,K], or [K,M] in boxes of 64 by 64
     uint64_t dims[2] = {(uint64_t)(q.a_mn ? q.M : q.K), (uint64_t)(q.a_mn ? q.K : q.M)};

@@ -107,7 +107,7 @@ struct DzArgs {
   long long lddy, ldp, ldz;
   int M, N, act;
 };
-constexpr int kDzWarps = 8;
+constexpr int kDzWarps = 8, kDzRows = 4;
 template <class T, int VEC>
 __global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
   pdl_launch_dependents();
@@ -125,26 +125,33 @@ __global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
   if (c < p.N)
     with_act(p.act, [&](auto act) {
       constexpr int kAct = decltype(act)::value;
-#pragma unroll 4
-      for (long long r = (long long)blockIdx.y * per + warp; r < r1; r += kDzWarps) {
-        F d[N];
-        widen<T, VEC>(load_vec<T, VEC>(static_cast<const T*>(p.dy) + r * p.lddy + c), d);
-        if constexpr (kAct != BXL_ACT_NONE) {
-          F z[N];
-          widen<T, VEC>(load_vec<T, VEC>(static_cast<const T*>(p.pre) + r * p.ldp + c), z);
+      // four rows are loaded before the first result is stored: the compiler cannot move loads over stores
+      for (long long r0 = (long long)blockIdx.y * per + warp; r0 < r1; r0 += kDzRows * kDzWarps) {
+        Vec<T, VEC> g[kDzRows], z[kDzRows];
 #pragma unroll
-          for (int j = 0; j < N; ++j) {
-            if constexpr (VEC == 1) {
-              d[j] *= act_slope<kAct>(z[j]);
-            } else {
-              const float2 u = split(z[j]);
-              d[j] = mul(d[j], f2(act_slope<kAct>(u.x), act_slope<kAct>(u.y)));
-            }
+        for (int i = 0; i < kDzRows; ++i) {
+          const long long r = r0 + i * kDzWarps;
+          if (r < r1) {
+            g[i] = load_vec<T, VEC>(static_cast<const T*>(p.dy) + r * p.lddy + c);
+            if constexpr (kAct != BXL_ACT_NONE) z[i] = load_vec<T, VEC>(static_cast<const T*>(p.pre) + r * p.ldp + c);
           }
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] = add(acc[j], d[j]);
-        if (p.dz) store_vec<T, VEC>(static_cast<T*>(p.dz) + r * p.ldz + c, narrow<T, VEC>(d));
+        for (int i = 0; i < kDzRows; ++i) {
+          const long long r = r0 + i * kDzWarps;
+          if (r >= r1) break;
+          F d[N];
+          widen<T, VEC>(g[i], d);
+          if constexpr (kAct != BXL_ACT_NONE) {
+            F u[N];
+            widen<T, VEC>(z[i], u);
+#pragma unroll
+            for (int j = 0; j < N; ++j) d[j] = mul(d[j], act_slope<kAct>(u[j]));
+          }
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] = add(acc[j], d[j]);
+          if (p.dz) store_vec<T, VEC>(static_cast<T*>(p.dz) + r * p.ldz + c, narrow<T, VEC>(d));
+        }
       }
     });
   if (!p.part) return;

@@ -147,7 +147,7 @@ def test_empty_and_wanted():
 @pytest.mark.parametrize("m", [2, 64])
 @pytest.mark.parametrize("act", ACTS)
 def test_infinite_and_missing_values(act, m):
-    """Infinite pre-activations give the limits, NaN stays in its row and column."""
+    """Infinite pre-activations give the limits (to 2^-50: a sigmoid is not formed below 2^-60), NaN stays in its row and column."""
     cuda_or_skip()
     _, ops = _ops()
     s = _inputs(m, 64, 40, torch.bfloat16)
@@ -162,10 +162,10 @@ def test_infinite_and_missing_values(act, m):
     y, pre = ops.linear_act(x, w, None, activation=act, want_pre=True)
     assert (pre[0, :20] == float("inf")).all() and (pre[0, 20:] == float("-inf")).all() and pre[1].isnan().all() and y[1].isnan().all()
     assert (y[0, :20] == float("inf")).all()
-    assert (y[0, 20:] == (float("-inf") if act == "none" else 0)).all()
+    assert (y[0, 20:] == float("-inf")).all() if act == "none" else (y[0, 20:].abs() < 2.0**-50).all()
     dy = torch.ones_like(y)
     _, _, db = ops.linear_act_bwd(dy[:1], x[:1], w, pre[:1], act)
-    assert (db[:20] == 1).all() and (db[20:] == (1 if act == "none" else 0)).all()
+    assert (db[:20] == 1).all() and ((db[20:] - (1 if act == "none" else 0)).abs() < 2.0**-50).all()
     if m > 2:
         assert torch.equal(y[2:], ops.linear_act(s["x"], w, None, activation=act)[2:])
 
