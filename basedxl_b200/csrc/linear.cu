@@ -15,44 +15,114 @@
 namespace bxl {
 
 // ---- forward of a few rows -------------------------------------------------------------------
-// A warp forms NB neighbouring columns of all MB rows over its share of K: every 16 bytes of W are loaded once, by one
-// lane, and meet the same 16 bytes of K of every row of x (from L1).  The block's warps share K and add in shared memory.
+// Up to eight rows are bound by reading W once, and a tile of 128 rows by what every tile costs to set up.  Here a block forms 16
+// columns: its warps share K, read W as it lies and add in shared memory.
 struct FewRows {
   const void *x, *w, *bias, *residual;
   void *y, *pre;
   long long ldx, ldw, ldr, ldy, ldp;
   int M, N, K, act;
 };
-template <class T, int VEC, int MB, int NB>
-__global__ void __launch_bounds__(256) few_rows_kernel(const FewRows p) {
-  static_assert(MB * NB <= 32, "one lane per result");
+constexpr int kFewRows = 8, kFewColumns = 16;
+// One result: `v` = x[m] . W[n].
+template <class T>
+__device__ __forceinline__ void few_rows_result(const FewRows& p, float v, int m, int n) {
+  if (m >= p.M || n >= p.N) return;
+  if (p.bias) v += to_f32(static_cast<const T*>(p.bias)[n]);
+  if (p.pre) static_cast<T*>(p.pre)[m * p.ldp + n] = from_f32<T>(v);
+  with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value>(v); });
+  if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[m * p.ldr + n]);
+  static_cast<T*>(p.y)[m * p.ldy + n] = from_f32<T>(v);
+}
+// D[16 x 8] += A[16 x 16] B[16 x 8] of one warp
+template <class T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Rows of whole 16-byte vectors.  The warp-wide product with W as its 16-row operand and x as its 8 columns needs three
+// 16-byte loads a lane for 32 values of K, and no widening: lane 4 g + q has values 8 q .. 8 q + 7 of rows g and g + 8 of W and of
+// row g of x, and hands them over as the k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of two products; both operands permute K alike.
+// Bound by the loads in flight: eight rows of 2560 x 10240 (52 MB) 11.6 us, 4.5 TB/s; 1280 x 5120 5.8, 320 x 1280 2.2.  With fused
+// multiply-adds instead the widening of x bounds it: 31.6, 8.9 and 3.0 us (one row of 2560 x 10240 10.5).
+constexpr int kFewMaxWarps = 8;
+template <class T>
+__global__ void __launch_bounds__(kFewMaxWarps * 32) few_rows_kernel(const FewRows p) {
   pdl_launch_dependents();
-  __shared__ float part[8][32];
+  __shared__ float part[kFewMaxWarps][kFewRows * kFewColumns];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int n0 = blockIdx.x * NB;
-  const T* x = static_cast<const T*>(p.x);
-  const T* w[NB];
+  const int g = lane >> 2, q = lane & 3, n0 = blockIdx.x * kFewColumns;
+  const T* w0 = static_cast<const T*>(p.w) + min(n0 + g, p.N - 1) * p.ldw;
+  const T* w1 = static_cast<const T*>(p.w) + min(n0 + g + 8, p.N - 1) * p.ldw;
+  const T* x = static_cast<const T*>(p.x) + min(g, p.M - 1) * p.ldx;
+  float d[4] = {0.f, 0.f, 0.f, 0.f};
+  pdl_wait();
+  auto step = [&](const uint4& a, const uint4& b, const uint4& c) {
+    mma_16x8x16<T>(d, a.x, b.x, a.y, b.y, c.x, c.y);
+    mma_16x8x16<T>(d, a.z, b.z, a.w, b.w, c.z, c.w);
+  };
+  const int whole = p.K / 32, share = (whole + warps - 1) / warps, last = min(whole, (warp + 1) * share);
+  int i = warp * share;
+  for (; i + 4 <= last; i += 4) {   // twelve loads on their way at once
+    uint4 a[4], b[4], c[4];
 #pragma unroll
-  for (int j = 0; j < NB; ++j) w[j] = static_cast<const T*>(p.w) + (long long)min(n0 + j, p.N - 1) * p.ldw;
+    for (int j = 0; j < 4; ++j) {
+      const int k = (i + j) * 32 + q * 8;
+      a[j] = *reinterpret_cast<const uint4*>(w0 + k), b[j] = *reinterpret_cast<const uint4*>(w1 + k), c[j] = *reinterpret_cast<const uint4*>(x + k);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) step(a[j], b[j], c[j]);
+  }
+#pragma unroll 3
+  for (; i < last; ++i) {
+    const int k = i * 32 + q * 8;
+    step(*reinterpret_cast<const uint4*>(w0 + k), *reinterpret_cast<const uint4*>(w1 + k), *reinterpret_cast<const uint4*>(x + k));
+  }
+  if (warp == warps - 1 && p.K % 32) {   // the lanes past K add nothing
+    const int k = whole * 32 + q * 8;
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    const bool in = k < p.K;
+    step(in ? *reinterpret_cast<const uint4*>(w0 + k) : none, in ? *reinterpret_cast<const uint4*>(w1 + k) : none, in ? *reinterpret_cast<const uint4*>(x + k) : none);
+  }
+  part[warp][2 * q * 16 + g] = d[0], part[warp][(2 * q + 1) * 16 + g] = d[1];
+  part[warp][2 * q * 16 + g + 8] = d[2], part[warp][(2 * q + 1) * 16 + g + 8] = d[3];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kFewRows * kFewColumns; i += blockDim.x) {
+    float v = 0.f;
+    for (int k = 0; k < warps; ++k) v += part[k][i];
+    few_rows_result<T>(p, v, i / 16, n0 + i % 16);
+  }
+}
+// Any other rows: a lane per value of K, NB columns a warp.
+template <class T, int MB>
+__global__ void __launch_bounds__(256) few_rows_any_kernel(const FewRows p) {
+  pdl_launch_dependents();
+  constexpr int NB = 2, kWarps = 8;   // 16 columns a block
+  const int lane = threadIdx.x & 31, n0 = blockIdx.x * kFewColumns + (threadIdx.x >> 5) * NB;
+  static_assert(NB * kWarps == kFewColumns, "a block's columns");
+  const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w);
   float acc[MB][NB];
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = 0.f;
   pdl_wait();
-  const int vecs = p.K / VEC;
-#pragma unroll 2
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    Vec<T, VEC> wv[NB];
+#pragma unroll 4
+  for (int k = lane; k < p.K; k += 32) {
+    float wv[NB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) wv[j] = load_vec<T, VEC>(w[j] + (long long)v * VEC);
+    for (int j = 0; j < NB; ++j) wv[j] = to_f32(w[min(n0 + j, p.N - 1) * p.ldw + k]);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-      const Vec<T, VEC> xv = load_vec<T, VEC>(x + min(i, p.M - 1) * p.ldx + (long long)v * VEC);
+      const float xv = to_f32(x[min(i, p.M - 1) * p.ldx + k]);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = fmaf(to_f32(xv.v[e]), to_f32(wv[j].v[e]), acc[i][j]);
+      for (int j = 0; j < NB; ++j) acc[i][j] = fmaf(xv, wv[j], acc[i][j]);
     }
   }
   float mine = 0.f;
@@ -65,37 +135,18 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewRows p) {
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == i * NB + j) mine = s;
     }
-  if (warps > 1) {
-    part[warp][lane] = mine;
-    __syncthreads();
-    if (warp) return;
-    for (int k = 1; k < warps; ++k) mine += part[k][lane];
-  }
-  const int m = lane / NB, n = n0 + lane % NB;
-  if (lane >= MB * NB || m >= p.M || n >= p.N) return;
-  if (p.bias) mine += to_f32(static_cast<const T*>(p.bias)[n]);
-  if (p.pre) static_cast<T*>(p.pre)[m * p.ldp + n] = from_f32<T>(mine);
-  with_act(p.act, [&](auto act) { mine = act_value<decltype(act)::value>(mine); });
-  if (p.residual) mine += to_f32(static_cast<const T*>(p.residual)[m * p.ldr + n]);
-  static_cast<T*>(p.y)[m * p.ldy + n] = from_f32<T>(mine);
+  if (lane < MB * NB) few_rows_result<T>(p, mine, lane / NB, n0 + lane % NB);
 }
 
-constexpr int kFewRows = 8;
-template <class T, int VEC, int MB>
-static int few_rows_launch(const FewRows& p, cudaStream_t s) {
-  constexpr int NB = 4;
-  const int groups = (p.N + NB - 1) / NB, most = (p.K / VEC + 31) / 32;
-  int warps = (sm_count() * 8 + groups - 1) / groups;   // eight warps an SM, as long as each has a vector per lane
-  warps = warps > most ? most : warps;
-  warps = warps > 8 ? 8 : warps < 1 ? 1 : warps;
-  return launch_kernel("few_rows_kernel launch", few_rows_kernel<T, VEC, MB, NB>, dim3(groups), dim3(32 * warps), 0, s, 1, p);
-}
 template <class T>
 static int few_rows(const FewRows& p, bool vec, cudaStream_t s) {
-  if (p.M == 1) return vec ? few_rows_launch<T, 8, 1>(p, s) : few_rows_launch<T, 1, 1>(p, s);
-  if (p.M == 2) return vec ? few_rows_launch<T, 8, 2>(p, s) : few_rows_launch<T, 1, 2>(p, s);
-  if (p.M <= 4) return vec ? few_rows_launch<T, 8, 4>(p, s) : few_rows_launch<T, 1, 4>(p, s);
-  return vec ? few_rows_launch<T, 8, 8>(p, s) : few_rows_launch<T, 1, 8>(p, s);
+  const dim3 grid((p.N + kFewColumns - 1) / kFewColumns);
+  if (vec) {
+    const int steps = (p.K + 31) / 32, warps = steps < kFewMaxWarps ? steps : kFewMaxWarps;
+    return launch_kernel("few_rows_kernel launch", few_rows_kernel<T>, grid, dim3(32 * warps), 0, s, 1, p);
+  }
+  auto any = [&](auto kernel) { return launch_kernel("few_rows_any_kernel launch", kernel, grid, dim3(256), 0, s, 1, p); };
+  return p.M == 1 ? any(few_rows_any_kernel<T, 1>) : p.M == 2 ? any(few_rows_any_kernel<T, 2>) : p.M <= 4 ? any(few_rows_any_kernel<T, 4>) : any(few_rows_any_kernel<T, 8>);
 }
 
 // ---- backward: dz and its column sums ----------------------------------------------------------
@@ -104,12 +155,14 @@ struct DzArgs {
   const void *dy, *pre;
   void* dz;                 // null: not stored
   float* part;              // [gridDim.y][N], or null
+  void* dbias;              // [N] where there is one share, or null
   long long lddy, ldp, ldz;
   int M, N, act;
 };
-constexpr int kDzWarps = 8, kDzRows = 4;
-template <class T, int VEC>
-__global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
+// Few rows: one share, whose block writes the sums' result itself (32 columns and 16 warps a block, for more blocks).
+constexpr int kDzRows = 2, kDzFew = 256;
+template <class T, int VEC, int kDzWarps>
+__global__ void __launch_bounds__(kDzWarps * 32, 32 / kDzWarps) dz_kernel(const DzArgs p) {
   pdl_launch_dependents();
   using F = typename Lanes<VEC>::F;
   constexpr int N = Lanes<VEC>::N;
@@ -125,7 +178,8 @@ __global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
   if (c < p.N)
     with_act(p.act, [&](auto act) {
       constexpr int kAct = decltype(act)::value;
-      // four rows are loaded before the first result is stored: the compiler cannot move loads over stores
+      // the rows' loads come before the first store, over which the compiler could not move them (8192 x 5120: two rows and 32 warps
+      // an SM 44.7 us, four and 16 47.5, one and 48 57)
       for (long long r0 = (long long)blockIdx.y * per + warp; r0 < r1; r0 += kDzRows * kDzWarps) {
         Vec<T, VEC> g[kDzRows], z[kDzRows];
 #pragma unroll
@@ -154,7 +208,7 @@ __global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
         }
       }
     });
-  if (!p.part) return;
+  if (!p.part && !p.dbias) return;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     if constexpr (VEC == 1) {
@@ -170,7 +224,9 @@ __global__ void __launch_bounds__(kDzWarps * 32) dz_kernel(const DzArgs p) {
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < kDzWarps; ++w) s += sums[w][i];
-    if (col < p.N) p.part[blockIdx.y * (long long)p.N + col] = s;
+    if (col >= p.N) continue;
+    if (p.dbias) static_cast<T*>(p.dbias)[col] = from_f32<T>(s);
+    else p.part[blockIdx.y * (long long)p.N + col] = s;
   }
 }
 
@@ -184,6 +240,7 @@ static long long round256(long long n) { return (n + 255) / 256 * 256; }
 
 // Shares of the rows in dz_kernel: about eight blocks an SM, and at least 32 rows each.
 static int dz_shares(int M, int N, int vec) {
+  if (M <= kDzFew) return 1;
   const long long cols = (N + 32ll * vec - 1) / (32 * vec);
   long long shares = (sm_count() * 8ll + cols - 1) / cols;
   const long long most = ((long long)M + 31) / 32;
@@ -231,7 +288,7 @@ static bool stores_dz(const bxl_linear_args* a) {
 static long long bwd_workspace(const bxl_linear_args* a) {
   long long n = 0;
   if (stores_dz(a)) n += round256(2ll * a->M * round8(a->N));
-  if (a->dbias) n += round256(4ll * dz_shares(a->M, a->N, 1) * a->N);
+  if (a->dbias && a->M > kDzFew) n += round256(4ll * dz_shares(a->M, a->N, 1) * a->N);
   if (a->dx) n += round256(copy_bytes(a->weight, a->ldw, a->N, a->K));
   if (a->dweight) n += round256(copy_bytes(a->x, a->ldx, a->M, a->K));
   return n;
@@ -290,16 +347,19 @@ extern "C" int bxl_linear_act_bwd(const bxl_linear_args* a, int* launches, void*
       ldz = p.ldz = round8(a->N);
       dz = p.dz = ws.take(2ll * a->M * ldz);
     }
-    const bool vec = a->N % 8 == 0 && al(a->dy, 16) && a->lddy % 8 == 0 && (a->act == BXL_ACT_NONE || (al(a->pre, 16) && a->ldp % 8 == 0));
+    const bool few = a->M <= kDzFew;
+    const bool vec = !few && a->N % 8 == 0 && al(a->dy, 16) && a->lddy % 8 == 0 && (a->act == BXL_ACT_NONE || (al(a->pre, 16) && a->ldp % 8 == 0));
     const int shares = dz_shares(a->M, a->N, vec ? 8 : 1), cols = vec ? 256 : 32;
-    if (a->dbias) p.part = static_cast<float*>(ws.take(4ll * dz_shares(a->M, a->N, 1) * a->N));
-    const dim3 grid((a->N + cols - 1) / cols, shares), block(kDzWarps * 32);
+    if (a->dbias && few) p.dbias = a->dbias;
+    else if (a->dbias) p.part = static_cast<float*>(ws.take(4ll * dz_shares(a->M, a->N, 1) * a->N));
+    const dim3 grid((a->N + cols - 1) / cols, shares);
+    auto launch = [&](auto kernel, int warps) { return launch_kernel("dz_kernel launch", kernel, grid, dim3(32 * warps), 0, s, 1, p); };
     int rc;
-    if (bf16) rc = vec ? launch_kernel("dz_kernel launch", dz_kernel<__nv_bfloat16, 8>, grid, block, 0, s, 1, p) : launch_kernel("dz_kernel launch", dz_kernel<__nv_bfloat16, 1>, grid, block, 0, s, 1, p);
-    else rc = vec ? launch_kernel("dz_kernel launch", dz_kernel<__half, 8>, grid, block, 0, s, 1, p) : launch_kernel("dz_kernel launch", dz_kernel<__half, 1>, grid, block, 0, s, 1, p);
+    if (bf16) rc = few ? launch(dz_kernel<__nv_bfloat16, 1, 16>, 16) : vec ? launch(dz_kernel<__nv_bfloat16, 8, 8>, 8) : launch(dz_kernel<__nv_bfloat16, 1, 8>, 8);
+    else rc = few ? launch(dz_kernel<__half, 1, 16>, 16) : vec ? launch(dz_kernel<__half, 8, 8>, 8) : launch(dz_kernel<__half, 1, 8>, 8);
     if (rc) return rc;
     ++count;
-    if (a->dbias) {
+    if (p.part) {
       if (int r = sum_partials(p.part, shares, a->N, a->N, a->dbias, nullptr, a->dtype, s)) return r;
       ++count;
     }

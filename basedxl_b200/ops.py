@@ -308,7 +308,7 @@ def linear_act(x, weight, bias=None, activation=None, residual=None, out=None, w
         _like("linear_act", residual, "residual", shape, dt, dev)
         r2 = _rows(residual)
     if out is None:
-        out = x.new_empty(shape)
+        out = torch.empty(shape, dtype=dt, device=dev)
     else:
         _like("linear_act", out, "out", shape, dt, dev)
         _req(out.is_contiguous(), "linear_act: out must be contiguous")
@@ -340,8 +340,8 @@ def linear_act_bwd(dy, x, weight, pre=None, activation=None, want_dx: bool = Tru
         _like("linear_act_bwd", pre, "pre", shape, dt, dev)
         pre2 = _rows(pre)
     _req(act == 0 or pre is not None, "linear_act_bwd: an activation needs the value before it (pre)")
-    dx = x.new_empty(x.shape) if want_dx else None
-    dweight = x.new_empty((n, k)) if want_dweight else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
+    dweight = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_dweight else None
     dbias = x.new_empty(n) if want_dbias else None
     if not m:
         for t in (dweight, dbias):

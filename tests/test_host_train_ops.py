@@ -175,7 +175,9 @@ def test_strides_reach_the_kernel(recorder):
 
 
 # ---- the C entry points: refused before any CUDA call --------------------------------------------
-P = 0x1000  # stands for an address; nothing reads it
+# (made-up addresses: not where a device could read them)
+P = 0x1000
+no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="a device is present")
 
 
 def _norm_fwd(**kw):
@@ -183,12 +185,14 @@ def _norm_fwd(**kw):
     return _lib.load().bxl_layernorm_fwd(*a.values(), None)
 
 
+@no_device
 @pytest.mark.parametrize("kw", [{"x": None}, {"y": None}, {"rows": 0}, {"rows": -1}, {"C": 0}, {"C": (1 << 30) + 1}, {"ldy": 63}, {"ldx": -1}, {"mean": None}, {"rstd": None},
                                 {"dtype": 3}, {"dtype": 2}, {"pt": 1}, {"eps": -1.0}, {"eps": float("nan")}, {"x": P + 1}, {"w": P + 1}, {"mean": P + 2}])
 def test_c_layernorm_fwd_refuses(kw):
     assert _norm_fwd(**kw) < 0 and b"bxl_layernorm_fwd" in _lib.load().bxl_last_error()
 
 
+@no_device
 @pytest.mark.parametrize("kw", [{"dy": None}, {"x": None}, {"mean": None}, {"rstd": None}, {"dx": None}, {"rows": 0}, {"C": -8}, {"lddx": 8}, {"lddy": -64}, {"pt": 1},
                                 {"dtype": -1}, {"dw": P + 1}, {"dx": P + 1}, {"ws": None, "rows": 4000}, {"ws": P + 8, "rows": 4000}, {"ws_bytes": 16, "rows": 4000}])
 def test_c_layernorm_bwd_refuses(kw):
@@ -209,13 +213,15 @@ def _linear(**kw):
 BOTH = [{"x": None}, {"weight": None}, {"M": 0}, {"N": -1}, {"K": 0}, {"M": (1 << 30) + 1}, {"dtype": 2}, {"dtype": 7}, {"act": 6}, {"act": -1}, {"x": P + 1}, {"bias": P + 1}, {"ldx": -1}]
 
 
+@no_device
 @pytest.mark.parametrize("kw", BOTH + [{"y": None}, {"ldy": 63}, {"pre": P, "ldp": 8}, {"ldx": 65, "workspace": None}, {"ldx": 65, "workspace_bytes": 64}])
 def test_c_linear_act_fwd_refuses(kw):
     l = _lib.load()
     assert l.bxl_linear_act_fwd(_linear(**kw), None) < 0 and b"bxl_linear_act_fwd" in l.bxl_last_error()
 
 
-@pytest.mark.parametrize("kw", BOTH + [{"dy": None}, {"act": 3}, {"lddx": 63}, {"lddw": 0}, {"lddy": -1}, {"workspace": None}, {"workspace": P + 4}, {"workspace_bytes": 8}])
+@no_device
+@pytest.mark.parametrize("kw", BOTH + [{"dy": None}, {"act": 3}, {"lddx": 63}, {"lddw": 0}, {"lddy": -1}, {"workspace": None, "M": 1000}, {"workspace": P + 4, "M": 1000}, {"workspace_bytes": 8, "M": 1000}])
 def test_c_linear_act_bwd_refuses(kw):
     l = _lib.load()
     assert l.bxl_linear_act_bwd(_linear(**kw), None, None) < 0 and b"bxl_linear_act_bwd" in l.bxl_last_error()
