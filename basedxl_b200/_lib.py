@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libbasedxl_b200.so")
@@ -130,6 +131,23 @@ def lib() -> C.CDLL:
         check(l.bxl_init(), l, kernels=0)
         _inited_devices.add(dev)
     return l
+
+
+_native = None
+
+
+def native():
+    """The native wrappers of the training operators (csrc/bindings.cpp), which call the same library."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise BxlError(f"basedxl_b200/_native.so cannot be loaded ({e}): build it with `python -m basedxl_b200.build` (there is no fallback path)") from e
+        module.connect(sys.modules[__name__])
+        _native = module
+    return _native
 
 
 # kernels of this library enqueued so far by this process (each successful

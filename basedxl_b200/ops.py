@@ -34,28 +34,6 @@ def _f16_cuda(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: expected a CUDA fp16 tensor, got {t.device} {t.dtype}")
 
 
-_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # BXL_F16, BXL_BF16, BXL_F32
-_HALF_TYPES = (torch.float16, torch.bfloat16)
-
-
-def _device() -> int:
-    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1   # no tensor of a device exists before
-
-
-def _here(name: str, x: torch.Tensor) -> torch.device:
-    """The device of ``x``, which has to be the current one: the kernels run on its current stream."""
-    dev = x.device
-    if dev.index != _device():
-        raise ValueError(f"{name}: expected tensors of the current CUDA device, got {dev}")
-    return dev
-
-
-def _rows(t):
-    """``t`` as a matrix of rows with unit-stride columns (a view where its strides allow one)."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
-
-
 # --------------------------------------------------------------------------- matmul
 def gemm(a, b, bias=None, residual=None, out=None, b_is_kn=False, out_f32=False):
     """``a[M,K] @ B`` with ``b`` given as [N,K] (default) or [K,N] (``b_is_kn``)."""
@@ -277,91 +255,25 @@ def gemm_split_f32(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "quick_gelu": 5}
 
 
-def _linear_operands(name, x, weight, activation):
-    """Checks what the two passes share; returns device, type, ``x`` and ``weight`` as rows, and the shape of the result."""
-    dev, dt, shape, ws = _here(name, x), x.dtype, x.shape, weight.shape
-    if dt not in _HALF_TYPES or len(shape) < 1 or len(ws) != 2 or weight.dtype != dt or ws[1] != shape[-1] or ws[0] < 1 or ws[1] < 1:
-        raise ValueError(f"{name}: expected fp16 or bf16 x [..., K] and weight [N, K], got {x.dtype} {list(shape)} and {weight.dtype} {list(ws)}")
-    if weight.device != dev:
-        raise ValueError(f"{name}: weight is on {weight.device}, x on {dev}")
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"{name}: unknown activation {activation!r}")
-    return dev, dt, _rows(x), _rows(weight), (*shape[:-1], ws[0])
-
-
-def _like(name, t, what, shape, dt, dev):
-    if t.shape != shape or t.dtype != dt or t.device != dev:
-        raise ValueError(f"{name}: {what} must be {list(shape)} in the type and on the device of x, got {t.dtype} {list(t.shape)} on {t.device}")
+def _activation(name, activation) -> int:
+    try:
+        return ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"{name}: unknown activation {activation!r}") from None
 
 
 def linear_act(x, weight, bias=None, activation=None, residual=None, out=None, want_pre: bool = False):
     """``act(x[..., K] @ weight[N, K]^T + bias) + residual`` in one product, fp16 or bf16, any extents; ``activation`` is one of
     ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``) receives the result.  ``want_pre`` also returns the value
     before the activation, rounded to the type of ``x``: the input of :func:`linear_act_bwd`."""
-    dev, dt, x2, w2, shape = _linear_operands("linear_act", x, weight, activation)
-    (m, k), n = x2.shape, shape[-1]
-    r2 = pre = None
-    if bias is not None:
-        _like("linear_act", bias, "bias", (n,), dt, dev)
-        _req(bias.is_contiguous(), "linear_act: bias must be contiguous")
-    if residual is not None:
-        _like("linear_act", residual, "residual", shape, dt, dev)
-        r2 = _rows(residual)
-    if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
-    else:
-        _like("linear_act", out, "out", shape, dt, dev)
-        _req(out.is_contiguous(), "linear_act: out must be contiguous")
-    if want_pre:
-        pre = torch.empty_like(out)
-    if m:
-        l = _lib.lib()
-        args = _lib.LinearArgs(
-            x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _p(bias), _p(r2), 0 if r2 is None else r2.stride(0), out.data_ptr(), n, _p(pre), n,
-            None, 0, None, 0, None, 0, None, None, 0, m, n, k, _TYPES[dt], ACTIVATIONS[activation])
-        ref = C.byref(args)
-        nbytes = l.bxl_linear_act_fwd_workspace_bytes(ref)
-        if nbytes:
-            ws = x.new_empty(nbytes, dtype=torch.uint8)
-            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        _lib.check(l.bxl_linear_act_fwd(ref, _stream()), l, kernels=2 if nbytes else 1)
-    return (out, pre) if want_pre else out
+    return _lib.native().linear_act(x, weight, bias, _activation("linear_act", activation), residual, out, bool(want_pre))
 
 
 def linear_act_bwd(dy, x, weight, pre=None, activation=None, want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
     """Gradients ``(dx, dweight, dbias)`` of :func:`linear_act`, given that of its result and, where it has an activation, the
     ``pre`` it returned; ``None`` for those that are not wanted.  The gradient of its residual is ``dy`` itself.  All have
     the type of ``x``; sums are fp32, ``dy * act'(pre)`` is rounded to that type between the products."""
-    dev, dt, x2, w2, shape = _linear_operands("linear_act_bwd", x, weight, activation)
-    act, (m, k), n = ACTIVATIONS[activation], x2.shape, shape[-1]
-    _like("linear_act_bwd", dy, "dy", shape, dt, dev)
-    pre2 = None
-    if pre is not None:
-        _like("linear_act_bwd", pre, "pre", shape, dt, dev)
-        pre2 = _rows(pre)
-    _req(act == 0 or pre is not None, "linear_act_bwd: an activation needs the value before it (pre)")
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_dx else None
-    dweight = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_dweight else None
-    dbias = x.new_empty(n) if want_dbias else None
-    if not m:
-        for t in (dweight, dbias):
-            if t is not None:
-                t.zero_()
-    elif want_dx or want_dweight or want_dbias:
-        dy2 = _rows(dy)
-        l = _lib.lib()
-        args = _lib.LinearArgs(
-            x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), None, None, 0, None, 0, _p(pre2), 0 if pre2 is None else pre2.stride(0),
-            dy2.data_ptr(), dy2.stride(0), _p(dx), k, _p(dweight), k, _p(dbias), None, 0, m, n, k, _TYPES[dt], act)
-        ref = C.byref(args)
-        nbytes = l.bxl_linear_act_bwd_workspace_bytes(ref)
-        if nbytes:
-            ws = x.new_empty(nbytes, dtype=torch.uint8)
-            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-        count = C.c_int(0)
-        _lib.check(l.bxl_linear_act_bwd(ref, C.byref(count), _stream()), l, kernels=0)
-        _lib.launches += count.value
-    return dx, dweight, dbias
+    return _lib.native().linear_act_bwd(dy, x, weight, pre, _activation("linear_act_bwd", activation), bool(want_dx), bool(want_dweight), bool(want_dbias))
 
 
 # --------------------------------------------------------------------------- convolution
@@ -573,88 +485,18 @@ def layernorm(x, gamma, beta, eps):
     return out
 
 
-def _norm_operands(name, x):
-    dev, shape = _here(name, x), x.shape
-    if x.dtype not in _TYPES or len(shape) < 1 or shape[-1] < 1:
-        raise ValueError(f"{name}: expected fp16, bf16 or fp32 rows of at least one element, got {x.dtype} {list(shape)}")
-    return dev, x.dtype, shape, shape[-1]
-
-
-def _norm_param(name, t, c, dt, dev):
-    """The type of a weight or bias vector, which is that of x or fp32."""
-    pt = t.dtype
-    if t.shape != (c,) or not t.is_contiguous() or (pt != dt and pt != torch.float32) or t.device != dev:
-        raise ValueError(f"{name}: weight and bias must be contiguous [{c}] vectors in the type of x or in fp32, on its device")
-    return pt
-
-
 def layernorm_fwd(x, weight=None, bias=None, eps: float = 1e-5, out=None, want_stats: bool = False):
     """LayerNorm over the last axis of ``x`` (fp16, bf16 or fp32, any width); ``weight`` and ``bias`` in its type or in
     fp32, either may be absent.  ``out`` (which may be ``x``) receives the result.  ``want_stats`` also returns the
     rows' fp32 ``mean`` and ``rstd``, the input of :func:`layernorm_bwd`."""
-    dev, dt, shape, c = _norm_operands("layernorm_fwd", x)
-    pt = dt
-    if weight is not None:
-        pt = _norm_param("layernorm_fwd", weight, c, dt, dev)
-    if bias is not None:
-        bt = _norm_param("layernorm_fwd", bias, c, dt, dev)
-        _req(weight is None or bt == pt, "layernorm_fwd: weight and bias must share a type")
-        pt = bt
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    else:
-        _like("layernorm_fwd", out, "out", shape, dt, dev)
-        _req(out.is_contiguous(), "layernorm_fwd: out must be contiguous")
-    rows = x.numel() // c
-    mean = rstd = None
-    if want_stats:
-        mean = x.new_empty(shape[:-1], dtype=torch.float32)
-        rstd = torch.empty_like(mean)
-    if rows:
-        x2 = _rows(x)
-        l = _lib.lib()
-        _lib.check(
-            l.bxl_layernorm_fwd(x2.data_ptr(), x2.stride(0), _p(weight), _p(bias), out.data_ptr(), c, _p(mean), _p(rstd), rows, c, _TYPES[dt], _TYPES[pt],
-                                eps, _stream()),
-            l,
-        )
-    return (out, mean, rstd) if want_stats else out
+    return _lib.native().layernorm_fwd(x, weight, bias, eps, out, bool(want_stats))
 
 
 def layernorm_bwd(dy, x, mean, rstd, weight=None, want_dweight: bool = True, want_dbias: bool = True):
     """Gradients ``(dx, dweight, dbias)`` of :func:`layernorm_fwd`, given that of its result and the ``mean`` and ``rstd``
     it returned.  ``dweight`` and ``dbias`` have the type of ``weight`` (that of ``x`` without one) and are ``None`` where
     they are not wanted; ``dweight`` is ``None`` without a ``weight``."""
-    dev, dt, shape, c = _norm_operands("layernorm_bwd", x)
-    _like("layernorm_bwd", dy, "dy", shape, dt, dev)
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.shape != shape[:-1] or t.device != dev or not t.is_contiguous():
-            raise ValueError("layernorm_bwd: mean and rstd must be contiguous fp32, one value per row of x, on its device")
-    pt = dt
-    if weight is not None:
-        pt = _norm_param("layernorm_bwd", weight, c, dt, dev)
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dweight = torch.empty_like(weight) if want_dweight and weight is not None else None
-    dbias = (x.new_empty(c) if weight is None else torch.empty_like(weight)) if want_dbias else None
-    rows = x.numel() // c
-    if rows:
-        dy2, x2 = _rows(dy), _rows(x)
-        l = _lib.lib()
-        ws, nbytes = None, 0
-        if dweight is not None or dbias is not None:
-            nbytes = l.bxl_layernorm_bwd_workspace_bytes(rows, c)
-            if nbytes:
-                ws = x.new_empty(nbytes, dtype=torch.uint8)
-        _lib.check(
-            l.bxl_layernorm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), mean.data_ptr(), rstd.data_ptr(), _p(weight), dx.data_ptr(), c,
-                                _p(dweight), _p(dbias), rows, c, _TYPES[dt], _TYPES[pt], _p(ws), nbytes, _stream()),
-            l, kernels=2 if nbytes else 1,
-        )
-    else:
-        for t in (dweight, dbias):
-            if t is not None:
-                t.zero_()
-    return dx, dweight, dbias
+    return _lib.native().layernorm_bwd(dy, x, mean, rstd, weight, bool(want_dweight), bool(want_dbias))
 
 
 def geglu(h):

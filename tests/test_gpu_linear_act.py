@@ -261,3 +261,43 @@ def test_feed_forward_block_trains():
                                    (dgamma, want[1], 9, "dgamma"), (dbeta, want[2], 9, "dbeta"), (dx, want[0], 9, "dx")]:
         off = float((got.double() - ref).norm() / ref.norm())
         assert off <= stages * 2.0**-8, f"{what}: {off:.2e}"
+
+
+def test_counted_launches():
+    """One kernel, one more for operands that the copy engine cannot read, none without rows."""
+    cuda_or_skip()
+    _lib, ops = _ops()
+
+    def count(call):
+        before = _lib.launches
+        call()
+        return _lib.launches - before
+
+    s = _inputs(300, 64, 96, torch.float16)
+    w, x, pre = s["weight"], s["x"], s["dy"]
+    odd = torch.zeros(300, 65, device="cuda", dtype=torch.float16)[:, 1:]
+    assert count(lambda: ops.linear_act(x, w)) == 1 and count(lambda: ops.linear_act(odd, w)) == 2 and count(lambda: ops.linear_act(x[:2], w)) == 1
+    assert count(lambda: ops.linear_act(x[:0], w)) == 0 and count(lambda: ops.linear_act_bwd(s["dy"][:0], x[:0], w)) == 0
+    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, pre, "gelu")) == 4     # dz, its sums, dx, dweight
+    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, want_dbias=False)) == 2
+    assert count(lambda: ops.linear_act_bwd(s["dy"][:9], x[:9], w, pre[:9], "gelu")) == 3
+    n = torch.ones(64, device="cuda", dtype=torch.float16)
+    rows = torch.zeros(2000, 64, device="cuda", dtype=torch.float16)
+    _, mean, rstd = ops.layernorm_fwd(rows, n, want_stats=True)
+    assert count(lambda: ops.layernorm_fwd(rows, n)) == 1 and count(lambda: ops.layernorm_fwd(rows[:0], n)) == 0
+    assert count(lambda: ops.layernorm_bwd(rows, rows, mean, rstd, n)) == 2 and count(lambda: ops.layernorm_bwd(rows[:5], rows[:5], mean[:5], rstd[:5], n)) == 1
+
+
+def test_mixed_devices_are_refused():
+    cuda_or_skip()
+    _, ops = _ops()
+    x, w = torch.zeros(4, 8, device="cuda", dtype=torch.float16), torch.zeros(6, 8, device="cuda", dtype=torch.float16)
+    mean = torch.zeros(4, device="cuda")
+    for call in (lambda: ops.linear_act(x, w.cpu()), lambda: ops.linear_act(x, w, w[:, 0].contiguous().cpu()), lambda: ops.linear_act(x.cpu(), w), lambda: ops.layernorm_fwd(x, x[0].cpu()),
+                 lambda: ops.layernorm_bwd(x.cpu(), x, mean, mean), lambda: ops.layernorm_bwd(x, x, mean.cpu(), mean), lambda: ops.linear_act_bwd(x[:, :6], x, w, out_of(x), "gelu")):
+        with pytest.raises(ValueError, match="cuda|current CUDA device"):
+            call()
+
+
+def out_of(x):
+    return torch.zeros(x.shape[0], 6, dtype=x.dtype)

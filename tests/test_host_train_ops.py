@@ -1,5 +1,6 @@
-"""Refusals and launch arguments of the training operators, with the library replaced by a recorder (no GPU), and what the
-C entry points refuse before any CUDA call."""
+"""What the training operators and their C entry points refuse before any CUDA call (no GPU).
+
+The wrappers look at the device last: a call on host tensors that is right in every other way is refused for that alone."""
 import ctypes as C
 
 import pytest
@@ -7,42 +8,17 @@ import torch
 
 from basedxl_b200 import _lib, ops
 
-
-class _Recorder:
-    """Stands for the loaded library: remembers the launches."""
-
-    def __init__(self):
-        self.calls = []
-
-    def __getattr__(self, name):
-        if name.endswith("_bytes"):
-            return lambda *a: 1024
-
-        def call(*args):
-            if name.startswith("bxl_linear"):
-                a = args[0]._obj
-                args = {f: getattr(a, f) for f, _ in a._fields_}
-            self.calls.append((name, args))
-            return 0
-
-        return call
+HOST = "expected tensors of the current CUDA device, got cpu"
 
 
-@pytest.fixture
-def recorder(monkeypatch):
-    rec = _Recorder()
-    monkeypatch.setattr(_lib, "lib", lambda: rec)
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
-
-    monkeypatch.setattr(ops, "_device", lambda: None)   # the index of the CPU's device
-    return rec
+def _refused(call, **kw):
+    with pytest.raises(ValueError) as e:
+        call(**kw)
+    return str(e.value)
 
 
-def _z(*shape, dtype=torch.float16, device="cpu"):
-    return torch.zeros(*shape, dtype=dtype, device=device)
-
-
-META = {"device": "meta"}
+def _z(*shape, dtype=torch.float16):
+    return torch.zeros(*shape, dtype=dtype)
 
 
 @pytest.mark.parametrize(
@@ -52,25 +28,21 @@ META = {"device": "meta"}
         {"x": _z(5, 8, dtype=torch.int32)},
         {"x": _z(5, 0)},
         {"x": torch.zeros((), dtype=torch.float16)},
-        {"x": _z(5, 8, **META)},
         {"weight": _z(7)},
         {"weight": _z(1, 8)},
         {"weight": _z(16)[::2]},
         {"weight": _z(8, dtype=torch.bfloat16)},
-        {"weight": _z(8, **META)},
         {"bias": _z(9)},
         {"bias": _z(8, dtype=torch.float32)},        # not the weight's type
         {"out": _z(5, 9)},
         {"out": _z(8, 5).t()},
         {"out": _z(5, 8, dtype=torch.float32)},
-        {"out": _z(5, 8, **META)},
     ],
 )
-def test_layernorm_fwd_refuses(recorder, kw):
-    args = {"x": _z(5, 8), "weight": _z(8), "bias": _z(8), **kw}
-    with pytest.raises(ValueError):
-        ops.layernorm_fwd(args.pop("x"), args.pop("weight"), args.pop("bias"), **args)
-    assert not recorder.calls
+def test_layernorm_fwd_refuses(kw):
+    good = {"x": _z(5, 8), "weight": _z(8), "bias": _z(8)}
+    assert HOST in _refused(ops.layernorm_fwd, **good)
+    assert HOST not in _refused(ops.layernorm_fwd, **{**good, **kw})
 
 
 @pytest.mark.parametrize(
@@ -79,21 +51,18 @@ def test_layernorm_fwd_refuses(recorder, kw):
         {"dy": _z(5, 9)},
         {"dy": _z(8)},
         {"dy": _z(5, 8, dtype=torch.float32)},
-        {"dy": _z(5, 8, **META)},
         {"mean": _z(4, dtype=torch.float32)},
         {"mean": _z(5)},
         {"rstd": _z(10, dtype=torch.float32)[::2]},
         {"rstd": _z(5, 1, dtype=torch.float32)},
-        {"mean": _z(5, dtype=torch.float32, **META)},
         {"weight": _z(5)},
         {"weight": _z(8, dtype=torch.bfloat16)},
     ],
 )
-def test_layernorm_bwd_refuses(recorder, kw):
-    args = {"dy": _z(5, 8), "x": _z(5, 8), "mean": _z(5, dtype=torch.float32), "rstd": _z(5, dtype=torch.float32), "weight": _z(8), **kw}
-    with pytest.raises(ValueError):
-        ops.layernorm_bwd(**args)
-    assert not recorder.calls
+def test_layernorm_bwd_refuses(kw):
+    good = {"dy": _z(5, 8), "x": _z(5, 8), "mean": _z(5, dtype=torch.float32), "rstd": _z(5, dtype=torch.float32), "weight": _z(8)}
+    assert HOST in _refused(ops.layernorm_bwd, **good)
+    assert HOST not in _refused(ops.layernorm_bwd, **{**good, **kw})
 
 
 @pytest.mark.parametrize(
@@ -102,31 +71,26 @@ def test_layernorm_bwd_refuses(recorder, kw):
         {"x": _z(5, 8, dtype=torch.float32), "weight": _z(6, 8, dtype=torch.float32)},
         {"x": _z(5, 8, dtype=torch.bfloat16)},
         {"x": _z(5, 9)},
-        {"x": _z(5, 8, **META)},
         {"weight": _z(8)},
         {"weight": _z(0, 8)},
         {"weight": _z(1, 6, 8)},
-        {"weight": _z(6, 8, **META)},
         {"bias": _z(5)},
         {"bias": _z(1, 6)},
         {"bias": _z(12)[::2]},
         {"bias": _z(6, dtype=torch.float32)},
-        {"bias": _z(6, **META)},
         {"residual": _z(6)},
         {"residual": _z(5, 6, dtype=torch.float32)},
-        {"residual": _z(5, 6, **META)},
         {"activation": "swish"},
         {"activation": 3},
         {"out": _z(5, 7)},
         {"out": _z(6, 5).t()},
         {"out": _z(5, 6, dtype=torch.float32)},
-        {"out": _z(5, 6, **META)},
     ],
 )
-def test_linear_act_refuses(recorder, kw):
-    with pytest.raises(ValueError):
-        ops.linear_act(**{"x": _z(5, 8), "weight": _z(6, 8), **kw})
-    assert not recorder.calls
+def test_linear_act_refuses(kw):
+    good = {"x": _z(5, 8), "weight": _z(6, 8), "bias": _z(6), "residual": _z(5, 6), "activation": "silu"}
+    assert HOST in _refused(ops.linear_act, **good)
+    assert HOST not in _refused(ops.linear_act, **{**good, **kw})
 
 
 @pytest.mark.parametrize(
@@ -135,43 +99,30 @@ def test_linear_act_refuses(recorder, kw):
         {"pre": None},
         {"pre": _z(5, 7)},
         {"pre": _z(5, 6, dtype=torch.float32)},
-        {"pre": _z(5, 6, **META)},
         {"dy": _z(5, 8)},
         {"dy": _z(5, 6, dtype=torch.bfloat16)},
-        {"dy": _z(5, 6, **META)},
         {"x": _z(4, 8)},
         {"activation": "tanh"},
     ],
 )
-def test_linear_act_bwd_refuses(recorder, kw):
-    with pytest.raises(ValueError):
-        ops.linear_act_bwd(**{"dy": _z(5, 6), "x": _z(5, 8), "weight": _z(6, 8), "pre": _z(5, 6), "activation": "gelu", **kw})
-    assert not recorder.calls
+def test_linear_act_bwd_refuses(kw):
+    good = {"dy": _z(5, 6), "x": _z(5, 8), "weight": _z(6, 8), "pre": _z(5, 6), "activation": "gelu"}
+    assert HOST in _refused(ops.linear_act_bwd, **good)
+    assert HOST not in _refused(ops.linear_act_bwd, **{**good, **kw})
 
 
-def test_empty_batches_launch_nothing(recorder):
-    y, mean, rstd = ops.layernorm_fwd(_z(0, 8), _z(8), want_stats=True)
-    dx, dw, db = ops.layernorm_bwd(_z(0, 8), _z(0, 8), mean, rstd, _z(8))
-    assert y.shape == dx.shape == (0, 8) and mean.shape == (0,) and not dw.any() and not db.any()
-    y, pre = ops.linear_act(_z(2, 0, 8), _z(6, 8), want_pre=True)
-    dx, dw, db = ops.linear_act_bwd(_z(2, 0, 6), _z(2, 0, 8), _z(6, 8))
-    assert y.shape == pre.shape == (2, 0, 6) and dx.shape == (2, 0, 8) and not dw.any() and not db.any()
-    assert not recorder.calls
-
-
-def test_strides_reach_the_kernel(recorder):
-    """Rows any distance apart are passed on as they lie; columns that are not next to one another are copied first."""
-    ops.layernorm_fwd(_z(5, 20)[:, 3:11], _z(8), want_stats=True)
-    ops.layernorm_fwd(_z(8, 5).t())
-    ops.layernorm_bwd(_z(1, 8).expand(5, 8), _z(5, 9)[:, :8], _z(5, dtype=torch.float32), _z(5, dtype=torch.float32))
-    (_, a), (_, b), (_, c) = recorder.calls
-    assert (a[1], a[5], a[8:12]) == (20, 8, (5, 8, 0, 0)) and b[1] == 8 and (c[1], c[3], c[8], c[9]) == (0, 9, 8, None)
-    recorder.calls.clear()
-    ops.linear_act(_z(5, 20)[:, 3:11], _z(6, 8), residual=_z(1, 6).expand(5, 6), activation="silu")
-    ops.linear_act_bwd(_z(5, 7)[:, :6], _z(5, 8), _z(6, 12)[:, :8], pre=_z(5, 6), activation="gelu", want_dweight=False)
-    (_, a), (_, b) = recorder.calls
-    assert (a["ldx"], a["ldw"], a["ldr"], a["ldy"], a["M"], a["N"], a["K"], a["act"]) == (20, 8, 0, 6, 5, 6, 8, 2) and a["pre"] is None
-    assert (b["lddy"], b["ldw"], b["ldp"], b["lddx"], b["act"], b["dweight"]) == (7, 12, 6, 8, 3, None) and b["workspace_bytes"] == 1024
+@pytest.mark.parametrize("what", [None, 3, [1.0], "x"])
+def test_no_tensor(what):
+    """Something else than a tensor is a TypeError, as for PyTorch's own operators."""
+    x, w, s = _z(5, 8), _z(6, 8), _z(5, dtype=torch.float32)
+    for call in (lambda: ops.layernorm_fwd(what), lambda: ops.layernorm_bwd(what, x, s, s), lambda: ops.linear_act(what, w), lambda: ops.linear_act_bwd(_z(5, 6), x, what)):
+        with pytest.raises(TypeError):
+            call()
+    if what is not None:
+        with pytest.raises(TypeError):
+            ops.layernorm_fwd(x, bias=what)
+    with pytest.raises(TypeError):
+        ops.layernorm_fwd(x, eps="small")
 
 
 # ---- the C entry points: refused before any CUDA call --------------------------------------------
