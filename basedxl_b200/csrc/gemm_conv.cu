@@ -418,8 +418,27 @@ __host__ __device__ inline int acc_sets(int parts, int bn) { return parts == 1 ?
 // instantiation, so that each variant carries only its own epilogue (and its registers).
 // kTwo: operands in two fp16 parts (p.parts == 2); likewise separate.
 // kLin: linear layers with an activation, of fp16 (1) or bf16 (2) operands; 0 everywhere else.
-template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin = 0>
-__global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const __grid_constant__ GemmParams p) {
+// Two products that do not depend on one another can share a launch (GemmTwo): the first `first` CTAs work on one, the others on
+// the other, each as if its share were the grid.
+struct GemmTwo {
+  GemmParams p[2];
+  unsigned first;
+};
+struct GridShare {
+  int block, blocks;
+};
+__device__ __forceinline__ const GemmParams& product_of(const GemmParams& q) { return q; }
+__device__ __forceinline__ const GemmParams& product_of(const GemmTwo& q) { return q.p[blockIdx.x >= q.first ? 1 : 0]; }
+__device__ __forceinline__ GridShare share_of(const GemmParams&) { return {static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x)}; }
+__device__ __forceinline__ GridShare share_of(const GemmTwo& q) {
+  return blockIdx.x >= q.first ? GridShare{static_cast<int>(blockIdx.x - q.first), static_cast<int>(gridDim.x - q.first)}
+                               : GridShare{static_cast<int>(blockIdx.x), static_cast<int>(q.first)};
+}
+template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin = 0, class Products = GemmParams>
+__global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const __grid_constant__ Products products) {
+  const GemmParams& p = product_of(products);
+  const GridShare grid = share_of(products);
+  static_assert(std::is_same_v<Products, GemmParams> || !(kPair || kSplit), "two products: one CTA a tile");
   static_assert(!(kPair && kSplit), "a CTA pair walks the whole K range");
   static_assert(!(kConv && kTwo), "convolutions have fp16 operands");
   static_assert(!kLin || !(kConv || kTwo), "an epilogue of plain products");
@@ -509,8 +528,8 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
   const int kb_begin = static_cast<int>((static_cast<long long>(krank) * num_kb) / S);
   const int kb_end = static_cast<int>((static_cast<long long>(krank + 1) * num_kb) / S);
   const int main_sets = sets > 1 ? min(sets - 1, kb_end - kb_begin) : 1;   // accumulators of hi*hi, each over at least one k-block
-  const int first_tile = blockIdx.x / (S * kWidth);
-  const int tile_step = gridDim.x / (S * kWidth);
+  const int first_tile = grid.block / (S * kWidth);
+  const int tile_step = grid.blocks / (S * kWidth);
 
   if (warp == kWarpA || warp == kWarpB) {
     // ======================= TMA producers =======================
@@ -973,6 +992,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
 struct TileConfig {
   int bn, split, stages, pair;
   int clusters;   // of the CTAs that share a tile: how many can be resident at one time
+  double cost_us; // what the time model says
 };
 
 constexpr int kSmemLnExtra = 1024;           // the weight column-sum row of a GEMM with a folded LayerNorm
@@ -1006,7 +1026,7 @@ static std::atomic<int> g_clusters[64][5] = {};
 static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int force_bn = 0, int force_split = 0,
                                int force_pair = -1, double a_min_us = 0.0, int extra_smem = 0, int parts = 1, bool heavy = false) {
   const int sms = sm_count();
-  TileConfig best{128, 1, stages_for(128, 1, 0, extra_smem, parts), 0, sms};
+  TileConfig best{128, 1, stages_for(128, 1, 0, extra_smem, parts), 0, sms, 0.0};
   int at_once[5] = {0, sms, 0, 0, 0};
   for (int w = 2; w <= 4; w *= 2) at_once[w] = resident_clusters(gemm_conv_kernel<false, false, true, false>, gemm_threads(0), kSmemBudget, w, g_clusters);
   double best_cost = 1e30;
@@ -1037,12 +1057,33 @@ static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int fo
         const double cost = (rounds * (kb_unit * kb_us + epi_us + pair_tile_us) + fill_us) * (1.0 - 0.05 * bn / 256.0);
         if (cost < best_cost - 1e-9) {
           best_cost = cost;
-          best = TileConfig{bn, split, st, pair, clusters};
+          best = TileConfig{bn, split, st, pair, clusters, cost};
         }
       }
     }
   }
   return best;
+}
+
+// The same model for one round of single CTAs.
+static double tiles_cost(int num_kb, int bn, bool heavy) {
+  const double kb_us = fmax(bn / 256.0 * 0.256, (16384.0 + bn * 128.0) / 139000.0);
+  return (num_kb * kb_us + (heavy ? 0.455 : 0.271) * (bn / 32.0) + 4.28) * (1.0 - 0.05 * bn / 256.0);
+}
+// Of two launches in a row the second one's set-up runs beside the first.
+constexpr double kOverlapUs = 1.5;
+template <int kLin>
+static int launch_two(const GemmTwo& two, int ctas, int smem, cudaStream_t stream) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !configured[dev]) {
+    if (int rc = check_cuda(cudaFuncSetAttribute(gemm_conv_kernel<false, false, false, false, kLin, GemmTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget),
+                            "cudaFuncSetAttribute(gemm)"))
+      return rc;
+    configured[dev] = true;
+  }
+  return launch_kernel("gemm_conv_kernel launch", gemm_conv_kernel<false, false, false, false, kLin, GemmTwo>, dim3(ctas), dim3(gemm_threads(kLin)), smem, stream, 1, two);
 }
 
 template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin>
@@ -1266,16 +1307,22 @@ int repack_rows(const RowCopy& a, const RowCopy& b, cudaStream_t s) {
   return launch_kernel("repack_rows_kernel launch", repack_rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, oa, ob);
 }
 
-int linear_product(const LinearProduct& q, cudaStream_t stream) {
+static bool linear_ragged(const LinearProduct& q) {
+  auto rows16 = [](const void* base, long long ld) { return aligned16(base) && ld % 8 == 0; };
+  return q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && !rows16(q.residual, q.ldr)) || (q.pre && !rows16(q.pre, q.ldp));
+}
+static int linear_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : kSmemOutExtra; }
+static bool linear_heavy(const LinearProduct& q) { return linear_ragged(q) || q.residual || q.pre; }
+static int tiles_along(int n, int of) { return (int)(((long long)n + of - 1) / of); }
+static TileConfig linear_tiles(const LinearProduct& q) {
+  return choose_tiles(tiles_along(q.M, kBM), q.N, tiles_along(q.K, kBK), q.b_kn != 0, g_force_bn, g_force_split, g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, linear_extra(q), 1,
+                      linear_heavy(q));
+}
+static int linear_params(const LinearProduct& q, const TileConfig& tc, GemmParams& p) {
   int* st = device_status_ptr();
   if (!st) return fail(kErrCuda, "linear layer: no device status word");
-  GemmParams p;
   memset(&p, 0, sizeof(p));
-  auto rows16 = [](const void* base, long long ld) { return aligned16(base) && ld % 8 == 0; };
-  const bool ragged = q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && !rows16(q.residual, q.ldr)) || (q.pre && !rows16(q.pre, q.ldp));
-  const int tiles_m = (int)(((long long)q.M + kBM - 1) / kBM);
-  const TileConfig tc = choose_tiles(tiles_m, q.N, (int)(((long long)q.K + kBK - 1) / kBK), q.b_kn != 0, g_force_bn, g_force_split, g_force_pair < 0 ? kDefaultPair : g_force_pair,
-                                     0.0, ragged ? ragged_bytes(1) : kSmemOutExtra, 1, ragged || q.residual || q.pre);
+  const bool ragged = linear_ragged(q);
   {
     // [M,K], or [K,M] in boxes of 64 by 64
     uint64_t dims[2] = {(uint64_t)(q.a_mn ? q.M : q.K), (uint64_t)(q.a_mn ? q.K : q.M)};
@@ -1305,8 +1352,61 @@ int linear_product(const LinearProduct& q, cudaStream_t stream) {
   }
   p.C = q.C, p.ldc = q.ldc, p.pre = q.pre, p.ldp = q.ldp, p.act = q.act, p.ragged = ragged ? 1 : 0;
   p.dev_status = st;
-  const int tiles_n = (q.N + tc.bn - 1) / tc.bn;
+  return kOk;
+}
+
+int linear_product(const LinearProduct& q, cudaStream_t stream) {
+  const TileConfig tc = linear_tiles(q);
+  GemmParams p;
+  if (int rc = linear_params(q, tc, p)) return rc;
+  const int tiles_m = tiles_along(q.M, kBM), tiles_n = tiles_along(q.N, tc.bn);
   return q.bf16 ? launch<false, false, 2>(p, tiles_m, tiles_n, stream) : launch<false, false, 1>(p, tiles_m, tiles_n, stream);
+}
+
+// Both in one launch where all their tiles run at once; otherwise, and where the time model says so, one after the other.
+int linear_products(const LinearProduct& a, const LinearProduct& b, int* launches, cudaStream_t stream) {
+  const LinearProduct* q[2] = {&a, &b};
+  TileConfig tc[2];
+  double cost[2][4];
+  int tiles[2][4];
+  for (int i = 0; i < 2; ++i) {
+    tc[i] = linear_tiles(*q[i]);
+    for (int w = 0; w < 4; ++w) {
+      const int bn = 64 * (w + 1);
+      tiles[i][w] = 0;
+      const long long all = (long long)tiles_along(q[i]->M, kBM) * tiles_along(q[i]->N, bn);
+      if (all > sm_count() || stages_for(bn, 1, 0, linear_extra(*q[i])) < 3) continue;
+      tiles[i][w] = (int)all;
+      cost[i][w] = tiles_cost(tiles_along(q[i]->K, kBK), bn, linear_heavy(*q[i]));
+    }
+  }
+  double best = tc[0].cost_us + tc[1].cost_us - kOverlapUs;
+  int wa = -1, wb = -1;
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) {
+      if (!tiles[0][i] || !tiles[1][j] || tiles[0][i] + tiles[1][j] > sm_count()) continue;
+      const double c = cost[0][i] > cost[1][j] ? cost[0][i] : cost[1][j];
+      if (c < best) best = c, wa = i, wb = j;
+    }
+  if (wa < 0 || g_force_bn || g_force_split || g_force_pair >= 0 || a.bf16 != b.bf16) {
+    if (int rc = linear_product(a, stream)) return rc;
+    if (int rc = linear_product(b, stream)) return rc;
+    *launches += 2;
+    return kOk;
+  }
+  GemmTwo two;
+  int smem = 0;
+  const int w[2] = {wa, wb};
+  for (int i = 0; i < 2; ++i) {
+    const int bn = 64 * (w[i] + 1), extra = linear_extra(*q[i]);
+    const TileConfig one{bn, 1, stages_for(bn, 1, 0, extra), 0, sm_count(), 0.0};
+    if (int rc = linear_params(*q[i], one, two.p[i])) return rc;
+    const int bytes = one.stages * (kABytes + bn * 128) + kSmemMisc + extra;
+    smem = bytes > smem ? bytes : smem;
+  }
+  two.first = (unsigned)tiles[0][wa];
+  *launches += 1;
+  return a.bf16 ? launch_two<2>(two, tiles[0][wa] + tiles[1][wb], smem, stream) : launch_two<1>(two, tiles[0][wa] + tiles[1][wb], smem, stream);
 }
 }  // namespace bxl
 

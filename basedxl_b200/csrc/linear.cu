@@ -373,20 +373,20 @@ extern "C" int bxl_linear_act_bwd(const bxl_linear_args* a, int* launches, void*
     if (int rc = repack_rows(x, w, s)) return rc;
     ++count;
   }
-  LinearProduct q = {};
-  q.bf16 = bf16;
-  if (a->dx) {
-    // dx[M,K] = dz[M,N] W[N,K]
-    q.A = dz, q.lda = ldz, q.a_mn = 0, q.B = w.dst ? w.dst : w.src, q.ldb = w.ld_dst, q.b_kn = 1, q.b_is_weight = !w.dst;
-    q.C = a->dx, q.ldc = a->lddx, q.M = a->M, q.N = a->K, q.K = a->N;
-    if (int rc = linear_product(q, s)) return rc;
-    ++count;
-  }
-  if (a->dweight) {
-    // dW[N,K] = dz^T[N,M] x[M,K]
-    q.A = dz, q.lda = ldz, q.a_mn = 1, q.B = x.dst ? x.dst : x.src, q.ldb = x.ld_dst, q.b_kn = 1, q.b_is_weight = 0;
-    q.C = a->dweight, q.ldc = a->lddw, q.M = a->N, q.N = a->K, q.K = a->M;
-    if (int rc = linear_product(q, s)) return rc;
+  // dx[M,K] = dz[M,N] W[N,K]
+  LinearProduct x_grad = {};
+  x_grad.bf16 = bf16;
+  x_grad.A = dz, x_grad.lda = ldz, x_grad.B = w.dst ? w.dst : w.src, x_grad.ldb = w.ld_dst, x_grad.b_kn = 1, x_grad.b_is_weight = !w.dst;
+  x_grad.C = a->dx, x_grad.ldc = a->lddx, x_grad.M = a->M, x_grad.N = a->K, x_grad.K = a->N;
+  // dW[N,K] = dz^T[N,M] x[M,K]
+  LinearProduct w_grad = {};
+  w_grad.bf16 = bf16;
+  w_grad.A = dz, w_grad.lda = ldz, w_grad.a_mn = 1, w_grad.B = x.dst ? x.dst : x.src, w_grad.ldb = x.ld_dst, w_grad.b_kn = 1;
+  w_grad.C = a->dweight, w_grad.ldc = a->lddw, w_grad.M = a->N, w_grad.N = a->K, w_grad.K = a->M;
+  if (a->dx && a->dweight) {
+    if (int rc = linear_products(x_grad, w_grad, &count, s)) return rc;
+  } else if (a->dx || a->dweight) {
+    if (int rc = linear_product(a->dx ? x_grad : w_grad, s)) return rc;
     ++count;
   }
   if (launches) *launches = count;

@@ -278,9 +278,12 @@ def test_counted_launches():
     odd = torch.zeros(300, 65, device="cuda", dtype=torch.float16)[:, 1:]
     assert count(lambda: ops.linear_act(x, w)) == 1 and count(lambda: ops.linear_act(odd, w)) == 2 and count(lambda: ops.linear_act(x[:2], w)) == 1
     assert count(lambda: ops.linear_act(x[:0], w)) == 0 and count(lambda: ops.linear_act_bwd(s["dy"][:0], x[:0], w)) == 0
-    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, pre, "gelu")) == 4     # dz, its sums, dx, dweight
-    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, want_dbias=False)) == 2
-    assert count(lambda: ops.linear_act_bwd(s["dy"][:9], x[:9], w, pre[:9], "gelu")) == 3
+    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, pre, "gelu")) == 3     # dz, its sums, both products
+    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, want_dbias=False)) == 1
+    assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, want_dbias=False, want_dx=False)) == 1
+    assert count(lambda: ops.linear_act_bwd(s["dy"][:9], x[:9], w, pre[:9], "gelu")) == 2
+    big = _inputs(3000, 1280, 1280, torch.float16)                                # more tiles than SMs: two launches
+    assert count(lambda: ops.linear_act_bwd(big["dy"], big["x"], big["weight"], want_dbias=False)) == 2
     n = torch.ones(64, device="cuda", dtype=torch.float16)
     rows = torch.zeros(2000, 64, device="cuda", dtype=torch.float16)
     _, mean, rstd = ops.layernorm_fwd(rows, n, want_stats=True)
