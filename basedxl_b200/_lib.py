@@ -59,7 +59,7 @@ SIGNATURES = {
     "bxl_gemm_ragged_workspace_bytes": (_ll, [_i, _i, _i]),
     "bxl_gemm_ragged_f16": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _ll, _vp, _ll, _i, _i, _i, _vp, _ll, _vp]),
     "bxl_linear_act_fwd_workspace_bytes": (_ll, [C.POINTER(LinearArgs)]),
-    "bxl_linear_act_fwd": (_i, [C.POINTER(LinearArgs), _vp]),
+    "bxl_linear_act_fwd": (_i, [C.POINTER(LinearArgs), C.POINTER(_i), _vp]),
     "bxl_linear_act_bwd_workspace_bytes": (_ll, [C.POINTER(LinearArgs)]),
     "bxl_linear_act_bwd": (_i, [C.POINTER(LinearArgs), C.POINTER(_i), _vp]),
     "bxl_conv_weight_pack_f16": (_i, [_vp, _vp, _i, _i, _vp]),

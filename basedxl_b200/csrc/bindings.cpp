@@ -263,7 +263,9 @@ PyObject* linear_act(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.workspace_bytes = bxl_linear_act_fwd_workspace_bytes(&a);
     const Tensor ws = a.workspace_bytes ? empty({a.workspace_bytes}, at::kByte, x.device()) : Tensor();
     if (ws.defined()) a.workspace = ws.mutable_data_ptr();
-    finish(bxl_linear_act_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()), ws.defined() ? 2 : 1);
+    int launches = 0;
+    const int rc = bxl_linear_act_fwd(&a, &launches, c10::cuda::getCurrentCUDAStream().stream());
+    finish(rc, launches);
   }
   if (!want_pre) return wrap(y);
   PyObject* r = PyTuple_New(2);

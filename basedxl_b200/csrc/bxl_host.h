@@ -87,9 +87,10 @@ struct LinearProduct {
   long long ldp;
   int act, bf16, M, N, K;
 };
-int linear_product(const LinearProduct& q, cudaStream_t stream);
-// Two that do not depend on one another, in one launch or two (added to *launches).
-int linear_products(const LinearProduct& a, const LinearProduct& b, int* launches, cudaStream_t stream);
+// One product, or two (n = 2) that do not depend on one another.  *launches grows by the kernels enqueued.  The workspace's size goes
+// by everything in the products but A and B.
+long long linear_workspace(const LinearProduct* const* q, int n);
+int linear_products(const LinearProduct* const* q, int n, void* workspace, int* launches, cudaStream_t stream);
 // Copies the rows of up to two 16-bit matrices to rows ld_dst (a multiple of 8) apart; dst null = nothing to copy.
 struct RowCopy {
   const void* src;

@@ -122,6 +122,11 @@ struct alignas(64) GemmParams {
   void* pre;                   // [M][ldp]: also store the value before the activation; or null
   long long ldp;
   int bias_vec;                // the bias starts at a 16-byte boundary
+  // few tiles and a long K: `slices` CTAs share a tile's K range and leave fp32 partial sums, [slices][M][part_ld], which a second
+  // launch joins and takes through the rest of the epilogue; 1 = the CTA does it all
+  int slices;
+  float* part;
+  long long part_ld;
   CUtensorMap c_map, pre_map;  // C and pre, for stores of 32 x 32 values (aligned rows)
 };
 
@@ -521,12 +526,23 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
   if (kConv) tiles_m1 = p.cB * p.tiles_y * p.tiles_x;
   else tiles_m1 = (p.M + kBM - 1) / kBM;
   const int tiles_m = kPair ? (tiles_m1 + 1) / 2 : tiles_m1;  // scheduling units along M (pairs of tiles in pair mode)
-  const int num_tiles = tiles_m * tiles_n;
+  const int whole_tiles = tiles_m * tiles_n;
+  const int num_tiles = whole_tiles * (kLin && !kSplit ? p.slices : 1);   // slices of a tile follow one another at that distance
   const int num_kb = kConv ? 9 * (p.cCin / kBK) : (p.K + kBK - 1) / kBK;
   // this CTA's share of the K loop (balanced; never empty because split <= num_kb)
   const uint32_t krank = kPair ? 0u : crank;  // both CTAs of a pair walk the whole K range
-  const int kb_begin = static_cast<int>((static_cast<long long>(krank) * num_kb) / S);
-  const int kb_end = static_cast<int>((static_cast<long long>(krank + 1) * num_kb) / S);
+  int kb_begin = static_cast<int>((static_cast<long long>(krank) * num_kb) / S);
+  int kb_end = static_cast<int>((static_cast<long long>(krank + 1) * num_kb) / S);
+  // which slice of its tile a tile index means; leaves the tile itself in `tile` and the slice's K range in kb_begin, kb_end
+  auto slice_of = [&](int& tile) {
+    if constexpr (kLin == 0 || kSplit) return 0;
+    if (p.slices == 1) return 0;
+    const int slice = tile / whole_tiles;
+    tile -= slice * whole_tiles;
+    kb_begin = static_cast<int>((static_cast<long long>(slice) * num_kb) / p.slices);
+    kb_end = static_cast<int>((static_cast<long long>(slice + 1) * num_kb) / p.slices);
+    return slice;
+  };
   const int main_sets = sets > 1 ? min(sets - 1, kb_end - kb_begin) : 1;   // accumulators of hi*hi, each over at least one k-block
   const int first_tile = grid.block / (S * kWidth);
   const int tile_step = grid.blocks / (S * kWidth);
@@ -549,7 +565,9 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+      for (int index = first_tile; index < num_tiles && ok; index += tile_step) {
+        int tile = index;
+        slice_of(tile);
         const int tm = (p.n_fastest ? tile / tiles_n : tile % tiles_m) * kWidth + (kPair ? static_cast<int>(crank) : 0);  // this CTA's 128-row tile
         const int tn = p.n_fastest ? tile % tiles_n : tile / tiles_m;
         const int n0 = tn * BN + (kPair ? static_cast<int>(crank) * b_rows : 0);           // first B row this CTA stages
@@ -662,7 +680,9 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
       uint32_t phase = 0;
       int it = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, ++it) {
+      for (int index = first_tile; index < num_tiles && ok; index += tile_step, ++it) {
+        int tile = index;
+        slice_of(tile);
         const int acc = it & 1;
         const uint32_t acc_phase = (it >> 1) & 1u;
         if (kPair ? !mbar_wait_cluster(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p.dev_status, 200)
@@ -742,7 +762,9 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
     const int cps = chunks / S;    // 32-column chunks per owner slice
     [[maybe_unused]] const uint32_t out_stage = smem_u32(s_turn) + warp * kOutBytes;
     int it = 0;
-    for (int tile = first_tile; tile < num_tiles; tile += tile_step, ++it) {
+    for (int index = first_tile; index < num_tiles; index += tile_step, ++it) {
+      int tile = index;
+      [[maybe_unused]] const int slice = slice_of(tile);
       const int acc = it & 1;
       const uint32_t acc_phase = (it >> 1) & 1u;
       const int tm = (p.n_fastest ? tile / tiles_n : tile % tiles_m) * kWidth + (kPair ? static_cast<int>(crank) : 0);
@@ -833,6 +855,14 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
             load_residual(p, out_row, nb, res_cur);
           }
           tmem_ld_wait();
+          if (p.slices > 1) {
+            if (out_row >= 0 && nb < p.N) {   // whole chunks: the partial sums' rows are padded to them
+              float* to = p.part + (static_cast<long long>(slice) * p.M + out_row) * p.part_ld + nb;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) st_global_v8(to + 8 * q, v[8 * q], v[8 * q + 1], v[8 * q + 2], v[8 * q + 3], v[8 * q + 4], v[8 * q + 5], v[8 * q + 6], v[8 * q + 7]);
+            }
+            continue;
+          }
           F2 f[16];
           add_bias<LinT>(v, bias, f);
           if (p.ragged) store_chunk_act_ragged<LinT>(p, f, row0, nb, s_turn + warp * kTurnFloats, lane);
@@ -1350,63 +1380,203 @@ static int linear_params(const LinearProduct& q, const TileConfig& tc, GemmParam
     if (q.pre)
       if (int rc = encode_tmap_f16(&p.pre_map, q.pre, 2, dims, pre_str, box, 64)) return rc;
   }
-  p.C = q.C, p.ldc = q.ldc, p.pre = q.pre, p.ldp = q.ldp, p.act = q.act, p.ragged = ragged ? 1 : 0;
+  p.C = q.C, p.ldc = q.ldc, p.pre = q.pre, p.ldp = q.ldp, p.act = q.act, p.ragged = ragged ? 1 : 0, p.slices = 1;
   p.dev_status = st;
   return kOk;
 }
 
-int linear_product(const LinearProduct& q, cudaStream_t stream) {
-  const TileConfig tc = linear_tiles(q);
-  GemmParams p;
-  if (int rc = linear_params(q, tc, p)) return rc;
-  const int tiles_m = tiles_along(q.M, kBM), tiles_n = tiles_along(q.N, tc.bn);
-  return q.bf16 ? launch<false, false, 2>(p, tiles_m, tiles_n, stream) : launch<false, false, 1>(p, tiles_m, tiles_n, stream);
+// ---- few tiles, long K ----
+// Adds the slices' partial sums of up to two products and finishes their epilogue.  Bound by memory: a thread has four
+// neighbouring columns of a row, and the slices' values are loaded eight at a time.
+struct JoinOne {
+  const float* part;
+  long long ld, slice;      // elements between rows and between slices
+  int slices, M, N;
+  const void *bias, *residual;
+  void *pre, *C;
+  long long ldr, ldp, ldc;
+  int act;
+};
+struct JoinTwo {
+  JoinOne q[2];
+  long long quads[2];       // threads' shares of each
+};
+template <class T>
+__global__ void __launch_bounds__(128) join_slices_kernel(const JoinTwo j) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long all = j.quads[0] + j.quads[1];
+  for (long long i = blockIdx.x * 128ll + threadIdx.x; i < all; i += gridDim.x * 128ll) {
+    const bool second = i >= j.quads[0];
+    const JoinOne& q = j.q[second];
+    const int per_row = (q.N + 3) / 4;
+    const long long k = second ? i - j.quads[0] : i, m = k / per_row;
+    const int n = static_cast<int>(k % per_row) * 4;
+    const float* from = q.part + m * q.ld + n;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < q.slices; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(from + s * q.slice);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    float f[4] = {sum.x, sum.y, sum.z, sum.w};
+    with_act(q.act, [&](auto act) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (n + e >= q.N) continue;
+        if (q.bias) f[e] += to_f32(static_cast<const T*>(q.bias)[n + e]);
+        if (q.pre) static_cast<T*>(q.pre)[m * q.ldp + n + e] = from_f32<T>(f[e]);
+        f[e] = act_value<decltype(act)::value>(f[e]);
+        if (q.residual) f[e] += to_f32(static_cast<const T*>(q.residual)[m * q.ldr + n + e]);
+        static_cast<T*>(q.C)[m * q.ldc + n + e] = from_f32<T>(f[e]);
+      }
+    });
+  }
 }
 
-// Both in one launch where all their tiles run at once; otherwise, and where the time model says so, one after the other.
-int linear_products(const LinearProduct& a, const LinearProduct& b, int* launches, cudaStream_t stream) {
-  const LinearProduct* q[2] = {&a, &b};
+// One round of single CTAs on at most `ctas` of them: tile width, slices of K, and what the time model says.
+struct Sliced {
+  int bn = 0, slices = 1, tiles = 0;
+  double cost_us = 1e30;
+};
+static long long part_ld(const LinearProduct& q) { return (q.N + 31ll) / 32 * 32; }
+static long long part_bytes(const LinearProduct& q, int slices) { return slices > 1 ? (4ll * slices * q.M * part_ld(q) + 255) / 256 * 256 : 0; }
+constexpr long long kMaxPartBytes = 32ll << 20;
+static Sliced sliced_within(const LinearProduct& q, int ctas) {
+  Sliced best;
+  const int kb = tiles_along(q.K, kBK);
+  for (int bn = 64; bn <= 256; bn += 64) {
+    const long long tiles = (long long)tiles_along(q.M, kBM) * tiles_along(q.N, bn);
+    if (tiles > ctas || stages_for(bn, 1, 0, linear_extra(q)) < 3) continue;
+    const double whole = tiles_cost(kb, bn, linear_heavy(q));
+    if (whole < best.cost_us) best.bn = bn, best.slices = 1, best.tiles = (int)tiles, best.cost_us = whole;
+    int s = (int)(ctas / tiles);
+    s = s < kb / 2 ? s : kb / 2;
+    while (s > 1 && part_bytes(q, s) > kMaxPartBytes) s /= 2;
+    if (s < 2) continue;
+    const int per = (kb + s - 1) / s;
+    s = (kb + per - 1) / per;
+    const double c = tiles_cost(per, bn, true) + 3.0 + part_bytes(q, s) / 2.0e6;   // the second launch reads what the first has left in L2
+    if (s > 1 && c < best.cost_us) best.bn = bn, best.slices = s, best.tiles = (int)tiles, best.cost_us = c;
+  }
+  return best;
+}
+static bool forced() { return g_force_bn || g_force_split || g_force_pair >= 0; }
+
+struct LinearPlan {
+  bool together = false;     // both products in one launch of single CTAs
+  bool sliced[2] = {};       // (not together) the sliced form instead of `tc`
+  Sliced single[2];
   TileConfig tc[2];
-  double cost[2][4];
-  int tiles[2][4];
-  for (int i = 0; i < 2; ++i) {
-    tc[i] = linear_tiles(*q[i]);
-    for (int w = 0; w < 4; ++w) {
-      const int bn = 64 * (w + 1);
-      tiles[i][w] = 0;
-      const long long all = (long long)tiles_along(q[i]->M, kBM) * tiles_along(q[i]->N, bn);
-      if (all > sm_count() || stages_for(bn, 1, 0, linear_extra(*q[i])) < 3) continue;
-      tiles[i][w] = (int)all;
-      cost[i][w] = tiles_cost(tiles_along(q[i]->K, kBK), bn, linear_heavy(*q[i]));
+  int slices(int i) const { return together || sliced[i] ? single[i].slices : 1; }
+};
+static LinearPlan make_plan(const LinearProduct* const* q, int n) {
+  LinearPlan plan;
+  double apart = 0.0;
+  for (int i = 0; i < n; ++i) {
+    plan.tc[i] = linear_tiles(*q[i]);
+    plan.single[i] = sliced_within(*q[i], sm_count());
+    // the plain forms' times are better known: a tenth of margin
+    plan.sliced[i] = !forced() && plan.single[i].slices > 1 && plan.single[i].cost_us < 0.9 * plan.tc[i].cost_us;
+    apart += plan.sliced[i] ? plan.single[i].cost_us : plan.tc[i].cost_us;
+  }
+  if (n < 2 || forced()) return plan;
+  apart -= kOverlapUs;
+  for (int part = 1; part <= 7; ++part) {   // shares of the SMs
+    const int ctas = sm_count() * part / 8;
+    const Sliced a = sliced_within(*q[0], ctas), b = sliced_within(*q[1], sm_count() - ctas);
+    const double c = a.cost_us > b.cost_us ? a.cost_us : b.cost_us;
+    if (c < apart) apart = c, plan.together = true, plan.single[0] = a, plan.single[1] = b;
+  }
+  return plan;
+}
+// A plan goes by extents, layouts and alignment alone and takes 2 to 4 us to make: the last ones of this thread are kept, under all
+// that they go by.
+struct PlanKey {
+  int v[2][5], n, sms, bn, split, pair;
+  bool operator==(const PlanKey& o) const { return memcmp(this, &o, sizeof(o)) == 0; }
+};
+static const LinearPlan& plan_products(const LinearProduct* const* q, int n) {
+  PlanKey key;
+  memset(&key, 0, sizeof(key));
+  unsigned hash = 0;
+  for (int i = 0; i < n; ++i) {
+    const int v[5] = {q[i]->M, q[i]->N, q[i]->K, q[i]->b_kn, (linear_ragged(*q[i]) ? 2 : 0) + (linear_heavy(*q[i]) ? 1 : 0)};
+    for (int j = 0; j < 5; ++j) key.v[i][j] = v[j], hash = hash * 31u + (unsigned)v[j];
+  }
+  key.n = n, key.sms = sm_count(), key.bn = g_force_bn, key.split = g_force_split, key.pair = g_force_pair;
+  struct Entry {
+    PlanKey key;
+    LinearPlan plan;
+  };
+  static thread_local Entry table[64] = {};
+  Entry& e = table[(hash ^ (hash >> 13)) % 64];
+  if (!(e.key == key)) e.key = key, e.plan = make_plan(q, n);
+  return e.plan;
+}
+static int sliced_params(const LinearProduct& q, const Sliced& f, float* part, GemmParams& p, int& smem) {
+  const int extra = linear_extra(q);
+  const TileConfig one{f.bn, 1, stages_for(f.bn, 1, 0, extra), 0, sm_count(), 0.0};
+  if (int rc = linear_params(q, one, p)) return rc;
+  p.slices = f.slices, p.part = part, p.part_ld = part_ld(q);
+  smem = one.stages * (kABytes + f.bn * 128) + kSmemMisc + extra;
+  return kOk;
+}
+static JoinOne join_of(const LinearProduct& q, int slices, const float* part) {
+  return JoinOne{part, part_ld(q), q.M * part_ld(q), slices, q.M, q.N, q.bias, q.residual, q.pre, q.C, q.ldr, q.ldp, q.ldc, q.act};
+}
+
+long long linear_workspace(const LinearProduct* const* q, int n) {
+  const LinearPlan& plan = plan_products(q, n);
+  long long bytes = 0;
+  for (int i = 0; i < n; ++i) bytes += part_bytes(*q[i], plan.slices(i));
+  return bytes;
+}
+
+int linear_products(const LinearProduct* const* q, int n, void* workspace, int* launches, cudaStream_t stream) {
+  const LinearPlan plan = plan_products(q, n);
+  const bool bf16 = q[0]->bf16;
+  float* part[2] = {static_cast<float*>(workspace), static_cast<float*>(workspace)};
+  if (n == 2) part[1] += part_bytes(*q[0], plan.slices(0)) / 4;
+  if (plan.together) {
+    GemmTwo two;
+    int smem[2];
+    for (int i = 0; i < 2; ++i)
+      if (int rc = sliced_params(*q[i], plan.single[i], part[i], two.p[i], smem[i])) return rc;
+    two.first = (unsigned)(plan.single[0].tiles * plan.single[0].slices);
+    const int ctas = (int)two.first + plan.single[1].tiles * plan.single[1].slices, most = smem[0] > smem[1] ? smem[0] : smem[1];
+    if (int rc = bf16 ? launch_two<2>(two, ctas, most, stream) : launch_two<1>(two, ctas, most, stream)) return rc;
+    ++*launches;
+  } else {
+    for (int i = 0; i < n; ++i) {
+      GemmParams p;
+      int smem, rc;
+      if (plan.sliced[i]) {
+        if ((rc = sliced_params(*q[i], plan.single[i], part[i], p, smem))) return rc;
+        const int units = plan.single[i].tiles * plan.single[i].slices;
+        rc = bf16 ? launch_one<false, false, false, false, 2>(p, units, stream) : launch_one<false, false, false, false, 1>(p, units, stream);
+      } else {
+        if ((rc = linear_params(*q[i], plan.tc[i], p))) return rc;
+        const int tiles_m = tiles_along(q[i]->M, kBM), tiles_n = tiles_along(q[i]->N, plan.tc[i].bn);
+        rc = bf16 ? launch<false, false, 2>(p, tiles_m, tiles_n, stream) : launch<false, false, 1>(p, tiles_m, tiles_n, stream);
+      }
+      if (rc) return rc;
+      ++*launches;
     }
   }
-  double best = tc[0].cost_us + tc[1].cost_us - kOverlapUs;
-  int wa = -1, wb = -1;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      if (!tiles[0][i] || !tiles[1][j] || tiles[0][i] + tiles[1][j] > sm_count()) continue;
-      const double c = cost[0][i] > cost[1][j] ? cost[0][i] : cost[1][j];
-      if (c < best) best = c, wa = i, wb = j;
+  JoinTwo j = {};
+  int joins = 0;
+  for (int i = 0; i < n; ++i)
+    if (plan.slices(i) > 1) {
+      j.q[joins] = join_of(*q[i], plan.slices(i), part[i]);
+      j.quads[joins++] = (long long)q[i]->M * ((q[i]->N + 3) / 4);
     }
-  if (wa < 0 || g_force_bn || g_force_split || g_force_pair >= 0 || a.bf16 != b.bf16) {
-    if (int rc = linear_product(a, stream)) return rc;
-    if (int rc = linear_product(b, stream)) return rc;
-    *launches += 2;
-    return kOk;
-  }
-  GemmTwo two;
-  int smem = 0;
-  const int w[2] = {wa, wb};
-  for (int i = 0; i < 2; ++i) {
-    const int bn = 64 * (w[i] + 1), extra = linear_extra(*q[i]);
-    const TileConfig one{bn, 1, stages_for(bn, 1, 0, extra), 0, sm_count(), 0.0};
-    if (int rc = linear_params(*q[i], one, two.p[i])) return rc;
-    const int bytes = one.stages * (kABytes + bn * 128) + kSmemMisc + extra;
-    smem = bytes > smem ? bytes : smem;
-  }
-  two.first = (unsigned)tiles[0][wa];
-  *launches += 1;
-  return a.bf16 ? launch_two<2>(two, tiles[0][wa] + tiles[1][wb], smem, stream) : launch_two<1>(two, tiles[0][wa] + tiles[1][wb], smem, stream);
+  if (!joins) return kOk;
+  const long long blocks = (j.quads[0] + j.quads[1] + 127) / 128, most = sm_count() * 16ll;
+  ++*launches;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  return bf16 ? launch_kernel("join_slices_kernel launch", join_slices_kernel<__nv_bfloat16>, grid, dim3(128), 0, stream, 1, j)
+              : launch_kernel("join_slices_kernel launch", join_slices_kernel<__half>, grid, dim3(128), 0, stream, 1, j);
 }
 }  // namespace bxl
 

@@ -277,9 +277,29 @@ static int check_workspace(const char* who, const bxl_linear_args* a, long long 
   return kOk;
 }
 
+// z = x W^T, before the operands' places are known
+static LinearProduct forward_product(const bxl_linear_args* a) {
+  LinearProduct q = {};
+  q.bf16 = a->dtype == BXL_BF16, q.bias = a->bias, q.residual = a->residual, q.ldr = a->ldr, q.C = a->y, q.ldc = a->ldy, q.pre = a->pre, q.ldp = a->ldp;
+  q.act = a->act, q.M = a->M, q.N = a->N, q.K = a->K;
+  return q;
+}
+// dx[M,K] = dz[M,N] W[N,K]
+static LinearProduct x_grad_product(const bxl_linear_args* a) {
+  LinearProduct q = {};
+  q.bf16 = a->dtype == BXL_BF16, q.b_kn = 1, q.C = a->dx, q.ldc = a->lddx, q.M = a->M, q.N = a->K, q.K = a->N;
+  return q;
+}
+// dW[N,K] = dz^T[N,M] x[M,K]
+static LinearProduct w_grad_product(const bxl_linear_args* a) {
+  LinearProduct q = {};
+  q.bf16 = a->dtype == BXL_BF16, q.a_mn = 1, q.b_kn = 1, q.C = a->dweight, q.ldc = a->lddw, q.M = a->N, q.N = a->K, q.K = a->M;
+  return q;
+}
 static long long fwd_workspace(const bxl_linear_args* a) {
   if (a->M <= kFewRows) return 0;
-  return round256(copy_bytes(a->x, a->ldx, a->M, a->K)) + round256(copy_bytes(a->weight, a->ldw, a->N, a->K));
+  const LinearProduct q = forward_product(a), *one = &q;
+  return round256(copy_bytes(a->x, a->ldx, a->M, a->K)) + round256(copy_bytes(a->weight, a->ldw, a->N, a->K)) + linear_workspace(&one, 1);
 }
 // dz is dy itself where there is no activation and the copy engine can read it
 static bool stores_dz(const bxl_linear_args* a) {
@@ -291,6 +311,9 @@ static long long bwd_workspace(const bxl_linear_args* a) {
   if (a->dbias && a->M > kDzFew) n += round256(4ll * dz_shares(a->M, a->N, 1) * a->N);
   if (a->dx) n += round256(copy_bytes(a->weight, a->ldw, a->N, a->K));
   if (a->dweight) n += round256(copy_bytes(a->x, a->ldx, a->M, a->K));
+  const LinearProduct x = x_grad_product(a), w = w_grad_product(a);
+  const LinearProduct* q[2] = {a->dx ? &x : &w, &w};
+  if (a->dx || a->dweight) n += linear_workspace(q, a->dx && a->dweight ? 2 : 1);
   return n;
 }
 
@@ -300,7 +323,7 @@ using namespace bxl;
 
 extern "C" long long bxl_linear_act_fwd_workspace_bytes(const bxl_linear_args* a) { return check_linear("bxl_linear_act_fwd", a) ? 0 : fwd_workspace(a); }
 
-extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, void* stream) {
+extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, int* launches, void* stream) {
   const char* who = "bxl_linear_act_fwd";
   if (int rc = check_linear(who, a)) return rc;
   if (!a->y) return fail(kErrInvalidArg, "%s: null operand", who);
@@ -308,6 +331,8 @@ extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, void* stream) {
   if (int rc = check_workspace(who, a, fwd_workspace(a))) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   const int bf16 = a->dtype == BXL_BF16;
+  int count = 0;
+  if (launches) *launches = 1;
   if (a->M <= kFewRows) {
     const FewRows p{a->x, a->weight, a->bias, a->residual, a->y, a->pre, a->ldx, a->ldw, a->ldr, a->ldy, a->ldp, a->M, a->N, a->K, a->act};
     const bool vec = a->K % 8 == 0 && al(a->x, 16) && al(a->weight, 16) && a->ldx % 8 == 0 && a->ldw % 8 == 0;
@@ -318,11 +343,13 @@ extern "C" int bxl_linear_act_fwd(const bxl_linear_args* a, void* stream) {
   if (const long long n = copy_bytes(a->x, a->ldx, a->M, a->K)) x.dst = ws.take(n), x.ld_dst = round8(a->K);
   if (const long long n = copy_bytes(a->weight, a->ldw, a->N, a->K)) w.dst = ws.take(n), w.ld_dst = round8(a->K);
   if (int rc = repack_rows(x, w, s)) return rc;
-  LinearProduct q = {};
+  LinearProduct q = forward_product(a);
+  const LinearProduct* one = &q;
   q.A = x.dst ? x.dst : x.src, q.lda = x.ld_dst, q.B = w.dst ? w.dst : w.src, q.ldb = w.ld_dst, q.b_is_weight = !w.dst;
-  q.bias = a->bias, q.residual = a->residual, q.ldr = a->ldr, q.C = a->y, q.ldc = a->ldy, q.pre = a->pre, q.ldp = a->ldp;
-  q.act = a->act, q.bf16 = bf16, q.M = a->M, q.N = a->N, q.K = a->K;
-  return linear_product(q, s);
+  if (x.dst || w.dst) ++count;
+  if (int rc = linear_products(&one, 1, ws.at, &count, s)) return rc;
+  if (launches) *launches = count;
+  return kOk;
 }
 
 extern "C" long long bxl_linear_act_bwd_workspace_bytes(const bxl_linear_args* a) { return check_linear("bxl_linear_act_bwd", a) ? 0 : bwd_workspace(a); }
@@ -373,22 +400,12 @@ extern "C" int bxl_linear_act_bwd(const bxl_linear_args* a, int* launches, void*
     if (int rc = repack_rows(x, w, s)) return rc;
     ++count;
   }
-  // dx[M,K] = dz[M,N] W[N,K]
-  LinearProduct x_grad = {};
-  x_grad.bf16 = bf16;
-  x_grad.A = dz, x_grad.lda = ldz, x_grad.B = w.dst ? w.dst : w.src, x_grad.ldb = w.ld_dst, x_grad.b_kn = 1, x_grad.b_is_weight = !w.dst;
-  x_grad.C = a->dx, x_grad.ldc = a->lddx, x_grad.M = a->M, x_grad.N = a->K, x_grad.K = a->N;
-  // dW[N,K] = dz^T[N,M] x[M,K]
-  LinearProduct w_grad = {};
-  w_grad.bf16 = bf16;
-  w_grad.A = dz, w_grad.lda = ldz, w_grad.a_mn = 1, w_grad.B = x.dst ? x.dst : x.src, w_grad.ldb = x.ld_dst, w_grad.b_kn = 1;
-  w_grad.C = a->dweight, w_grad.ldc = a->lddw, w_grad.M = a->N, w_grad.N = a->K, w_grad.K = a->M;
-  if (a->dx && a->dweight) {
-    if (int rc = linear_products(x_grad, w_grad, &count, s)) return rc;
-  } else if (a->dx || a->dweight) {
-    if (int rc = linear_product(a->dx ? x_grad : w_grad, s)) return rc;
-    ++count;
-  }
+  LinearProduct x_grad = x_grad_product(a), w_grad = w_grad_product(a);
+  x_grad.A = dz, x_grad.lda = ldz, x_grad.B = w.dst ? w.dst : w.src, x_grad.ldb = w.ld_dst, x_grad.b_is_weight = !w.dst;
+  w_grad.A = dz, w_grad.lda = ldz, w_grad.B = x.dst ? x.dst : x.src, w_grad.ldb = x.ld_dst;
+  const LinearProduct* q[2] = {a->dx ? &x_grad : &w_grad, &w_grad};
+  if (a->dx || a->dweight)
+    if (int rc = linear_products(q, a->dx && a->dweight ? 2 : 1, ws.at, &count, s)) return rc;
   if (launches) *launches = count;
   return kOk;
 }

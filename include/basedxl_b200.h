@@ -170,8 +170,8 @@ int bxl_gemm_ragged_f16(const void* A, long long lda, const void* B, long long l
  * (written ones apart).  Operands of the tensor cores that the copy engine cannot read (rows not 16-byte aligned) are first
  * copied to the workspace.  dz is rounded to `dtype` between its two products; sums have a fixed order.
  * Written operands overlap nothing else of the call, except that y may be the residual.
- * bxl_linear_act_*_workspace_bytes reads all fields but the workspace.  The forward pass enqueues one kernel, and one
- * more where it has a workspace; *launches (or NULL): what the backward pass enqueued.
+ * bxl_linear_act_*_workspace_bytes reads all fields but the workspace.  *launches (or NULL): kernels
+ * enqueued.  Few tiles and a long sum are shared among CTAs by parts of it, joined in a fixed order by a second kernel.
  * The forward pass replaces bxl_gemm_f16 and the activation around it; no counterpart of the backward pass in the
  * reference, which only runs inference. */
 enum { BXL_ACT_NONE = 0, BXL_ACT_RELU = 1, BXL_ACT_SILU = 2, BXL_ACT_GELU = 3 /* erf */, BXL_ACT_GELU_TANH = 4, BXL_ACT_QUICK_GELU = 5 };
@@ -190,7 +190,7 @@ typedef struct bxl_linear_args {
   int M, N, K, dtype, act;
 } bxl_linear_args;
 long long bxl_linear_act_fwd_workspace_bytes(const bxl_linear_args* args);
-int bxl_linear_act_fwd(const bxl_linear_args* args, void* stream);
+int bxl_linear_act_fwd(const bxl_linear_args* args, int* launches, void* stream);
 long long bxl_linear_act_bwd_workspace_bytes(const bxl_linear_args* args);
 int bxl_linear_act_bwd(const bxl_linear_args* args, int* launches, void* stream);
 

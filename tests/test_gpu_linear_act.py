@@ -44,7 +44,7 @@ def _check_bwd(s, act, pre):
 
 SHAPES = [(1, 1, 1), (1, 320, 1280), (2, 320, 1280), (2, 1280, 640), (3, 7, 5), (4, 256, 33), (5, 1000, 130), (6, 65, 64), (7, 2048, 9), (8, 640, 1283), (9, 64, 64),
           (16, 8, 32), (33, 1, 7), (77, 2048, 1280), (128, 64, 256), (129, 65, 33), (200, 104, 1000), (257, 1003, 1501), (300, 1280, 640), (1024, 320, 1288),
-          (2050, 640, 328), (5000, 17, 19), (40, 5120, 8)]
+          (2050, 640, 328), (5000, 17, 19), (40, 5120, 8), (13000, 42, 33), (159, 34, 5832), (60, 3528, 24), (300, 4999, 40), (6000, 744, 16)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -201,7 +201,7 @@ def test_results_past_32_bit_offsets():
     _lib.device_status()
 
 
-@pytest.mark.parametrize("m,k,n", [(2, 320, 640), (300, 320, 640), (300, 321, 643)])
+@pytest.mark.parametrize("m,k,n", [(2, 320, 640), (300, 320, 640), (300, 321, 643), (2500, 48, 40), (70, 3001, 24)])
 def test_same_bits_every_time_and_from_graphs(m, k, n):
     """Two captured graphs, replayed in turn on a stream of their own with new inputs, give what eager calls give."""
     cuda_or_skip()
@@ -282,6 +282,8 @@ def test_counted_launches():
     assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, want_dbias=False)) == 1
     assert count(lambda: ops.linear_act_bwd(s["dy"], x, w, want_dbias=False, want_dx=False)) == 1
     assert count(lambda: ops.linear_act_bwd(s["dy"][:9], x[:9], w, pre[:9], "gelu")) == 2
+    long = _inputs(9000, 64, 96, torch.float16)                                   # and one that joins parts of the long sum
+    assert count(lambda: ops.linear_act_bwd(long["dy"], long["x"], long["weight"], want_dbias=False)) == 2
     big = _inputs(3000, 1280, 1280, torch.float16)                                # more tiles than SMs: two launches
     assert count(lambda: ops.linear_act_bwd(big["dy"], big["x"], big["weight"], want_dbias=False)) == 2
     n = torch.ones(64, device="cuda", dtype=torch.float16)

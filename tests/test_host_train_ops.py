@@ -168,7 +168,7 @@ BOTH = [{"x": None}, {"weight": None}, {"M": 0}, {"N": -1}, {"K": 0}, {"M": (1 <
 @pytest.mark.parametrize("kw", BOTH + [{"y": None}, {"ldy": 63}, {"pre": P, "ldp": 8}, {"ldx": 65, "workspace": None}, {"ldx": 65, "workspace_bytes": 64}])
 def test_c_linear_act_fwd_refuses(kw):
     l = _lib.load()
-    assert l.bxl_linear_act_fwd(_linear(**kw), None) < 0 and b"bxl_linear_act_fwd" in l.bxl_last_error()
+    assert l.bxl_linear_act_fwd(_linear(**kw), None, None) < 0 and b"bxl_linear_act_fwd" in l.bxl_last_error()
 
 
 @no_device
