@@ -364,13 +364,59 @@ __device__ __forceinline__ void add_bias(const uint32_t (&acc)[32], const BiasCh
     }
   }
 }
+// A chunk whose rows are not 16-byte aligned, through the transposing stage: a lane has a column, and eight rows of it (and of what
+// is added) are on their way at once.
 template <class T>
-__device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, uint32_t out, int lane) {
-  if (p.pre) store_tile_chunk<T>(&p.pre_map, f, row0, nb, out, lane);
+__device__ __forceinline__ void store_turned(const GemmParams& p, T* to, long long ld, const T* plus, long long ld_plus, const F2 (&f)[16], int row0, int nb, float* turn, int lane) {
+  __syncwarp();   // the previous chunk has been stored
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float2 u = split(f[j]);
+    turn[lane * 33 + 2 * j] = u.x, turn[lane * 33 + 2 * j + 1] = u.y;
+  }
+  __syncwarp();
+  const int col = nb + lane, rows = min(32, p.M - row0);
+  if (col >= p.N) return;
+  to += row0 * ld + col;
+  if (plus) plus += row0 * ld_plus + col;
+  const float* from = turn + lane;
+  // (a test in front of each row's store cost 85 cycles a row)
+  auto eight = [&](auto all, int n) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = from[i * 33];
+    if (plus) {
+      T w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i, plus += ld_plus) w[i] = decltype(all)::value || i < n ? *plus : from_f32<T>(0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += to_f32(w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i, to += ld)
+      if (decltype(all)::value || i < n) *to = from_f32<T>(v[i]);
+    from += 8 * 33;
+  };
+  int r = rows;
+#pragma unroll 1
+  for (; r >= 8; r -= 8) eight(std::true_type{}, 8);
+  if (r > 0) eight(std::false_type{}, r);
+}
+template <class T>
+__device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, uint32_t out, float* turn,
+                                                int lane) {
+  if (p.pre) {
+    if (p.ragged) store_turned<T>(p, static_cast<T*>(p.pre), p.ldp, nullptr, 0, f, row0, nb, turn, lane);
+    else store_tile_chunk<T>(&p.pre_map, f, row0, nb, out, lane);
+  }
   with_act(p.act, [&](auto act) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) f[j] = act_value<decltype(act)::value>(f[j]);
   });
+  if (p.ragged) {
+    store_turned<T>(p, static_cast<T*>(p.C), p.ldc, reinterpret_cast<const T*>(p.residual), p.ldr, f, row0, nb, turn, lane);
+    return;
+  }
   if (p.residual && out_row >= 0) {
     const T* rr = reinterpret_cast<const T*>(p.residual) + out_row * p.ldr + nb;
     if (res.valid) {
@@ -386,31 +432,6 @@ __device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16]
     }
   }
   store_tile_chunk<T>(&p.c_map, f, row0, nb, out, lane);
-}
-// The same through the transposing stage, for rows that are not 16-byte aligned.
-template <class T>
-__device__ __forceinline__ void store_chunk_act_ragged(const GemmParams& p, const F2 (&f)[16], int row0, int nb, float* turn, int lane) {
-  __syncwarp();   // the previous chunk has been stored
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const float2 u = split(f[j]);
-    turn[lane * 33 + 2 * j] = u.x, turn[lane * 33 + 2 * j + 1] = u.y;
-  }
-  __syncwarp();
-  const int col = nb + lane;
-  if (col >= p.N) return;
-  const int rows = min(32, p.M - row0);
-  with_act(p.act, [&](auto act) {
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      float v = turn[r * 33 + lane];
-      const long long m = row0 + r;
-      if (p.pre) static_cast<T*>(p.pre)[m * p.ldp + col] = from_f32<T>(v);
-      v = act_value<decltype(act)::value>(v);
-      if (p.residual) v += to_f32(reinterpret_cast<const T*>(p.residual)[m * p.ldr + col]);
-      static_cast<T*>(p.C)[m * p.ldc + col] = from_f32<T>(v);
-    }
-  });
 }
 
 // Accumulators of one tile.  The tensor core truncates its fp32 sums, by an amount that follows the sum's size and the
@@ -865,8 +886,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
           }
           F2 f[16];
           add_bias<LinT>(v, bias, f);
-          if (p.ragged) store_chunk_act_ragged<LinT>(p, f, row0, nb, s_turn + warp * kTurnFloats, lane);
-          else if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, f, out_row, row0, nb, res_cur, out_stage, lane);
+          if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, f, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
         }
       } else if constexpr (!kSplit) {
         // One chunk at a time per warp (measured: several accumulator loads in flight per warp do not
@@ -966,8 +986,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
             for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(f[j]);
             add_bias<LinT>(u, bias, g);
             const int row0 = tm * kBM + quarter * 32;
-            if (p.ragged) store_chunk_act_ragged<LinT>(p, g, row0, nb, s_turn + warp * kTurnFloats, lane);
-            else if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, g, out_row, row0, nb, res_cur, out_stage, lane);
+            if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, g, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
           } else if (!kConv && p.ragged)
             store_chunk_ragged(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
           else if (out_row >= 0 && nb < p.N)
