@@ -360,6 +360,8 @@ struct TeamRing {
   }
 };
 
+template <int VEC, int NV>
+__host__ __device__ constexpr bool fwd_params_shared() { return VEC == 8 && NV > 3; }
 // kSub: teams of a warp or less.
 template <class T, int VEC, int NV, bool kSub>
 __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_teams_kernel(const LnArgs a, const LnTeams t) {
@@ -375,14 +377,24 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
   pdl_wait();
   if (me.warp == 0)
     for (int i = 0; i < t.stages; ++i) ring.load(first + i * ring.step, i);
-  F w[NV][N], b[NV][N];
+  constexpr bool kShared = fwd_params_shared<VEC, NV>();
+  float* sw = reinterpret_cast<float*>(smem + t.off_w);
+  F w[kShared ? 1 : NV][N], b[kShared ? 1 : NV][N];
   {
     const Param<T> pw{a.weight, a.param_f32}, pb{a.bias, a.param_f32};
+    if constexpr (kShared) {
+      for (int c = threadIdx.x; c < a.C; c += kTeamThreads) {
+        const int at = shared_param_index<VEC>(n, c);
+        sw[at] = pw.p ? pw.at(c) : 1.f, sw[a.C + at] = pb.p ? pb.at(c) : 0.f;
+      }
+      __syncthreads();
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = min(me.lane + i * t.TL, n - 1);
-      pw.template get<VEC>((long long)v * VEC, 1.f, w[i]);
-      pb.template get<VEC>((long long)v * VEC, 0.f, b[i]);
+      for (int i = 0; i < NV; ++i) {
+        const int v = min(me.lane + i * t.TL, n - 1);
+        pw.template get<VEC>((long long)v * VEC, 1.f, w[i]);
+        pb.template get<VEC>((long long)v * VEC, 0.f, b[i]);
+      }
     }
   }
   bool failed = false;
@@ -433,8 +445,10 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
       for (int i = 0; i < NV; ++i) {
         const int v = me.lane + i * t.TL;
         if (has_vector<VEC, NV>(i, v, n)) {
+          if constexpr (kShared) shared_param<VEC>(sw, n, v, w[0]), shared_param<VEC>(sw + a.C, n, v, b[0]);
+          constexpr int k = kShared ? 0 : 1;
 #pragma unroll
-          for (int j = 0; j < N; ++j) x[i][j] = fma(mul(x[i][j], scale), w[i][j], b[i][j]);
+          for (int j = 0; j < N; ++j) x[i][j] = fma(mul(x[i][j], scale), w[k * i][j], b[k * i][j]);
           store_vec<T, VEC>(yr + v * VEC, narrow<T, VEC>(x[i]));
         }
       }
@@ -742,13 +756,14 @@ static long long ln_bwd_blocks(long long rows) {
 static bool back_to_back(const void* base, long long ld, int C) { return al16(base) && ld == C; }
 
 constexpr long long kSmemSm = 227 * 1024, kSmemHalf = kSmemSm / 2 - 1024;   // of an SM; a block's where two share one
-// Fills `t` for rows of `mats` matrices and threads of at most `most` vectors; false where rows of this size do not fit.
+// Fills `t` for rows of `mats` matrices and threads of at most `most` vectors (`most_sub` in teams of up to a warp); false where rows of this size do not fit.
 // `params`: bytes of shared memory for the parameters; `sums`: whether the block's column sums meet in the rings at the end;
 // `room`: shared memory of a block.  NV of the kernel: t.nv.
-static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats, int most, long long params, bool sums, long long room, int& nv, int& smem) {
+static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats, int most_sub, int most, long long params, bool sums, long long room, int& nv,
+                       int& smem) {
   const long long row = a.C * (long long)elem, n = a.C / vec;
   int TL = 8;
-  while (TL < kTeamThreads && n > (long long)most * TL) TL *= 2;
+  while (TL < kTeamThreads && n > (TL > 32 ? most : most_sub) * (long long)TL) TL *= 2;
   if (n > (long long)most * TL) return false;
   nv = (int)((n + TL - 1) / TL);
   if (vec == 1) nv = (nv + 3) / 4 * 4;
@@ -775,9 +790,12 @@ static int team_blocks(const LnTeams& t, int per_sm) {
   return (int)(need < most ? need : most);
 }
 
+// Vectors a thread holds in teams of up to a warp.
+template <int VEC>
+constexpr int fwd_most_sub() { return VEC == 1 ? 12 : VEC == 8 ? 7 : 6; }
 template <class T, int VEC, int NV, bool kSub = false>
 static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
-  if constexpr (!kSub)
+  if constexpr (!kSub && NV <= fwd_most_sub<VEC>())
     if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, true>(a, t, smem, s);
   if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kSub>>(kSmemSm)) return rc;
   return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV, kSub>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
@@ -787,10 +805,11 @@ static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
   LnTeams t = {};
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C);
-  const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 6, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
+  constexpr int sub = fwd_most_sub<VEC>(), most = VEC == 8 ? 8 : sub, wide = VEC == 1 ? 16 : 8;
+  const long long params = VEC == 8 ? 8ll * a.C : 0;
   done = (VEC > 1 || close) &&
-         (plan_teams(t, a, sizeof(T), VEC, 1, most, 0, false, kSmemSm, nv, smem) || plan_teams(t, a, sizeof(T), VEC, 1, wide, 0, false, kSmemSm, nv, smem));
-  if (done && nv * VEC <= 8) plan_teams(t, a, sizeof(T), VEC, 1, most, 0, false, kSmemHalf, nv, smem);   // two blocks an SM
+         (plan_teams(t, a, sizeof(T), VEC, 1, sub, most, params, false, kSmemSm, nv, smem) || plan_teams(t, a, sizeof(T), VEC, 1, sub, wide, params, false, kSmemSm, nv, smem));
+  if (done && nv * VEC <= 8) plan_teams(t, a, sizeof(T), VEC, 1, sub, most, params, false, kSmemHalf, nv, smem);   // two blocks an SM
   if (!done) return kOk;
   t.one_copy = close || t.rows == 1;
   if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_fwd: no device status word");
@@ -804,13 +823,10 @@ static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
     if (nv == 2) return ln_fwd_teams_launch<T, VEC, 2>(a, t, smem, s);
     if (nv == 3) return ln_fwd_teams_launch<T, VEC, 3>(a, t, smem, s);
     if (nv == 4) return ln_fwd_teams_launch<T, VEC, 4>(a, t, smem, s);
-    if constexpr (VEC == 4) {
-      if (nv == 5) return ln_fwd_teams_launch<T, VEC, 5>(a, t, smem, s);
-      if (nv == 6) return ln_fwd_teams_launch<T, VEC, 6>(a, t, smem, s);
-      if (nv == 7) return ln_fwd_teams_launch<T, VEC, 7>(a, t, smem, s);
-      return ln_fwd_teams_launch<T, VEC, 8>(a, t, smem, s);
-    }
-    return fail(kErrUnsupported, "bxl_layernorm_fwd: no kernel for %d vectors a thread", nv);
+    if (nv == 5) return ln_fwd_teams_launch<T, VEC, 5>(a, t, smem, s);
+    if (nv == 6) return ln_fwd_teams_launch<T, VEC, 6>(a, t, smem, s);
+    if (nv == 7) return ln_fwd_teams_launch<T, VEC, 7>(a, t, smem, s);
+    return ln_fwd_teams_launch<T, VEC, 8>(a, t, smem, s);
   }
 }
 
@@ -862,8 +878,8 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
   const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
   // Vectors a thread holds: 24 values of 16 bits or 16 of fp32 (8192 x 5120: 96 us with 24, 86 with 16); wider rows spill.
   const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 4, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
-  done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
-                                         plan_teams(t, a, sizeof(T), VEC, 2, wide, 4ll * a.C, true, kSmemSm, nv, smem));
+  done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
+                                         plan_teams(t, a, sizeof(T), VEC, 2, most, wide, 4ll * a.C, true, kSmemSm, nv, smem));
   if (!done) return kOk;
   t.one_copy = close || t.rows == 1;
   if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_bwd: no device status word");
