@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const LnArgs a) {
 // neighbours), and what lies behind the tensor's last boundary is copied by hand.
 struct LnTeams {
   int TL, rows, stages;     // threads of a team; rows and copies in flight of a ring
-  long long units;          // a.rows in steps of `rows`
+  uint32_t units;           // a.rows in steps of `rows`
   int one_copy;             // a unit's rows lie back to back
   int mat_bytes;            // a stage's room for one matrix
   unsigned long long ceiling;    // elements of x and dy before their last 16-byte boundary
@@ -182,12 +182,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 // Where a stage's first element lies in its room.
 template <class T, int VEC>
-__device__ __forceinline__ uint32_t stage_shift(long long row0, int C) {
-  return VEC == 1 ? (static_cast<uint32_t>(row0) * static_cast<uint32_t>(C)) & (16 / sizeof(T) - 1) : 0;
+__device__ __forceinline__ uint32_t stage_shift(uint32_t row0, int C) {
+  return VEC == 1 ? (row0 * static_cast<uint32_t>(C)) & (16 / sizeof(T) - 1) : 0;
 }
 // Called by all lanes of one warp: rows [row0, row0 + n) of the given matrices, each to its room of the stage.
 template <class T, int VEC, int MATS>
-__device__ __forceinline__ void load_stage(const T* const (&src)[MATS], const long long (&ld)[MATS], const LnArgs& a, const LnTeams& t, long long row0, int n,
+__device__ __forceinline__ void load_stage(const T* const (&src)[MATS], const long long (&ld)[MATS], const LnArgs& a, const LnTeams& t, uint32_t row0, int n,
                                            uint8_t* stage, uint32_t bar) {
   const int lane = threadIdx.x & 31;
   if constexpr (VEC == 1) {
@@ -317,26 +317,27 @@ __device__ __forceinline__ bool has_vector(int i, int v, int n) {
   return i < NV - (VEC == 1 ? 4 : 1) || v < n;
 }
 
-// The ring of a team: what its first warp fills and all of it waits on.
+// The ring of a team: what its first warp fills and all of it waits on.  Rows are counted in 32 bits (the products and comparisons
+// of 64 were a fifth of the instructions of narrow rows), and little is kept between units: registers bound the backward kernel.
 template <class T, int VEC, int MATS, bool kSub>
 struct TeamRing {
   const LnArgs& a;
   const LnTeams& t;
-  const T* src[MATS];
-  long long ld[MATS];
   uint8_t* base;
   uint32_t bars;
   volatile int* abort_flag;
-  long long step;           // units that the grid's teams take at a time
+  uint32_t row, step;       // the unit's first row; rows that the grid's teams take at a time
+  int left, last_n;         // units of this team still to come, this one included; rows of its last one
   int stage;
   uint32_t phase;
   __device__ __forceinline__ TeamRing(const LnArgs& a_, const LnTeams& t_, uint8_t* smem, const TeamRole& me) : a(a_), t(t_) {
-    src[0] = static_cast<const T*>(a.x), ld[0] = a.ldx;
-    if constexpr (MATS == 2) src[1] = static_cast<const T*>(a.dy), ld[1] = a.lddy;
+    const uint32_t first = blockIdx.x * me.teams + me.team, units = gridDim.x * me.teams, rows = kSub ? t.rows : 1;
+    row = first * rows, step = units * rows;
+    left = first < t.units ? static_cast<int>((t.units - 1 - first) / units + 1) : 0;
+    last_n = kSub && left && first + (left - 1) * units == t.units - 1 ? static_cast<int>(static_cast<uint32_t>(a.rows) - (t.units - 1) * rows) : rows;
     base = smem + me.team * t.stages * MATS * t.mat_bytes;
     bars = smem_u32(smem + t.off_bar) + 8 * me.team * t.stages;
     abort_flag = reinterpret_cast<volatile int*>(smem + t.off_bar + 8 * t.stages * me.teams);
-    step = gridDim.x * (long long)me.teams;
     stage = 0, phase = 0;
     if (me.warp == 0 && (threadIdx.x & 31) == 0)
       for (int i = 0; i < t.stages; ++i) mbar_init(bars + 8 * i, 1);
@@ -344,20 +345,30 @@ struct TeamRing {
     if ((threadIdx.x & 31) == 0) mbar_fence_init();
     __syncthreads();
   }
-  __device__ __forceinline__ void load(long long unit, int st) {
-    if (unit >= t.units) return;
-    const long long row0 = kSub ? unit * t.rows : unit;
-    load_stage<T, VEC, MATS>(src, ld, a, t, row0, kSub ? (int)min((long long)t.rows, a.rows - row0) : 1, base + st * MATS * t.mat_bytes, bars + 8 * st);
+  // called by the team's first warp: the unit `ahead` behind the present one
+  __device__ __forceinline__ void load(int ahead, int st) {
+    if (ahead >= left) return;
+    const T* src[MATS];
+    long long ld[MATS];
+    src[0] = static_cast<const T*>(a.x), ld[0] = a.ldx;
+    if constexpr (MATS == 2) src[1] = static_cast<const T*>(a.dy), ld[1] = a.lddy;
+    load_stage<T, VEC, MATS>(src, ld, a, t, row + ahead * step, ahead == left - 1 ? last_n : kSub ? t.rows : 1, base + st * MATS * t.mat_bytes, bars + 8 * st);
+  }
+  __device__ __forceinline__ void fill() {
+    for (int i = 0; i < t.stages; ++i) load(i, i);
   }
   __device__ __forceinline__ bool wait(int site) { return mbar_wait_warp(bars + 8 * stage, phase, abort_flag, t.dev_status, site); }
-  __device__ __forceinline__ const T* mat(int m, long long row0) const {
-    return reinterpret_cast<const T*>(base + (stage * MATS + m) * t.mat_bytes) + stage_shift<T, VEC>(row0, a.C);
+  __device__ __forceinline__ const T* mat(int m) const {
+    return reinterpret_cast<const T*>(base + (stage * MATS + m) * t.mat_bytes) + stage_shift<T, VEC>(row, a.C);
   }
+  // whether row `sub` of the unit `ahead` behind the present one exists
+  __device__ __forceinline__ bool has(int ahead, int sub) const { return ahead < left - 1 || (ahead == left - 1 && sub < last_n); }
   // after the team has read the stage: called by its first warp
-  __device__ __forceinline__ void refill(long long unit) { load(unit + t.stages * step, stage); }
-  __device__ __forceinline__ void next() {
+  __device__ __forceinline__ void refill() { load(t.stages, stage); }
+  __device__ __forceinline__ void next_stage() {
     if (++stage == t.stages) stage = 0, phase ^= 1u;
   }
+  __device__ __forceinline__ void next_unit() { row += step, --left; }
 };
 
 template <int VEC, int NV>
@@ -373,10 +384,8 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
   TeamRing<T, VEC, 1, kSub> ring(a, t, smem, me);
   float* slots = reinterpret_cast<float*>(smem + t.off_red);
   const int n = a.C / VEC;
-  const long long first = blockIdx.x * (long long)me.teams + me.team;
   pdl_wait();
-  if (me.warp == 0)
-    for (int i = 0; i < t.stages; ++i) ring.load(first + i * ring.step, i);
+  if (me.warp == 0) ring.fill();
   constexpr bool kShared = fwd_params_shared<VEC, NV>();
   float* sw = reinterpret_cast<float*>(smem + t.off_w);
   F w[kShared ? 1 : NV][N], b[kShared ? 1 : NV][N];
@@ -398,12 +407,12 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
     }
   }
   bool failed = false;
-  for (long long unit = first; unit < t.units; unit += ring.step) {
-    const long long row0 = kSub ? unit * t.rows : unit, row = row0 + (kSub ? me.sub : 0);
-    const bool in = !kSub || row < a.rows;
+  for (; ring.left > 0; ring.next_unit()) {
+    const uint32_t row = ring.row + (kSub ? me.sub : 0);
+    const bool in = !kSub || ring.has(0, me.sub);
     failed = !ring.wait(700);
     if (kSub && failed) break;
-    const T* xs = ring.mat(0, row0) + (kSub ? me.sub * a.C : 0);
+    const T* xs = ring.mat(0) + (kSub ? me.sub * a.C : 0);
     F x[NV][N];
     F s[2] = {splat<F>(0.f), splat<F>(0.f)};   // two chains of additions
 #pragma unroll
@@ -420,8 +429,8 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
     if (failed) break;
     // the stage has been read by the whole team
     __syncwarp();
-    if (me.warp == 0) ring.refill(unit);
-    ring.next();
+    if (me.warp == 0) ring.refill();
+    ring.next_stage();
     const float mean = mean_of(sum[0], a);
     const F minus = splat<F>(-mean);
     s[0] = s[1] = splat<F>(0.f);
@@ -470,10 +479,8 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
   float* slots = reinterpret_cast<float*>(smem + t.off_red);
   float* sw = reinterpret_cast<float*>(smem + t.off_w);
   const int n = a.C / VEC;
-  const long long first = blockIdx.x * (long long)me.teams + me.team;
   pdl_wait();
-  if (me.warp == 0)
-    for (int i = 0; i < t.stages; ++i) ring.load(first + i * ring.step, i);
+  if (me.warp == 0) ring.fill();
   {
     const Param<T> w{a.weight, a.param_f32};
     for (int c = threadIdx.x; c < a.C; c += kTeamThreads) sw[shared_param_index<VEC>(n, c)] = w.p ? w.at(c) : 1.f;
@@ -484,23 +491,22 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
 #pragma unroll
     for (int j = 0; j < N; ++j) dw[i][j] = db[i][j] = splat<F>(0.f);
   float mean_next = 0.f, rstd_next = 0.f;
-  auto moments = [&](long long row) {
-    if (row < a.rows) mean_next = a.mean[row], rstd_next = a.rstd[row];
+  auto moments = [&](int ahead) {
+    const uint32_t r = ring.row + ahead * ring.step + me.sub;
+    if (ring.has(ahead, me.sub)) mean_next = a.mean[r], rstd_next = a.rstd[r];
   };
-  moments(kSub ? first * t.rows + me.sub : first);
+  moments(0);
   __syncthreads();
   bool failed = false;
-  int turn = 0;
-  for (long long unit = first; unit < t.units; unit += ring.step, turn ^= 1) {
-    const long long row0 = kSub ? unit * t.rows : unit, row = row0 + (kSub ? me.sub : 0);
-    const bool in = !kSub || row < a.rows;
+  for (; ring.left > 0; ring.next_unit()) {
+    const bool in = !kSub || ring.has(0, me.sub);
     failed = !ring.wait(701);
     if (kSub && failed) break;
-    const T* xs = ring.mat(0, row0) + (kSub ? me.sub * a.C : 0);
-    const T* ds = ring.mat(1, row0) + (kSub ? me.sub * a.C : 0);
+    const T* xs = ring.mat(0) + (kSub ? me.sub * a.C : 0);
+    const T* ds = ring.mat(1) + (kSub ? me.sub * a.C : 0);
     Vec<T, VEC> rx[NV], rd[NV];          // as loaded, and widened twice: registers bound this kernel
     const float mean = mean_next, rstd = rstd_next;
-    moments(kSub ? (unit + ring.step) * t.rows + me.sub : unit + ring.step);
+    moments(1);
     F s1 = splat<F>(0.f), s2 = s1;       // sum(g), sum(g (x - mean))
     const F minus = splat<F>(-mean);
 #pragma unroll
@@ -520,14 +526,14 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
       }
     }
     float sum[2] = {total(s1), total(s2)};
-    failed = team_sum<2, kSub>(sum, t, me, slots, turn, failed);
+    failed = team_sum<2, kSub>(sum, t, me, slots, ring.left & 1, failed);
     if (failed) break;
     __syncwarp();
-    if (me.warp == 0) ring.refill(unit);   // the stage has been read by the whole team
-    ring.next();
+    if (me.warp == 0) ring.refill();   // the stage has been read by the whole team
+    ring.next_stage();
     const F r = splat<F>(rstd), c1 = splat<F>(-rstd * (sum[0] * a.inv_c)), c2 = splat<F>(-rstd * (rstd * (sum[1] * a.inv_c)));
     if (in) {
-      T* out = static_cast<T*>(a.y) + row * a.ldy;
+      T* out = static_cast<T*>(a.y) + (ring.row + (kSub ? me.sub : 0)) * a.ldy;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = me.lane + i * t.TL;
@@ -569,8 +575,8 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
           }
         }
   }
-  float* out = a.part + blockIdx.x * 2ll * a.C;
-  float* to = me.teams > 1 ? reinterpret_cast<float*>(smem) + me.team * 2 * a.C : out;
+  float* sums = a.part + blockIdx.x * 2ll * a.C;
+  float* to = me.teams > 1 ? reinterpret_cast<float*>(smem) + me.team * 2 * a.C : sums;
   if (me.sub == 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
     float s = 0.f;
 #pragma unroll 4
     for (int k = 0; k < me.teams; ++k) s += reinterpret_cast<const float*>(smem)[k * 2 * a.C + c];
-    out[c] = s;
+    sums[c] = s;
   }
 }
 
@@ -762,6 +768,7 @@ constexpr long long kSmemSm = 227 * 1024, kSmemHalf = kSmemSm / 2 - 1024;   // o
 static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats, int most_sub, int most, long long params, bool sums, long long room, int& nv,
                        int& smem) {
   const long long row = a.C * (long long)elem, n = a.C / vec;
+  if (a.rows > INT_MAX) return false;
   int TL = 8;
   while (TL < kTeamThreads && n > (TL > 32 ? most : most_sub) * (long long)TL) TL *= 2;
   if (n > (long long)most * TL) return false;
@@ -769,7 +776,7 @@ static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats,
   if (vec == 1) nv = (nv + 3) / 4 * 4;
   const int warps = TL > 32 ? TL / 32 : 1, teams = kTeamWarps / warps;
   t.ceiling = (unsigned long long)a.rows * a.C / (16 / elem) * (16 / elem);
-  t.TL = TL, t.rows = TL < 32 ? 32 / TL : 1, t.units = (a.rows + t.rows - 1) / t.rows;
+  t.TL = TL, t.rows = TL < 32 ? 32 / TL : 1, t.units = (uint32_t)((a.rows + t.rows - 1) / t.rows);
   t.mat_bytes = (int)((t.rows * row + 15) / 16 * 16 + (vec == 1 ? 32 : 0));   // a widened span begins and ends up to 15 bytes further out
   const long long slots = 2ll * kTeamWarps * mats * 4, rest = params + slots + teams * 8 * 8 + 512;
   const long long scratch = sums && teams > 1 ? teams * 2ll * a.C * 4 : 0;
@@ -786,7 +793,7 @@ static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats,
   return smem <= room;
 }
 static int team_blocks(const LnTeams& t, int per_sm) {
-  const long long teams = kTeamWarps / (t.TL > 32 ? t.TL / 32 : 1), need = (t.units + teams - 1) / teams, most = (long long)sm_count() * per_sm;
+  const long long teams = kTeamWarps / (t.TL > 32 ? t.TL / 32 : 1), need = ((long long)t.units + teams - 1) / teams, most = (long long)sm_count() * per_sm;
   return (int)(need < most ? need : most);
 }
 
