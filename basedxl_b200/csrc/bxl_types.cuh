@@ -22,7 +22,7 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// VEC elements that are loaded and stored at once (16 bytes, or one element).
+// VEC elements that are loaded and stored at once (16 or 8 bytes, or one element).
 template <class T, int VEC>
 struct alignas(sizeof(T) * VEC) Vec {
   T v[VEC];
@@ -31,12 +31,14 @@ template <class T, int VEC>
 __device__ __forceinline__ Vec<T, VEC> load_vec(const T* p) {
   Vec<T, VEC> r;
   if constexpr (sizeof(r) == 16) *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
+  else if constexpr (sizeof(r) == 8) *reinterpret_cast<uint2*>(&r) = *reinterpret_cast<const uint2*>(p);
   else r.v[0] = *p;
   return r;
 }
 template <class T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, VEC>& r) {
   if constexpr (sizeof(r) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
+  else if constexpr (sizeof(r) == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&r);
   else *p = r.v[0];
 }
 
@@ -118,6 +120,9 @@ template <class T, int VEC>
 __device__ __forceinline__ void widen(const Vec<T, VEC>& u, typename Lanes<VEC>::F (&out)[Lanes<VEC>::N]) {
   if constexpr (VEC == 1) {
     out[0] = to_f32(u.v[0]);
+  } else if constexpr (sizeof(u) == 8) {
+    const uint2 q = *reinterpret_cast<const uint2*>(&u);
+    out[0] = widen2<T>(q.x), out[1] = widen2<T>(q.y);
   } else {
     const uint4 q = *reinterpret_cast<const uint4*>(&u);
     if constexpr (sizeof(T) == 4) {
@@ -132,6 +137,8 @@ __device__ __forceinline__ Vec<T, VEC> narrow(const typename Lanes<VEC>::F (&in)
   Vec<T, VEC> r;
   if constexpr (VEC == 1) {
     r.v[0] = from_f32<T>(in[0]);
+  } else if constexpr (sizeof(r) == 8) {
+    *reinterpret_cast<uint2*>(&r) = make_uint2(narrow2<T>(in[0]), narrow2<T>(in[1]));
   } else {
     uint4 q;
     if constexpr (sizeof(T) == 4) {

@@ -897,6 +897,11 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
     if (nv <= 12) return ln_bwd_teams_launch<T, 1, 12>(a, t, blocks, smem, s);
     return ln_bwd_teams_launch<T, 1, 16>(a, t, blocks, smem, s);
   } else {
+    if constexpr (VEC == 8) {
+      const int half = (a.C / 4 + t.TL - 1) / t.TL;
+      if (half == 3) return ln_bwd_teams_launch<T, 4, 3>(a, t, blocks, smem, s);
+      if (half == 5) return ln_bwd_teams_launch<T, 4, 5>(a, t, blocks, smem, s);
+    }
     if (nv == 1) return ln_bwd_teams_launch<T, VEC, 1>(a, t, blocks, smem, s);
     if (nv == 2) return ln_bwd_teams_launch<T, VEC, 2>(a, t, blocks, smem, s);
     if (nv == 3) return ln_bwd_teams_launch<T, VEC, 3>(a, t, blocks, smem, s);

@@ -64,6 +64,37 @@ def test_fp32_weights(rows, c, dtype):
     _check(*_inputs(rows, c, dtype, torch.float32))
 
 
+MANY = [(8009, 136), (4001, 320), (2101, 512), (1701, 648), (1501, 768), (1201, 1152), (1101, 1280), (801, 1608), (601, 2048), (601, 2560), (601, 4096),
+        (600, 5120), (530, 8192), (520, 12000), (517, 16000), (513, 20000), (1701, 643), (601, 2049), (530, 8190)]
+
+
+@pytest.mark.parametrize("dtype,param", [(torch.float16, torch.float16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)], ids=str)
+@pytest.mark.parametrize("rows,c", MANY)
+def test_many_rows(rows, c, dtype, param):
+    """Every width of a team and number of vectors of a thread, with a last unit that is not full."""
+    cuda_or_skip()
+    _check(*_inputs(rows, c, dtype, param))
+
+
+@pytest.mark.parametrize("rows,c", [(4001, 320), (2101, 512), (801, 1608), (601, 4096), (1701, 643)])
+def test_many_rows_apart(rows, c):
+    """Rows of a wider tensor, between values that are not to be read.  Rows of whole 16-byte vectors give the same bits as a copy of them;
+    others are summed in another order where they do not lie back to back, and are held to the bounds that cover any order."""
+    cuda_or_skip()
+    _, ops = _ops()
+    x, w, b, dy = _inputs(rows, c, torch.bfloat16)
+    wide = torch.full((rows, 2 * c + 8), float("nan"), device="cuda", dtype=x.dtype)
+    apart = wide[:, 8 : 8 + c]
+    apart.copy_(x)
+    _check(apart, w, b, dy)
+    if c % 8 == 0:
+        want = ops.layernorm_fwd(x, w, b, EPS, want_stats=True)
+        got = ops.layernorm_fwd(apart, w, b, EPS, want_stats=True)
+        want += ops.layernorm_bwd(dy, x, *want[1:], w)
+        got += ops.layernorm_bwd(dy, apart, *got[1:], w)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 @pytest.mark.parametrize("c", [5, 640, 2048, 17000])
 def test_absent_weight_or_bias(c):
     cuda_or_skip()
