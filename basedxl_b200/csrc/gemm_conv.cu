@@ -402,18 +402,18 @@ __device__ __forceinline__ void store_turned(const GemmParams& p, T* to, long lo
   for (; r >= 8; r -= 8) eight(std::true_type{}, 8);
   if (r > 0) eight(std::false_type{}, r);
 }
-template <class T>
+template <class T, bool kTurn>
 __device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, uint32_t out, float* turn,
                                                 int lane) {
   if (p.pre) {
-    if (p.ragged) store_turned<T>(p, static_cast<T*>(p.pre), p.ldp, nullptr, 0, f, row0, nb, turn, lane);
+    if (kTurn && p.ragged) store_turned<T>(p, static_cast<T*>(p.pre), p.ldp, nullptr, 0, f, row0, nb, turn, lane);
     else store_tile_chunk<T>(&p.pre_map, f, row0, nb, out, lane);
   }
   with_act(p.act, [&](auto act) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) f[j] = act_value<decltype(act)::value>(f[j]);
   });
-  if (p.ragged) {
+  if (kTurn && p.ragged) {
     store_turned<T>(p, static_cast<T*>(p.C), p.ldc, reinterpret_cast<const T*>(p.residual), p.ldr, f, row0, nb, turn, lane);
     return;
   }
@@ -443,7 +443,8 @@ __host__ __device__ inline int acc_sets(int parts, int bn) { return parts == 1 ?
 // kSplit: the K loop is split over the CTAs of a cluster (p.split of them); a separate
 // instantiation, so that each variant carries only its own epilogue (and its registers).
 // kTwo: operands in two fp16 parts (p.parts == 2); likewise separate.
-// kLin: linear layers with an activation, of fp16 (1) or bf16 (2) operands; 0 everywhere else.
+// kLin: linear layers with an activation, of fp16 (1, 3) or bf16 (2, 4) operands; 0 everywhere else.  3 and 4 can also store rows that
+// are not 16-byte aligned; that code costs the others registers (8192 x 64 x 8192: 40.5 us without, 45.0 with).
 // Two products that do not depend on one another can share a launch (GemmTwo): the first `first` CTAs work on one, the others on
 // the other, each as if its share were the grid.
 struct GemmTwo {
@@ -468,9 +469,11 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
   static_assert(!(kPair && kSplit), "a CTA pair walks the whole K range");
   static_assert(!(kConv && kTwo), "convolutions have fp16 operands");
   static_assert(!kLin || !(kConv || kTwo), "an epilogue of plain products");
+  static_assert(kLin < 3 || !(kPair || kSplit), "rows of any alignment: one CTA a tile");
   constexpr int kSub = epi_sub(kLin), kSubThreads = kSub * 128;                       // epilogue warps of a quarter of the tile
   constexpr int kWarpA = 4 * kSub, kWarpMma = kWarpA + 1, kWarpB = kWarpA + 2;         // after the epilogue warps: A loads, MMA, B loads
-  using LinT = std::conditional_t<kLin == 2, __nv_bfloat16, __half>;
+  using LinT = std::conditional_t<kLin == 2 || kLin == 4, __nv_bfloat16, __half>;
+  constexpr bool kTurn = kLin > 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
       // odd CTA of a pair: the leader issues the MMAs for both
     } else if (elect_one()) {
       const bool a_mn = kLin && p.a_mn;
-      const uint32_t idesc = make_idesc_f16(kBM * kWidth, BN, a_mn ? 1 : 0, (!kConv && p.b_kn) ? 1 : 0) | (kLin == 2 ? kIdescBf16 : 0u);
+      const uint32_t idesc = make_idesc_f16(kBM * kWidth, BN, a_mn ? 1 : 0, (!kConv && p.b_kn) ? 1 : 0) | (std::is_same_v<LinT, __nv_bfloat16> ? kIdescBf16 : 0u);
       const uint32_t a_step = a_mn ? 128u : 2u;   // kUmmaK further along K, in 16-byte units: 16 rows of 128 bytes, or 32 bytes of a row
       int stage = 0;
       uint32_t phase = 0;
@@ -886,7 +889,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
           }
           F2 f[16];
           add_bias<LinT>(v, bias, f);
-          if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, f, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
+          if (row0 < p.M && nb < p.N) store_chunk_act<LinT, kTurn>(p, f, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
         }
       } else if constexpr (!kSplit) {
         // One chunk at a time per warp (measured: several accumulator loads in flight per warp do not
@@ -986,7 +989,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
             for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(f[j]);
             add_bias<LinT>(u, bias, g);
             const int row0 = tm * kBM + quarter * 32;
-            if (row0 < p.M && nb < p.N) store_chunk_act<LinT>(p, g, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
+            if (row0 < p.M && nb < p.N) store_chunk_act<LinT, kTurn>(p, g, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
           } else if (!kConv && p.ragged)
             store_chunk_ragged(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
           else if (out_row >= 0 && nb < p.N)
@@ -1364,7 +1367,8 @@ static int linear_extra(const LinearProduct& q) { return linear_ragged(q) ? ragg
 static bool linear_heavy(const LinearProduct& q) { return linear_ragged(q) || q.residual || q.pre; }
 static int tiles_along(int n, int of) { return (int)(((long long)n + of - 1) / of); }
 static TileConfig linear_tiles(const LinearProduct& q) {
-  return choose_tiles(tiles_along(q.M, kBM), q.N, tiles_along(q.K, kBK), q.b_kn != 0, g_force_bn, g_force_split, g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, linear_extra(q), 1,
+  const bool one = linear_ragged(q);   // no variant with pairs or splits
+  return choose_tiles(tiles_along(q.M, kBM), q.N, tiles_along(q.K, kBK), q.b_kn != 0, g_force_bn, one ? 1 : g_force_split, one ? 0 : g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, linear_extra(q), 1,
                       linear_heavy(q));
 }
 static int linear_params(const LinearProduct& q, const TileConfig& tc, GemmParams& p) {
@@ -1564,7 +1568,11 @@ int linear_products(const LinearProduct* const* q, int n, void* workspace, int* 
       if (int rc = sliced_params(*q[i], plan.single[i], part[i], two.p[i], smem[i])) return rc;
     two.first = (unsigned)(plan.single[0].tiles * plan.single[0].slices);
     const int ctas = (int)two.first + plan.single[1].tiles * plan.single[1].slices, most = smem[0] > smem[1] ? smem[0] : smem[1];
-    if (int rc = bf16 ? launch_two<2>(two, ctas, most, stream) : launch_two<1>(two, ctas, most, stream)) return rc;
+    const bool turn = two.p[0].ragged || two.p[1].ragged;
+    int rc;
+    if (turn) rc = bf16 ? launch_two<4>(two, ctas, most, stream) : launch_two<3>(two, ctas, most, stream);
+    else rc = bf16 ? launch_two<2>(two, ctas, most, stream) : launch_two<1>(two, ctas, most, stream);
+    if (rc) return rc;
     ++*launches;
   } else {
     for (int i = 0; i < n; ++i) {
@@ -1577,7 +1585,8 @@ int linear_products(const LinearProduct* const* q, int n, void* workspace, int* 
       } else {
         if ((rc = linear_params(*q[i], plan.tc[i], p))) return rc;
         const int tiles_m = tiles_along(q[i]->M, kBM), tiles_n = tiles_along(q[i]->N, plan.tc[i].bn);
-        rc = bf16 ? launch<false, false, 2>(p, tiles_m, tiles_n, stream) : launch<false, false, 1>(p, tiles_m, tiles_n, stream);
+        if (p.ragged) rc = bf16 ? launch_one<false, false, false, false, 4>(p, tiles_m * tiles_n, stream) : launch_one<false, false, false, false, 3>(p, tiles_m * tiles_n, stream);
+        else rc = bf16 ? launch<false, false, 2>(p, tiles_m, tiles_n, stream) : launch<false, false, 1>(p, tiles_m, tiles_n, stream);
       }
       if (rc) return rc;
       ++*launches;
