@@ -127,7 +127,7 @@ struct alignas(64) GemmParams {
   int slices;
   float* part;
   long long part_ld;
-  CUtensorMap c_map, pre_map;  // C and pre, for stores of 32 x 32 values (aligned rows)
+  CUtensorMap c_map, pre_map, res_map;  // C, pre and residual, for copies of 32 x 32 values (aligned rows)
 };
 
 // Split-K exchange buffer of one CTA: for each of the (split-1) peers, the fp32
@@ -309,6 +309,19 @@ __device__ __forceinline__ void store_chunk_ragged(const GemmParams& p, const fl
 // at a time, and took 1.8 us of a 256-column tile's 6.9 (8192 x 1280 x 5120 with the pre-activation kept: 93 us of 77 without).
 // A buffer of 2 KB per warp; rows and columns past the matrix are clipped.
 constexpr int kOutBytes = 32 * 32 * 2;
+// The residual comes the same way, a chunk ahead, into a buffer of its own per warp (8192 x 320 x 2560: 39.3 us with lanes that load
+// their rows, 28.4 so).
+struct ResidualRing {
+  uint32_t buf, bar, phase;
+  __device__ __forceinline__ void ask(const GemmParams& p, int row0, int nb, int lane) const {
+    if (row0 >= p.M || nb >= p.N) return;
+    __syncwarp();   // the chunk before has been read
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bar, kOutBytes);
+      tma_load_2d(buf, &p.res_map, bar, nb, row0);
+    }
+  }
+};
 template <class T>
 __device__ __forceinline__ void store_tile_chunk(const CUtensorMap* map, const F2 (&f)[16], int row0, int nb, uint32_t buf, int lane) {
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the copy before has read the buffer
@@ -402,9 +415,11 @@ __device__ __forceinline__ void store_turned(const GemmParams& p, T* to, long lo
   for (; r >= 8; r -= 8) eight(std::true_type{}, 8);
   if (r > 0) eight(std::false_type{}, r);
 }
-template <class T, bool kTurn>
-__device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, uint32_t out, float* turn,
-                                                int lane) {
+// `ring`: where the residual arrives if it comes by the copy engine (`res`: with a split K; two products in one launch have none).
+// False if it did not come.
+template <class T, bool kTurn, bool kRing, bool kSplit>
+__device__ __forceinline__ bool store_chunk_act(const GemmParams& p, F2 (&f)[16], long long out_row, int row0, int nb, const ResidualChunk& res, ResidualRing& ring, uint32_t out,
+                                                float* turn, volatile int* abort_flag, int lane) {
   if (p.pre) {
     if (kTurn && p.ragged) store_turned<T>(p, static_cast<T*>(p.pre), p.ldp, nullptr, 0, f, row0, nb, turn, lane);
     else store_tile_chunk<T>(&p.pre_map, f, row0, nb, out, lane);
@@ -415,9 +430,21 @@ __device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16]
   });
   if (kTurn && p.ragged) {
     store_turned<T>(p, static_cast<T*>(p.C), p.ldc, reinterpret_cast<const T*>(p.residual), p.ldr, f, row0, nb, turn, lane);
-    return;
+    return true;
   }
-  if (p.residual && out_row >= 0) {
+  if constexpr (kRing) {
+    if (p.residual) {
+      if (!mbar_wait_warp(ring.bar, ring.phase, abort_flag, p.dev_status, 303)) return false;
+      ring.phase ^= 1u;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint4 u;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(ring.buf + lane * 64u + ((q ^ ((lane >> 1) & 3)) << 4)));
+        f[4 * q] = add(f[4 * q], widen2<T>(u.x)), f[4 * q + 1] = add(f[4 * q + 1], widen2<T>(u.y));
+        f[4 * q + 2] = add(f[4 * q + 2], widen2<T>(u.z)), f[4 * q + 3] = add(f[4 * q + 3], widen2<T>(u.w));
+      }
+    }
+  } else if (kSplit && p.residual && out_row >= 0) {
     const T* rr = reinterpret_cast<const T*>(p.residual) + out_row * p.ldr + nb;
     if (res.valid) {
 #pragma unroll
@@ -432,6 +459,7 @@ __device__ __forceinline__ void store_chunk_act(const GemmParams& p, F2 (&f)[16]
     }
   }
   store_tile_chunk<T>(&p.c_map, f, row0, nb, out, lane);
+  return true;
 }
 
 // Accumulators of one tile.  The tensor core truncates its fp32 sums, by an amount that follows the sum's size and the
@@ -473,7 +501,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
   constexpr int kSub = epi_sub(kLin), kSubThreads = kSub * 128;                       // epilogue warps of a quarter of the tile
   constexpr int kWarpA = 4 * kSub, kWarpMma = kWarpA + 1, kWarpB = kWarpA + 2;         // after the epilogue warps: A loads, MMA, B loads
   using LinT = std::conditional_t<kLin == 2 || kLin == 4, __nv_bfloat16, __half>;
-  constexpr bool kTurn = kLin > 2;
+  constexpr bool kTurn = kLin > 2, kRing = kLin != 0 && !kSplit && !kTurn && std::is_same_v<Products, GemmParams>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -510,6 +538,8 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
   const uint32_t crank = (S > 1 || kPair) ? cluster_ctarank() : 0u;
 
   if (threadIdx.x == 0) {
+    if (kRing)
+      for (int w = 0; w < kWarpA; ++w) mbar_init(smem_u32(s_bias) + 8u * w, 1);
     for (int s = 0; s < p.stages; ++s) {
       // one arrival (with its byte count) from each of this CTA's two producer threads
       mbar_init(full_bar(s), 2);
@@ -785,6 +815,8 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
     const int chunks = BN / 32;
     const int cps = chunks / S;    // 32-column chunks per owner slice
     [[maybe_unused]] const uint32_t out_stage = smem_u32(s_turn) + warp * kOutBytes;
+    [[maybe_unused]] ResidualRing ring{out_stage + kWarpA * kOutBytes, smem_u32(s_bias) + 8u * warp, 0u};   // (the bias row has no other use here)
+    const bool by_ring = kRing && p.residual && p.slices == 1;
     int it = 0;
     for (int index = first_tile; index < num_tiles; index += tile_step, ++it) {
       int tile = index;
@@ -848,7 +880,9 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
       // the chunk before it (of this warp) is converted and stored.
       ResidualChunk res_cur, res_next;
       res_cur.valid = res_next.valid = false;
-      if (!kSplit) {
+      if constexpr (kRing) {
+        if (by_ring && half < chunks) ring.ask(p, tm * kBM + quarter * 32, n0 + half * 32, lane);
+      } else if (kLin == 0 && !kSplit) {
         // the residual of the first chunk travels while the MMAs of this tile still run
         if (half < chunks) load_residual(p, out_row, n0 + half * 32, res_cur);
       }
@@ -869,15 +903,13 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
         }
       };
       if constexpr (kLin != 0 && !kSplit) {
+        bool came = true;
 #pragma unroll 1
         for (int c = half; c < chunks; c += kSub) {
           const int nb = n0 + c * 32, row0 = tm * kBM + quarter * 32;
           uint32_t v[32];
           tmem_ld_32x32(t_row + c * 32, v);
-          if (c != half) {
-            load_bias<LinT>(p, nb, bias);
-            load_residual(p, out_row, nb, res_cur);
-          }
+          if (c != half) load_bias<LinT>(p, nb, bias);
           tmem_ld_wait();
           if (p.slices > 1) {
             if (out_row >= 0 && nb < p.N) {   // whole chunks: the partial sums' rows are padded to them
@@ -889,8 +921,11 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
           }
           F2 f[16];
           add_bias<LinT>(v, bias, f);
-          if (row0 < p.M && nb < p.N) store_chunk_act<LinT, kTurn>(p, f, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
+          if (row0 < p.M && nb < p.N && !(came = store_chunk_act<LinT, kTurn, kRing, kSplit>(p, f, out_row, row0, nb, res_cur, ring, out_stage, s_turn + warp * kTurnFloats, abort_flag, lane)))
+            break;
+          if (by_ring && c + kSub < chunks) ring.ask(p, row0, nb + kSub * 32, lane);
         }
+        if (!came) break;
       } else if constexpr (!kSplit) {
         // One chunk at a time per warp (measured: several accumulator loads in flight per warp do not
         // shorten the epilogue; a second warp on the same scheduler does).
@@ -989,7 +1024,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
             for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(f[j]);
             add_bias<LinT>(u, bias, g);
             const int row0 = tm * kBM + quarter * 32;
-            if (row0 < p.M && nb < p.N) store_chunk_act<LinT, kTurn>(p, g, out_row, row0, nb, res_cur, out_stage, s_turn + warp * kTurnFloats, lane);
+            if (row0 < p.M && nb < p.N) store_chunk_act<LinT, kTurn, kRing, kSplit>(p, g, out_row, row0, nb, res_cur, ring, out_stage, s_turn + warp * kTurnFloats, abort_flag, lane);
           } else if (!kConv && p.ragged)
             store_chunk_ragged(p, f, tm * kBM + quarter * 32, nb, has_bias ? s_bias + c * 32 : nullptr, s_turn + warp * kTurnFloats, lane);
           else if (out_row >= 0 && nb < p.N)
@@ -1050,7 +1085,8 @@ struct TileConfig {
 constexpr int kSmemLnExtra = 1024;           // the weight column-sum row of a GEMM with a folded LayerNorm
 constexpr int ragged_bytes(int lin) { return 4 * epi_sub(lin) * kTurnFloats * 4; }   // the epilogue warps' transposing stages
 
-constexpr int kSmemOutExtra = 4 * kEpiSubLin * kOutBytes;          // ... or their output buffers (linear layers)
+// ... or their buffers of output and residual (linear layers)
+constexpr int out_bytes(bool residual) { return 4 * kEpiSubLin * kOutBytes * (residual ? 2 : 1); }
 
 static int stages_for(int bn, int split, int pair = 0, int extra_smem = 0, int parts = 1) {
   const int stage = parts * (kABytes + (pair ? bn * 64 : bn * 128));
@@ -1142,7 +1178,7 @@ template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin>
 static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   const int b_rows = kPair ? p.bn / 2 : p.bn;
   const int smem = p.stages * p.parts * (kABytes + b_rows * 128) + recv_bytes(p.bn, kSplit ? p.split : 1) + kSmemMisc +
-                   (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? ragged_bytes(kLin) : kLin ? kSmemOutExtra : 0);
+                   (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? ragged_bytes(kLin) : kLin ? out_bytes(p.residual) : 0);
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1363,7 +1399,7 @@ static bool linear_ragged(const LinearProduct& q) {
   auto rows16 = [](const void* base, long long ld) { return aligned16(base) && ld % 8 == 0; };
   return q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && !rows16(q.residual, q.ldr)) || (q.pre && !rows16(q.pre, q.ldp));
 }
-static int linear_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : kSmemOutExtra; }
+static int linear_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(q.residual); }
 static bool linear_heavy(const LinearProduct& q) { return linear_ragged(q) || q.residual || q.pre; }
 static int tiles_along(int n, int of) { return (int)(((long long)n + of - 1) / of); }
 static TileConfig linear_tiles(const LinearProduct& q) {
@@ -1397,11 +1433,13 @@ static int linear_params(const LinearProduct& q, const TileConfig& tc, GemmParam
   p.bias_vec = aligned16(q.bias);
   if (!ragged) {
     uint64_t dims[2] = {(uint64_t)q.N, (uint64_t)q.M};
-    uint64_t str[1] = {(uint64_t)q.ldc * 2}, pre_str[1] = {(uint64_t)q.ldp * 2};
+    uint64_t str[1] = {(uint64_t)q.ldc * 2}, pre_str[1] = {(uint64_t)q.ldp * 2}, res_str[1] = {(uint64_t)q.ldr * 2};
     uint32_t box[2] = {32, 32};
     if (int rc = encode_tmap_f16(&p.c_map, q.C, 2, dims, str, box, 64)) return rc;
     if (q.pre)
       if (int rc = encode_tmap_f16(&p.pre_map, q.pre, 2, dims, pre_str, box, 64)) return rc;
+    if (q.residual)
+      if (int rc = encode_tmap_f16(&p.res_map, q.residual, 2, dims, res_str, box, 64)) return rc;
   }
   p.C = q.C, p.ldc = q.ldc, p.pre = q.pre, p.ldp = q.ldp, p.act = q.act, p.ragged = ragged ? 1 : 0, p.slices = 1;
   p.dev_status = st;
@@ -1524,7 +1562,7 @@ static const LinearPlan& plan_products(const LinearProduct* const* q, int n) {
   memset(&key, 0, sizeof(key));
   unsigned hash = 0;
   for (int i = 0; i < n; ++i) {
-    const int v[5] = {q[i]->M, q[i]->N, q[i]->K, q[i]->b_kn, (linear_ragged(*q[i]) ? 2 : 0) + (linear_heavy(*q[i]) ? 1 : 0)};
+    const int v[5] = {q[i]->M, q[i]->N, q[i]->K, q[i]->b_kn, (linear_ragged(*q[i]) ? 2 : 0) + (linear_heavy(*q[i]) ? 1 : 0) + (q[i]->residual ? 4 : 0)};
     for (int j = 0; j < 5; ++j) key.v[i][j] = v[j], hash = hash * 31u + (unsigned)v[j];
   }
   key.n = n, key.sms = sm_count(), key.bn = g_force_bn, key.split = g_force_split, key.pair = g_force_pair;
