@@ -248,6 +248,9 @@ static int dz_shares(int M, int N, int vec) {
   return shares < 1 ? 1 : shares > 4096 ? 4096 : (int)shares;
 }
 
+// The partial sums of dbias: room for the vector form, which has more shares than the other.
+static long long dbias_part_bytes(const bxl_linear_args* a) { return a->dbias && a->M > kDzFew ? 4ll * dz_shares(a->M, a->N, 8) * a->N : 0; }
+
 static int check_linear(const char* who, const bxl_linear_args* a) {
   if (!a) return fail(kErrInvalidArg, "%s: null argument block", who);
   if (a->M <= 0 || a->N <= 0 || a->K <= 0) return fail(kErrInvalidArg, "%s: non-positive extent M=%d N=%d K=%d", who, a->M, a->N, a->K);
@@ -308,7 +311,7 @@ static bool stores_dz(const bxl_linear_args* a) {
 static long long bwd_workspace(const bxl_linear_args* a) {
   long long n = 0;
   if (stores_dz(a)) n += round256(2ll * a->M * round8(a->N));
-  if (a->dbias && a->M > kDzFew) n += round256(4ll * dz_shares(a->M, a->N, 1) * a->N);
+  n += round256(dbias_part_bytes(a));
   if (a->dx) n += round256(copy_bytes(a->weight, a->ldw, a->N, a->K));
   if (a->dweight) n += round256(copy_bytes(a->x, a->ldx, a->M, a->K));
   const LinearProduct x = x_grad_product(a), w = w_grad_product(a);
@@ -378,7 +381,7 @@ extern "C" int bxl_linear_act_bwd(const bxl_linear_args* a, int* launches, void*
     const bool vec = !few && a->N % 8 == 0 && al(a->dy, 16) && a->lddy % 8 == 0 && (a->act == BXL_ACT_NONE || (al(a->pre, 16) && a->ldp % 8 == 0));
     const int shares = dz_shares(a->M, a->N, vec ? 8 : 1), cols = vec ? 256 : 32;
     if (a->dbias && few) p.dbias = a->dbias;
-    else if (a->dbias) p.part = static_cast<float*>(ws.take(4ll * dz_shares(a->M, a->N, 1) * a->N));
+    else if (a->dbias) p.part = static_cast<float*>(ws.take(dbias_part_bytes(a)));
     const dim3 grid((a->N + cols - 1) / cols, shares);
     auto launch = [&](auto kernel, int warps) { return launch_kernel("dz_kernel launch", kernel, grid, dim3(32 * warps), 0, s, 1, p); };
     int rc;
