@@ -489,6 +489,9 @@ __device__ __forceinline__ GridShare share_of(const GemmTwo& q) {
   return blockIdx.x >= q.first ? GridShare{static_cast<int>(blockIdx.x - q.first), static_cast<int>(gridDim.x - q.first)}
                                : GridShare{static_cast<int>(blockIdx.x), static_cast<int>(q.first)};
 }
+// Columns of B that a stage holds: an MN-major B comes in boxes of 64, of which a tile of another width leaves part of the last one unused
+// (its neighbour's, or zeros past the matrix).
+__host__ __device__ inline int staged_cols(int cols, int b_kn) { return b_kn ? (cols + 63) / 64 * 64 : cols; }
 template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin = 0, class Products = GemmParams>
 __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const __grid_constant__ Products products) {
   const GemmParams& p = product_of(products);
@@ -509,7 +512,8 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
   const int S = kSplit ? p.split : 1;
   const int b_rows = kPair ? BN / 2 : BN;       // rows of the B tile this CTA stages
   constexpr int parts = kTwo ? 2 : 1;
-  const int b_bytes = b_rows * 128;
+  const int b_cols = kLin ? staged_cols(b_rows, p.b_kn) : b_rows;
+  const int b_bytes = b_cols * 128;
   const int stage_bytes = parts * (kABytes + b_bytes);   // every part of A, then every part of B
   constexpr int kWidth = kPair ? 2 : 1;          // CTAs that cooperate on one tile (besides a K split)
   const uint32_t recv_base = smem_base + p.stages * stage_bytes;            // 1024-aligned (stage_bytes % 1024 == 0)
@@ -703,7 +707,7 @@ __global__ void __launch_bounds__(gemm_threads(kLin), 1) gemm_conv_kernel(const 
               if (p.b_kn) {
                 // B[K,N]: one 64(n) x 64(k) box per 64 output columns
                 for (int s = 0; s < parts; ++s)
-                  for (int j = 0; j < b_rows / 64; ++j) load_2d(b_dst + s * b_bytes + j * 8192, &p.b_map[s], n0 + j * 64, k0);
+                  for (int j = 0; j < b_cols / 64; ++j) load_2d(b_dst + s * b_bytes + j * 8192, &p.b_map[s], n0 + j * 64, k0);
               } else {
                 load_2d(b_dst, &p.b_map[0], k0, n0);
               }
@@ -1088,9 +1092,10 @@ constexpr int ragged_bytes(int lin) { return 4 * epi_sub(lin) * kTurnFloats * 4;
 // ... or their buffers of output and residual (linear layers)
 constexpr int out_bytes(bool residual) { return 4 * kEpiSubLin * kOutBytes * (residual ? 2 : 1); }
 
-static int stages_for(int bn, int split, int pair = 0, int extra_smem = 0, int parts = 1) {
-  const int stage = parts * (kABytes + (pair ? bn * 64 : bn * 128));
-  int st = (kSmemBudget - kSmemMisc - extra_smem - recv_bytes(bn, split)) / stage;
+// `staged`: columns of B in a stage, of a pair in its two; `bn` where that differs
+static int stages_for(int staged, int split, int pair = 0, int extra_smem = 0, int parts = 1, int bn = 0) {
+  const int stage = parts * (kABytes + (pair ? staged * 64 : staged * 128));
+  int st = (kSmemBudget - kSmemMisc - extra_smem - recv_bytes(bn ? bn : staged, split)) / stage;
   if (st > kMaxStages) st = kMaxStages;
   return st;
 }
@@ -1112,7 +1117,8 @@ static std::atomic<int> g_clusters[64][5] = {};
 // than the best configuration in the mean (convolutions 0.7 %, fp32 products 1.0 %, linear layers 3.0 %), half of
 // them have the best, and the worst, 36 %, are products of two to four rows.
 static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int force_bn = 0, int force_split = 0,
-                               int force_pair = -1, double a_min_us = 0.0, int extra_smem = 0, int parts = 1, bool heavy = false) {
+                               int force_pair = -1, double a_min_us = 0.0, int extra_smem = 0, int parts = 1, bool heavy = false,
+                               bool any_width = false) {
   const int sms = sm_count();
   TileConfig best{128, 1, stages_for(128, 1, 0, extra_smem, parts), 0, sms, 0.0};
   int at_once[5] = {0, sms, 0, 0, 0};
@@ -1121,7 +1127,8 @@ static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int fo
   for (int pair = 0; pair <= 1; ++pair) {
     if (force_pair >= 0 && pair != force_pair) continue;
     for (int bn = 32; bn <= 256; bn += 32) {
-      if (b_kn && (pair ? bn % 128 : bn % 64)) continue;  // MN-major B is loaded in 64-column boxes
+      if (b_kn && !any_width && (pair ? bn % 128 : bn % 64)) continue;  // MN-major B is loaded in 64-column boxes
+      const int staged = pair ? 2 * staged_cols(bn / 2, b_kn) : staged_cols(bn, b_kn);
       if (force_bn && bn != force_bn) continue;
       if (2 * acc_sets(parts, bn) * bn > 512) continue;   // tensor memory
       const int units_m = pair ? (tiles_m + 1) / 2 : tiles_m;
@@ -1129,13 +1136,13 @@ static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int fo
       for (int split = 1; split <= (pair ? 1 : 4); split *= 2) {
         if (force_split && split != force_split) continue;
         if ((bn / 32) % split || split > num_kb) continue;
-        const int st = stages_for(bn, split, pair, extra_smem, parts);
+        const int st = stages_for(staged, split, pair, extra_smem, parts, bn);
         if (st < 3) continue;
         const int width = pair ? 2 : split;
         const int clusters = at_once[width];
         const int par = tiles < clusters ? tiles : clusters;
         const int rounds = (tiles + par - 1) / par;
-        const double bytes = 16384.0 + bn * (pair ? 64.0 : 128.0);
+        const double bytes = 16384.0 + staged * (pair ? 64.0 : 128.0);
         const double kb_us = fmax(fmax((2 * parts - 1) * bn / 256.0 * 0.256, parts * (pair ? 0.117 + 0.000643 * bn : bytes / 139000.0)), a_min_us);
         const double kb_unit = (num_kb + split - 1) / split;
         // accumulator read-out (and the exchange of a K split)
@@ -1176,7 +1183,7 @@ static int launch_two(const GemmTwo& two, int ctas, int smem, cudaStream_t strea
 
 template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin>
 static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
-  const int b_rows = kPair ? p.bn / 2 : p.bn;
+  const int b_rows = kLin ? staged_cols(kPair ? p.bn / 2 : p.bn, p.b_kn) : kPair ? p.bn / 2 : p.bn;
   const int smem = p.stages * p.parts * (kABytes + b_rows * 128) + recv_bytes(p.bn, kSplit ? p.split : 1) + kSmemMisc +
                    (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? ragged_bytes(kLin) : kLin ? out_bytes(p.residual) : 0);
   static bool configured[64] = {};
@@ -1405,7 +1412,7 @@ static int tiles_along(int n, int of) { return (int)(((long long)n + of - 1) / o
 static TileConfig linear_tiles(const LinearProduct& q) {
   const bool one = linear_ragged(q);   // no variant with pairs or splits
   return choose_tiles(tiles_along(q.M, kBM), q.N, tiles_along(q.K, kBK), q.b_kn != 0, g_force_bn, one ? 1 : g_force_split, one ? 0 : g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, linear_extra(q), 1,
-                      linear_heavy(q));
+                      linear_heavy(q), true);
 }
 static int linear_params(const LinearProduct& q, const TileConfig& tc, GemmParams& p) {
   int* st = device_status_ptr();

@@ -86,6 +86,23 @@ def test_every_tiling(m, k, n, tiles):
     _lib.device_status()
 
 
+@pytest.mark.parametrize("tiles", [(32, 1, 0), (96, 1, 0), (160, 1, 0), (224, 1, 0), (96, 1, 1), (192, 1, 1), (224, 1, 1), (192, 2, 0), (0, 0, -1)], ids=str)
+@pytest.mark.parametrize("m,k,n", [(300, 456, 520), (8000, 96, 648)])
+def test_any_width(m, k, n, tiles):
+    """Tiles that are no multiple of the 64 columns that an operand is fetched in, one and many of them for each CTA."""
+    cuda_or_skip()
+    _lib, _ = _ops()
+    l = _lib.lib()
+    s = _inputs(m, k, n, torch.bfloat16)
+    _lib.check(l.bxl_debug_force_tiles(*tiles), l, kernels=0)
+    try:
+        pre = _check_fwd(s, "silu")
+        _check_bwd(s, "silu", pre)
+        _lib.device_status()
+    finally:
+        _lib.check(l.bxl_debug_force_tiles(0, 0, -1), l, kernels=0)
+
+
 @pytest.mark.parametrize("m", [3, 140])
 @pytest.mark.parametrize("layout", ["slice", "odd slice", "one row", "columns first", "three axes", "one axis"])
 def test_layouts(layout, m):
