@@ -51,8 +51,11 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
 // row g of x, and hands them over as the k = 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of two products; both operands permute K alike.
 // Bound by the loads in flight: eight rows of 2560 x 10240 (52 MB) 11.6 us, 4.5 TB/s; 1280 x 5120 5.8, 320 x 1280 2.2.  With fused
 // multiply-adds instead the widening of x bounds it: 31.6, 8.9 and 3.0 us (one row of 2560 x 10240 10.5).
+// Any other rows are loaded value by value, lane 4 g + q the values q, q + 4 .. q + 28, which is bound by the number of loads: 8 x 2051 x
+// 8193 20.9 us, 4 x 1748 x 4672 12.3 (54.7 and 16.3 with a lane per value of K and fused multiply-adds; rows turned in shared memory 21.8
+// and 10.3, but the small calls slower).
 constexpr int kFewMaxWarps = 8;
-template <class T>
+template <class T, bool kVec>
 __global__ void __launch_bounds__(kFewMaxWarps * 32) few_rows_kernel(const FewRows p) {
   pdl_launch_dependents();
   __shared__ float part[kFewMaxWarps][kFewRows * kFewColumns];
@@ -67,29 +70,47 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32) few_rows_kernel(const FewRo
     mma_16x8x16<T>(d, a.x, b.x, a.y, b.y, c.x, c.y);
     mma_16x8x16<T>(d, a.z, b.z, a.w, b.w, c.z, c.w);
   };
+  // this lane's eight values of a row's i-th 32; behind K there are zeros
+  struct Narrow {
+    unsigned short v[8];
+  };
+  using Loaded = std::conditional_t<kVec, uint4, Narrow>;
+  auto eight = [&](const T* row, int i, auto all) {
+    if constexpr (kVec) {
+      const int k = i * 32 + q * 8;
+      return decltype(all)::value || k < p.K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
+    } else {
+      Narrow u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = i * 32 + 4 * j + q;
+        u.v[j] = 0;
+        if (decltype(all)::value || k < p.K) asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(u.v[j]) : "l"(row + k));   // volatile: all of them before the first use
+      }
+      return u;
+    }
+  };
+  auto words = [](const Loaded& u) {
+    if constexpr (kVec) return u;
+    else return make_uint4(u.v[0] | u.v[1] << 16, u.v[2] | u.v[3] << 16, u.v[4] | u.v[5] << 16, u.v[6] | u.v[7] << 16);
+  };
+  auto take = [&](int i, auto all) {
+    const Loaded a = eight(w0, i, all), b = eight(w1, i, all), c = eight(x, i, all);
+    step(words(a), words(b), words(c));
+  };
+  constexpr int kAhead = kVec ? 4 : 2;   // twelve loads on their way at once, or 48 narrow ones
   const int whole = p.K / 32, share = (whole + warps - 1) / warps, last = min(whole, (warp + 1) * share);
   int i = warp * share;
-  for (; i + 4 <= last; i += 4) {   // twelve loads on their way at once
-    uint4 a[4], b[4], c[4];
+  for (; i + kAhead <= last; i += kAhead) {
+    Loaded a[kAhead], b[kAhead], c[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = (i + j) * 32 + q * 8;
-      a[j] = *reinterpret_cast<const uint4*>(w0 + k), b[j] = *reinterpret_cast<const uint4*>(w1 + k), c[j] = *reinterpret_cast<const uint4*>(x + k);
-    }
+    for (int j = 0; j < kAhead; ++j) a[j] = eight(w0, i + j, std::true_type{}), b[j] = eight(w1, i + j, std::true_type{}), c[j] = eight(x, i + j, std::true_type{});
 #pragma unroll
-    for (int j = 0; j < 4; ++j) step(a[j], b[j], c[j]);
+    for (int j = 0; j < kAhead; ++j) step(words(a[j]), words(b[j]), words(c[j]));
   }
 #pragma unroll 3
-  for (; i < last; ++i) {
-    const int k = i * 32 + q * 8;
-    step(*reinterpret_cast<const uint4*>(w0 + k), *reinterpret_cast<const uint4*>(w1 + k), *reinterpret_cast<const uint4*>(x + k));
-  }
-  if (warp == warps - 1 && p.K % 32) {   // the lanes past K add nothing
-    const int k = whole * 32 + q * 8;
-    const uint4 none = make_uint4(0, 0, 0, 0);
-    const bool in = k < p.K;
-    step(in ? *reinterpret_cast<const uint4*>(w0 + k) : none, in ? *reinterpret_cast<const uint4*>(w1 + k) : none, in ? *reinterpret_cast<const uint4*>(x + k) : none);
-  }
+  for (; i < last; ++i) take(i, std::true_type{});
+  if (warp == warps - 1 && p.K % 32) take(whole, std::false_type{});
   part[warp][2 * q * 16 + g] = d[0], part[warp][(2 * q + 1) * 16 + g] = d[1];
   part[warp][2 * q * 16 + g + 8] = d[2], part[warp][(2 * q + 1) * 16 + g + 8] = d[3];
   __syncthreads();
@@ -99,54 +120,12 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32) few_rows_kernel(const FewRo
     few_rows_result<T>(p, v, i / 16, n0 + i % 16);
   }
 }
-// Any other rows: a lane per value of K, NB columns a warp.
-template <class T, int MB>
-__global__ void __launch_bounds__(256) few_rows_any_kernel(const FewRows p) {
-  pdl_launch_dependents();
-  constexpr int NB = 2, kWarps = 8;   // 16 columns a block
-  const int lane = threadIdx.x & 31, n0 = blockIdx.x * kFewColumns + (threadIdx.x >> 5) * NB;
-  static_assert(NB * kWarps == kFewColumns, "a block's columns");
-  const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w);
-  float acc[MB][NB];
-#pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = 0.f;
-  pdl_wait();
-#pragma unroll 4
-  for (int k = lane; k < p.K; k += 32) {
-    float wv[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) wv[j] = to_f32(w[min(n0 + j, p.N - 1) * p.ldw + k]);
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const float xv = to_f32(x[min(i, p.M - 1) * p.ldx + k]);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) acc[i][j] = fmaf(xv, wv[j], acc[i][j]);
-    }
-  }
-  float mine = 0.f;
-#pragma unroll
-  for (int i = 0; i < MB; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      float s = acc[i][j];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == i * NB + j) mine = s;
-    }
-  if (lane < MB * NB) few_rows_result<T>(p, mine, lane / NB, n0 + lane % NB);
-}
-
 template <class T>
 static int few_rows(const FewRows& p, bool vec, cudaStream_t s) {
   const dim3 grid((p.N + kFewColumns - 1) / kFewColumns);
-  if (vec) {
-    const int steps = (p.K + 31) / 32, warps = steps < kFewMaxWarps ? steps : kFewMaxWarps;
-    return launch_kernel("few_rows_kernel launch", few_rows_kernel<T>, grid, dim3(32 * warps), 0, s, 1, p);
-  }
-  auto any = [&](auto kernel) { return launch_kernel("few_rows_any_kernel launch", kernel, grid, dim3(256), 0, s, 1, p); };
-  return p.M == 1 ? any(few_rows_any_kernel<T, 1>) : p.M == 2 ? any(few_rows_any_kernel<T, 2>) : p.M <= 4 ? any(few_rows_any_kernel<T, 4>) : any(few_rows_any_kernel<T, 8>);
+  const int steps = (p.K + 31) / 32, warps = steps < kFewMaxWarps ? steps : kFewMaxWarps;
+  return vec ? launch_kernel("few_rows_kernel launch", few_rows_kernel<T, true>, grid, dim3(32 * warps), 0, s, 1, p)
+             : launch_kernel("few_rows_kernel launch", few_rows_kernel<T, false>, grid, dim3(32 * warps), 0, s, 1, p);
 }
 
 // ---- backward: dz and its column sums ----------------------------------------------------------
