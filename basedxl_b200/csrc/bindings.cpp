@@ -85,6 +85,20 @@ void same_device(const char* who, std::initializer_list<const Tensor*> others, c
   for (const Tensor* t : others) TORCH_CHECK_VALUE(!t || t->device() == x.device(), who, ": expected all tensors on ", text(x.device()), ", got ", text(t->device()));
 }
 
+// `out` is written while other rows of the inputs are still being read: it may be one of them from end to end where that is said, and
+// otherwise shares no memory with them.
+void apart(const char* who, const Tensor& out, const char* what, const Tensor* other, bool may_be_it) {
+  if (!other || !out.numel() || !other->numel()) return;
+  auto behind = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.const_data_ptr()) + (last + 1) * t.element_size();
+  };
+  const char *a = static_cast<const char*>(out.const_data_ptr()), *b = static_cast<const char*>(other->const_data_ptr());
+  if (a >= behind(*other) || b >= behind(out)) return;
+  TORCH_CHECK_VALUE(may_be_it && a == b && other->is_contiguous(), who, ": out overlaps ", what);
+}
+
 // The library, set up for the current device (through _lib.lib(), once per device).
 void ensure_device(int dev) {
   static bool ready[64] = {};
@@ -154,6 +168,7 @@ PyObject* layernorm_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (into) {
     same(who, "out", *into.t, x.sizes(), type);
     TORCH_CHECK_VALUE(into->is_contiguous(), who, ": out must be contiguous");
+    apart(who, *into.t, "x", &x, true), apart(who, *into.t, "weight", w.t, false), apart(who, *into.t, "bias", b.t, false);
   }
   same_device(who, {w.t, b.t, into.t}, x);
   const int64_t c = x.size(-1), rows = x.numel() / c;
@@ -243,6 +258,7 @@ PyObject* linear_act(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (into) {
     same(who, "out", *into.t, sizes, type);
     TORCH_CHECK_VALUE(into->is_contiguous(), who, ": out must be contiguous");
+    apart(who, *into.t, "x", &x, false), apart(who, *into.t, "weight", &w, false), apart(who, *into.t, "bias", b.t, false), apart(who, *into.t, "residual", res.t, true);
   }
   same_device(who, {&w, b.t, res.t, into.t}, x);
   Tensor y = into ? *into.t : empty(sizes, type, x.device()), pre;

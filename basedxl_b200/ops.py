@@ -264,8 +264,9 @@ def _activation(name, activation) -> int:
 
 def linear_act(x, weight, bias=None, activation=None, residual=None, out=None, want_pre: bool = False):
     """``act(x[..., K] @ weight[N, K]^T + bias) + residual`` in one product, fp16 or bf16, any extents; ``activation`` is one of
-    ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``) receives the result.  ``want_pre`` also returns the value
-    before the activation, rounded to the type of ``x``: the input of :func:`linear_act_bwd`."""
+    ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``, and overlaps no other input) receives the result.
+    ``want_pre`` also returns the value before the activation, rounded to the type of ``x``: the input of
+    :func:`linear_act_bwd`."""
     return _lib.native().linear_act(x, weight, bias, _activation("linear_act", activation), residual, out, bool(want_pre))
 
 

@@ -95,6 +95,15 @@ def test_many_rows_apart(rows, c):
         assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("rows,c", [(40, 1285), (4001, 320), (801, 1608), (601, 4096), (1701, 643), (513, 20000)])
+def test_in_place(rows, c):
+    cuda_or_skip()
+    _, ops = _ops()
+    x, w, b, _ = _inputs(rows, c, torch.float16, torch.float32)
+    want = ops.layernorm_fwd(x, w, b, EPS)
+    assert ops.layernorm_fwd(x, w, b, EPS, out=x) is not want and torch.equal(x, want)
+
+
 @pytest.mark.parametrize("c", [5, 640, 2048, 17000])
 def test_absent_weight_or_bias(c):
     cuda_or_skip()

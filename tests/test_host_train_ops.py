@@ -93,6 +93,25 @@ def test_linear_act_refuses(kw):
     assert HOST not in _refused(ops.linear_act, **{**good, **kw})
 
 
+def test_results_over_inputs_are_refused():
+    """Other rows of an input are still read while a result is written; in place is where a row depends on itself alone."""
+    buf = _z(48)
+    x, shifted = buf[:40].view(5, 8), buf[8:].view(5, 8)
+    assert "out overlaps x" in _refused(ops.layernorm_fwd, x=x, out=shifted)
+    wide = _z(5, 16)
+    assert "out overlaps x" in _refused(ops.layernorm_fwd, x=wide[:, :8], out=wide.view(-1)[:40].view(5, 8))
+    assert "out overlaps weight" in _refused(ops.layernorm_fwd, x=_z(5, 8), weight=buf[:8], out=x)
+    assert "out overlaps bias" in _refused(ops.layernorm_fwd, x=_z(5, 8), bias=buf[32:40], out=x)
+    assert HOST in _refused(ops.layernorm_fwd, x=x, out=x)
+    assert HOST in _refused(ops.layernorm_fwd, x=x, weight=buf[40:], out=x)
+    w = _z(8, 8)
+    assert "out overlaps x" in _refused(ops.linear_act, x=x, weight=w, out=x)
+    assert "out overlaps weight" in _refused(ops.linear_act, x=_z(8, 8), weight=w, out=w)
+    assert "out overlaps bias" in _refused(ops.linear_act, x=_z(5, 8), weight=w, bias=buf[:8], out=x)
+    assert "out overlaps residual" in _refused(ops.linear_act, x=_z(5, 8), weight=w, residual=x, out=shifted)
+    assert HOST in _refused(ops.linear_act, x=_z(5, 8), weight=w, residual=x, out=x)
+
+
 @pytest.mark.parametrize(
     "kw",
     [
