@@ -720,9 +720,12 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* part, i
     for (int i = warp; i < count; i += warps) v += part[i * pitch + blockIdx.y * (long long)C + c];
   s[warp][lane] = v;
   __syncthreads();
-  if (warp) return;
-  for (int i = 1; i < warps; ++i) v += s[i][lane];
-  if (c < C) out[c] = from_f32<P>(v);
+  for (int k = warp; k < 32; k += warps) {
+    float sum[1] = {lane < warps ? s[lane][k] : 0.f};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) add_lanes<1>(sum, o);
+    if (lane == 0 && blockIdx.x * 32 + k < C) out[blockIdx.x * 32 + k] = from_f32<P>(sum[0]);
+  }
 }
 
 int sum_partials(const float* part, int count, long long pitch, int C, void* out0, void* out1, int dtype, cudaStream_t s) {
