@@ -6,6 +6,8 @@ flushed between launches) and print one JSON line with its achieved rate.
     python -m basedxl_b200.kernel_bench attention --B 2 --heads 10 --Lq 4096 --Lslot 4096 --slots 1
     python -m basedxl_b200.kernel_bench groupnorm --B 2 --C 1280 --H 32 --W 32          # two-launch form
     python -m basedxl_b200.kernel_bench groupnorm_fused --B 2 --C 1280 --H 32 --W 32    # one-launch form
+    python -m basedxl_b200.kernel_bench layernorm_bwd --M 32768 --C 640                 # with the weight's and bias's gradients
+    python -m basedxl_b200.kernel_bench linear_act --M 8192 --K 1280 --N 5120 --act gelu # bias, activation, pre-activation kept
 
 The same command line is what the profiler captures are taken on (few launches,
 small device footprint).
@@ -42,11 +44,13 @@ def _time(fn, iters: int, warmup: int, flush: bool = True) -> float:
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "conv", "attention", "groupnorm", "groupnorm_fused", "geglu", "layernorm"])
+    ap.add_argument("kernel", choices=["gemm", "conv", "attention", "groupnorm", "groupnorm_fused", "geglu", "layernorm", "layernorm_fwd", "layernorm_bwd",
+                                       "linear_act", "linear_act_bwd"])
     for n, d in [("M", 2048), ("K", 1280), ("N", 1280), ("B", 2), ("Cin", 640), ("Cout", 640), ("C", 1280), ("H", 64), ("W", 64),
                  ("heads", 10), ("Lq", 4096), ("Lslot", 4096), ("slots", 1), ("stride", 1), ("iters", 10), ("warmup", 3),
                  ("bn", 0), ("split", 0), ("pair", -1)]:
         ap.add_argument(f"--{n}", type=int, default=d)
+    ap.add_argument("--act", default="silu", choices=sorted(k for k in ops.ACTIVATIONS if k))
     ap.add_argument("--no-flush", action="store_true")
     a = ap.parse_args()
     dev = torch.device("cuda:0")
@@ -96,10 +100,23 @@ def main():
         h = rn(a.M, 2 * a.N)
         fn = lambda: ops.geglu(h)
         work, unit, desc = 3.0 * a.M * a.N * 2, "GB/s", {"rows": a.M, "F": a.N}
-    else:
+    elif a.kernel == "layernorm":
         x, gamma, beta = rn(a.M, a.C), rn(a.C), rn(a.C)
         fn = lambda: ops.layernorm(x, gamma, beta, 1e-5)
         work, unit, desc = 2.0 * a.M * a.C * 2, "GB/s", {"rows": a.M, "C": a.C}
+    elif a.kernel in ("layernorm_fwd", "layernorm_bwd"):
+        x, dy, w = rn(a.M, a.C), rn(a.M, a.C), rn(a.C)
+        _, mean, rstd = ops.layernorm_fwd(x, w, w, want_stats=True)
+        forward = a.kernel == "layernorm_fwd"
+        fn = (lambda: ops.layernorm_fwd(x, w, w)) if forward else (lambda: ops.layernorm_bwd(dy, x, mean, rstd, w))
+        work, unit, desc = 2.0 * a.M * a.C * (2 if forward else 3), "GB/s", {"rows": a.M, "C": a.C}
+    else:
+        x, w, b, dy = rn(a.M, a.K), rn(a.N, a.K) * a.K**-0.5, rn(a.N), rn(a.M, a.N)
+        forward = lambda: ops.linear_act(x, w, b, activation=a.act, want_pre=True)
+        pre = forward()[1]
+        fn = forward if a.kernel == "linear_act" else lambda: ops.linear_act_bwd(dy, x, w, pre, activation=a.act)
+        work, unit = (2.0 if a.kernel == "linear_act" else 4.0) * a.M * a.N * a.K, "TFLOP/s"
+        desc = {"M": a.M, "N": a.N, "K": a.K, "act": a.act}
     us = _time(fn, a.iters, a.warmup, flush=not a.no_flush)
     _lib.device_status()
     rate = work / us / (1e6 if unit == "TFLOP/s" else 1e3)
