@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(const LnArgs a) {
 // aligned address on: the span is then widened to 16-byte boundaries (what it touches beside the row belongs to its
 // neighbours), and what lies behind the tensor's last boundary is copied by hand.
 struct LnTeams {
-  int TL, rows, stages;     // threads of a team; rows and copies in flight of a ring
+  int TL, stages;           // threads of a team; copies in flight of a ring
+  int per, groups, rows;    // rows that a warp has at a time; how often in a unit; the unit's rows
   uint32_t units;           // a.rows in steps of `rows`
   int one_copy;             // a unit's rows lie back to back
   int mat_bytes;            // a stage's room for one matrix
@@ -175,6 +176,8 @@ struct LnTeams {
   int* dev_status;
 };
 constexpr int kTeamThreads = 512, kTeamWarps = kTeamThreads / 32;
+// Teams of several warps; of a warp or less (kSub below); of a warp or less with several rows of each team in a unit.
+enum { kWide, kNarrow, kGrouped };
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
@@ -377,9 +380,9 @@ struct TeamRing {
 template <int VEC, int NV>
 __host__ __device__ constexpr bool fwd_params_shared() { return VEC == 8 && NV > 3; }
 // Bound by memory: 65536 x 1280 fp16 58 us (5.8 TB/s, 89 % of a copy's rate), 50000 x 1280 fp32 90 us (5.7 TB/s).
-// kSub: teams of a warp or less.
-template <class T, int VEC, int NV, bool kSub>
+template <class T, int VEC, int NV, int kTeams>
 __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_teams_kernel(const LnArgs a, const LnTeams t) {
+  constexpr bool kSub = kTeams != kWide;
   pdl_launch_dependents();
   using F = typename Lanes<VEC>::F;
   constexpr int N = Lanes<VEC>::N;
@@ -411,61 +414,65 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
     }
   }
   bool failed = false;
-  for (; ring.left > 0; ring.next_unit()) {
-    const uint32_t row = ring.row + (kSub ? me.sub : 0);
-    const bool in = !kSub || ring.has(0, me.sub);
+  const int groups = kTeams == kGrouped ? t.groups : 1;
+  for (; ring.left > 0 && !failed; ring.next_unit()) {
     failed = !ring.wait(700);
     if (kSub && failed) break;
     const T* xs = ring.mat(0) + (kSub ? me.sub * a.C : 0);
-    F x[NV][N];
-    F s[2] = {splat<F>(0.f), splat<F>(0.f)};   // two chains of additions
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = me.lane + i * t.TL;
-      if (in && has_vector<VEC, NV>(i, v, n)) {
-        widen<T, VEC>(load_vec<T, VEC>(xs + v * VEC), x[i]);
-#pragma unroll
-        for (int j = 0; j < N; ++j) s[(i * N + j) % 2] = add(s[(i * N + j) % 2], x[i][j]);
-      }
-    }
-    float sum[1] = {total(add(s[0], s[1]))};
-    failed = team_sum<1, kSub>(sum, t, me, slots, 0, failed);
-    if (failed) break;
-    // the stage has been read by the whole team
-    __syncwarp();
-    if (me.warp == 0) ring.refill();
-    ring.next_stage();
-    const float mean = mean_of(sum[0], a);
-    const F minus = splat<F>(-mean);
-    s[0] = s[1] = splat<F>(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (has_vector<VEC, NV>(i, me.lane + i * t.TL, n)) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          x[i][j] = add(x[i][j], minus);
-          s[(i * N + j) % 2] = fma(x[i][j], x[i][j], s[(i * N + j) % 2]);
-        }
-      }
-    }
-    sum[0] = total(add(s[0], s[1]));
-    team_sum<1, kSub>(sum, t, me, slots, 1, false);
-    const float rstd = rsqrtf(sum[0] * a.inv_c + a.eps);
-    if (in) {
-      const F scale = splat<F>(rstd);
-      T* yr = static_cast<T*>(a.y) + row * a.ldy;
+    for (int sub = kSub ? me.sub : 0, g = 1; g <= groups; ++g, sub += t.per, xs += t.per * a.C) {
+      const uint32_t row = ring.row + sub;
+      const bool in = !kSub || ring.has(0, sub);
+      F x[NV][N];
+      F s[2] = {splat<F>(0.f), splat<F>(0.f)};   // two chains of additions
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = me.lane + i * t.TL;
-        if (has_vector<VEC, NV>(i, v, n)) {
-          if constexpr (kShared) shared_param<VEC>(sw, n, v, w[0]), shared_param<VEC>(sw + a.C, n, v, b[0]);
-          constexpr int k = kShared ? 0 : 1;
+        if (in && has_vector<VEC, NV>(i, v, n)) {
+          widen<T, VEC>(load_vec<T, VEC>(xs + v * VEC), x[i]);
 #pragma unroll
-          for (int j = 0; j < N; ++j) x[i][j] = fma(mul(x[i][j], scale), w[k * i][j], b[k * i][j]);
-          store_vec<T, VEC>(yr + v * VEC, narrow<T, VEC>(x[i]));
+          for (int j = 0; j < N; ++j) s[(i * N + j) % 2] = add(s[(i * N + j) % 2], x[i][j]);
         }
       }
-      if (a.mean && me.lane == 0) a.mean[row] = mean, a.rstd[row] = rstd;
+      float sum[1] = {total(add(s[0], s[1]))};
+      failed = team_sum<1, kSub>(sum, t, me, slots, 0, failed);
+      if (failed) break;
+      if (g == groups) {   // the stage has been read by the whole team
+        __syncwarp();
+        if (me.warp == 0) ring.refill();
+        ring.next_stage();
+      }
+      const float mean = mean_of(sum[0], a);
+      const F minus = splat<F>(-mean);
+      s[0] = s[1] = splat<F>(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (has_vector<VEC, NV>(i, me.lane + i * t.TL, n)) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            x[i][j] = add(x[i][j], minus);
+            s[(i * N + j) % 2] = fma(x[i][j], x[i][j], s[(i * N + j) % 2]);
+          }
+        }
+      }
+      sum[0] = total(add(s[0], s[1]));
+      team_sum<1, kSub>(sum, t, me, slots, 1, false);
+      const float rstd = rsqrtf(sum[0] * a.inv_c + a.eps);
+      if (in) {
+        const F scale = splat<F>(rstd);
+        T* yr = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int v = me.lane + i * t.TL;
+          if (has_vector<VEC, NV>(i, v, n)) {
+            if constexpr (kShared) shared_param<VEC>(sw, n, v, w[0]), shared_param<VEC>(sw + a.C, n, v, b[0]);
+            constexpr int k = kShared ? 0 : 1;
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[i][j] = fma(mul(x[i][j], scale), w[k * i][j], b[k * i][j]);
+            store_vec<T, VEC>(yr + v * VEC, narrow<T, VEC>(x[i]));
+          }
+        }
+        if (a.mean && me.lane == 0) a.mean[row] = mean, a.rstd[row] = rstd;
+      }
     }
   }
   if (__syncthreads_or(failed)) let_copies_land();
@@ -473,10 +480,11 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
 
 // ---- backward --------------------------------------------------------------------------------
 // fp32 rows are bound by memory (8192 x 5120 76 us without the column sums' second launch, 6.6 TB/s), 16-bit ones by issue slots (58 to 60 %
-// of them taken, by 16 warps an SM: the sums' registers allow no more): 50000 x 1280 72 us, 5.3 TB/s; 32768 x 640 28.5 us and 4.7 for
+// of them taken, by 16 warps an SM: the sums' registers allow no more): 50000 x 1280 71 us, 5.4 TB/s; 32768 x 640 27 us and 4.7 for
 // the second launch.
-template <class T, int VEC, int NV, bool kSub>
+template <class T, int VEC, int NV, int kTeams>
 __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnArgs a, const LnTeams t) {
+  constexpr bool kSub = kTeams != kWide;
   pdl_launch_dependents();
   using F = typename Lanes<VEC>::F;
   constexpr int N = Lanes<VEC>::N;
@@ -498,65 +506,71 @@ __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnA
 #pragma unroll
     for (int j = 0; j < N; ++j) dw[i][j] = db[i][j] = splat<F>(0.f);
   float mean_next = 0.f, rstd_next = 0.f;
-  auto moments = [&](int ahead) {
-    const uint32_t r = ring.row + ahead * ring.step + me.sub;
-    if (ring.has(ahead, me.sub)) mean_next = a.mean[r], rstd_next = a.rstd[r];
+  auto moments = [&](int ahead, int sub) {
+    const uint32_t r = ring.row + ahead * ring.step + sub;
+    if (ring.has(ahead, sub)) mean_next = a.mean[r], rstd_next = a.rstd[r];
   };
-  moments(0);
+  moments(0, me.sub);
   __syncthreads();
   bool failed = false;
-  for (; ring.left > 0; ring.next_unit()) {
-    const bool in = !kSub || ring.has(0, me.sub);
+  const int groups = kTeams == kGrouped ? t.groups : 1;
+  for (; ring.left > 0 && !failed; ring.next_unit()) {
     failed = !ring.wait(701);
     if (kSub && failed) break;
     const T* xs = ring.mat(0) + (kSub ? me.sub * a.C : 0);
     const T* ds = ring.mat(1) + (kSub ? me.sub * a.C : 0);
-    Vec<T, VEC> rx[NV], rd[NV];          // as loaded, and widened twice: registers bound this kernel
-    const float mean = mean_next, rstd = rstd_next;
-    moments(1);
-    F s1 = splat<F>(0.f), s2 = s1;       // sum(g), sum(g (x - mean))
-    const F minus = splat<F>(-mean);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = me.lane + i * t.TL;
-      if (in && has_vector<VEC, NV>(i, v, n)) {
-        F w[N], d[N], x[N];
-        rx[i] = load_vec<T, VEC>(xs + v * VEC), rd[i] = load_vec<T, VEC>(ds + v * VEC);
-        widen<T, VEC>(rx[i], x), widen<T, VEC>(rd[i], d);
-        shared_param<VEC>(sw, n, v, w);
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const F g = mul(d[j], w[j]);
-          s1 = add(s1, g);
-          s2 = fma(g, add(x[j], minus), s2);
-        }
-      }
-    }
-    float sum[2] = {total(s1), total(s2)};
-    failed = team_sum<2, kSub>(sum, t, me, slots, ring.left & 1, failed);
-    if (failed) break;
-    __syncwarp();
-    if (me.warp == 0) ring.refill();   // the stage has been read by the whole team
-    ring.next_stage();
-    const F r = splat<F>(rstd), c1 = splat<F>(-rstd * (sum[0] * a.inv_c)), c2 = splat<F>(-rstd * (rstd * (sum[1] * a.inv_c)));
-    if (in) {
-      T* out = static_cast<T*>(a.y) + (ring.row + (kSub ? me.sub : 0)) * a.ldy;
+    for (int sub = kSub ? me.sub : 0, g = 1; g <= groups; ++g, sub += t.per, xs += t.per * a.C, ds += t.per * a.C) {
+      const bool in = !kSub || ring.has(0, sub);
+      Vec<T, VEC> rx[NV], rd[NV];          // as loaded, and widened twice: registers bound this kernel
+      const float mean = mean_next, rstd = rstd_next;
+      if (g < groups) moments(0, sub + t.per);
+      else moments(1, kSub ? me.sub : 0);
+      F s1 = splat<F>(0.f), s2 = s1;       // sum(g), sum(g (x - mean))
+      const F minus = splat<F>(-mean);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int v = me.lane + i * t.TL;
-        if (has_vector<VEC, NV>(i, v, n)) {
+        if (in && has_vector<VEC, NV>(i, v, n)) {
           F w[N], d[N], x[N];
+          rx[i] = load_vec<T, VEC>(xs + v * VEC), rd[i] = load_vec<T, VEC>(ds + v * VEC);
           widen<T, VEC>(rx[i], x), widen<T, VEC>(rd[i], d);
           shared_param<VEC>(sw, n, v, w);
 #pragma unroll
           for (int j = 0; j < N; ++j) {
-            // dx = dy (w r) + h c2 + c1
-            const F h = mul(add(x[j], minus), r);
-            dw[i][j] = fma(d[j], h, dw[i][j]);
-            db[i][j] = add(db[i][j], d[j]);
-            x[j] = fma(d[j], mul(w[j], r), fma(h, c2, c1));
+            const F g = mul(d[j], w[j]);
+            s1 = add(s1, g);
+            s2 = fma(g, add(x[j], minus), s2);
           }
-          store_vec<T, VEC>(out + v * VEC, narrow<T, VEC>(x));
+        }
+      }
+      float sum[2] = {total(s1), total(s2)};
+      failed = team_sum<2, kSub>(sum, t, me, slots, ring.left & 1, failed);
+      if (failed) break;
+      if (g == groups) {   // the stage has been read by the whole team
+        __syncwarp();
+        if (me.warp == 0) ring.refill();
+        ring.next_stage();
+      }
+      const F r = splat<F>(rstd), c1 = splat<F>(-rstd * (sum[0] * a.inv_c)), c2 = splat<F>(-rstd * (rstd * (sum[1] * a.inv_c)));
+      if (in) {
+        T* out = static_cast<T*>(a.y) + (ring.row + sub) * a.ldy;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int v = me.lane + i * t.TL;
+          if (has_vector<VEC, NV>(i, v, n)) {
+            F w[N], d[N], x[N];
+            widen<T, VEC>(rx[i], x), widen<T, VEC>(rd[i], d);
+            shared_param<VEC>(sw, n, v, w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              // dx = dy (w r) + h c2 + c1
+              const F h = mul(add(x[j], minus), r);
+              dw[i][j] = fma(d[j], h, dw[i][j]);
+              db[i][j] = add(db[i][j], d[j]);
+              x[j] = fma(d[j], mul(w[j], r), fma(h, c2, c1));
+            }
+            store_vec<T, VEC>(out + v * VEC, narrow<T, VEC>(x));
+          }
         }
       }
     }
@@ -786,11 +800,21 @@ static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats,
   if (vec == 1) nv = (nv + 3) / 4 * 4;
   const int warps = TL > 32 ? TL / 32 : 1, teams = kTeamWarps / warps;
   t.ceiling = (unsigned long long)a.rows * a.C / (16 / elem) * (16 / elem);
-  t.TL = TL, t.rows = TL < 32 ? 32 / TL : 1, t.units = (uint32_t)((a.rows + t.rows - 1) / t.rows);
-  t.mat_bytes = (int)((t.rows * row + 15) / 16 * 16 + (vec == 1 ? 32 : 0));   // a widened span begins and ends up to 15 bytes further out
   const long long slots = 2ll * kTeamWarps * mats * 4, rest = params + slots + teams * 8 * 8 + 512;
   const long long scratch = sums && teams > 1 ? teams * 2ll * a.C * 4 : 0;
-  long long stages = (room - rest) / ((long long)teams * mats * t.mat_bytes);
+  auto bytes = [&](long long rows) { return (rows * row + 15) / 16 * 16 + (vec == 1 ? 32 : 0); };   // a widened span begins and ends up to 15 bytes further out
+  auto stages_of = [&](long long rows) { return (room - rest) / (teams * mats * bytes(rows)); };
+  // A warp's waits and refills cost as many instructions as 600 values of a row: several rows of 16-bit values share them, as long as two
+  // stages remain (three forward: with two, 100000 x 640 49.1 us for 43.8) and every team has six units or more.  fp16 backward of 1000000 x
+  // 64 93.5 -> 80.7 us, 100000 x 640 80.0 -> 77.6; fp32 and rows that are not 16-byte aligned gain nothing (65536 x 320 fp32 29.7, 32.3).
+  t.TL = TL, t.per = TL < 32 ? 32 / TL : 1, t.groups = 1;
+  const long long grid_teams = (long long)teams * sm_count() * (room < kSmemSm ? 2 : 1);
+  while (elem == 2 && vec > 1 && TL <= 32 && t.groups < 8 && stages_of(2ll * t.groups * t.per) >= (mats == 1 ? 3 : 2) &&
+         a.rows >= 6 * grid_teams * 2 * t.groups * t.per)
+    t.groups *= 2;
+  t.rows = t.per * t.groups, t.units = (uint32_t)((a.rows + t.rows - 1) / t.rows);
+  t.mat_bytes = (int)bytes(t.rows);
+  long long stages = stages_of(t.rows);
   if (stages > 8) stages = 8;
   if (stages < 2 || scratch > room - rest) return false;
   t.stages = (int)stages;
@@ -810,12 +834,15 @@ static int team_blocks(const LnTeams& t, int per_sm) {
 // Vectors a thread holds in teams of up to a warp (eight of 16-bit values spill there: 2048 columns 52.4 us, with seven 46.6).
 template <int VEC>
 constexpr int fwd_most_sub() { return VEC == 1 ? 12 : VEC == 8 ? 7 : 6; }
-template <class T, int VEC, int NV, bool kSub = false>
+template <class T, int VEC, int NV, int kTeams = kWide>
 static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
-  if constexpr (!kSub && NV <= fwd_most_sub<VEC>())
-    if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, true>(a, t, smem, s);
-  if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kSub>>(kSmemSm)) return rc;
-  return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV, kSub>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
+  if constexpr (kTeams == kWide && NV <= fwd_most_sub<VEC>()) {
+    if constexpr (sizeof(T) == 2 && VEC > 1)
+      if (t.groups > 1) return ln_fwd_teams_launch<T, VEC, NV, kGrouped>(a, t, smem, s);
+    if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, kNarrow>(a, t, smem, s);
+  }
+  if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
+  return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV, kTeams>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
 }
 template <class T, int VEC>
 static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
@@ -881,20 +908,25 @@ static int ln_fwd(const LnArgs& a, bool vec, cudaStream_t s) {
   return launch_kernel("ln_fwd_long_kernel launch", ln_fwd_long_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, s, 1, a);
 }
 
-template <class T, int VEC, int NV, bool kSub = false>
+// Vectors a thread holds: 24 values of 16 bits or 16 of fp32 (8192 x 5120: 96 us with 24, 86 with 16); wider rows spill.
+template <int VEC>
+constexpr int bwd_most() { return VEC == 1 ? 12 : VEC == 8 ? 3 : 4; }
+template <class T, int VEC, int NV, int kTeams = kWide>
 static int ln_bwd_teams_launch(const LnArgs& a, const LnTeams& t, int blocks, int smem, cudaStream_t s) {
-  if constexpr (!kSub)
-    if (t.TL <= 32) return ln_bwd_teams_launch<T, VEC, NV, true>(a, t, blocks, smem, s);
-  if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV, kSub>>(kSmemSm)) return rc;
-  return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV, kSub>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
+  if constexpr (kTeams == kWide && NV <= (VEC == 4 && sizeof(T) == 2 ? 5 : bwd_most<VEC>())) {
+    if constexpr (sizeof(T) == 2 && VEC > 1)
+      if (t.groups > 1) return ln_bwd_teams_launch<T, VEC, NV, kGrouped>(a, t, blocks, smem, s);
+    if (t.TL <= 32) return ln_bwd_teams_launch<T, VEC, NV, kNarrow>(a, t, blocks, smem, s);
+  }
+  if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
+  return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV, kTeams>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
 }
 template <class T, int VEC>
 static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s) {
   LnTeams t = {};
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
-  // Vectors a thread holds: 24 values of 16 bits or 16 of fp32 (8192 x 5120: 96 us with 24, 86 with 16); wider rows spill.
-  const int most = VEC == 1 ? 12 : VEC == 8 ? 3 : 4, wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
+  constexpr int most = bwd_most<VEC>(), wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
   done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
                                          plan_teams(t, a, sizeof(T), VEC, 2, most, wide, 4ll * a.C, true, kSmemSm, nv, smem));
   if (!done) return kOk;

@@ -95,6 +95,16 @@ def test_many_rows_apart(rows, c):
         assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype,param", [(torch.float16, torch.float16), (torch.bfloat16, torch.float32)], ids=str)
+@pytest.mark.parametrize("rows,c", [(240007, 64), (470003, 40), (115003, 128), (60011, 512), (60013, 640), (30011, 1024)])
+def test_units_of_several_rows(rows, c, dtype, param):
+    """Rows enough for several of them to share a stage of the ring, the last one not full; and rows of a wider tensor."""
+    cuda_or_skip()
+    x, w, b, dy = _inputs(rows, c, dtype, param)
+    _check(x, w, b, dy)
+    _check(torch.cat([x, x], dim=1)[:, c:], w, b, dy)
+
+
 @pytest.mark.parametrize("rows,c", [(40, 1285), (4001, 320), (801, 1608), (601, 4096), (1701, 643), (513, 20000)])
 def test_in_place(rows, c):
     cuda_or_skip()
