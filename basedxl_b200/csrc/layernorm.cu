@@ -837,12 +837,16 @@ constexpr int fwd_most_sub() { return VEC == 1 ? 12 : VEC == 8 ? 7 : 6; }
 template <class T, int VEC, int NV, int kTeams = kWide>
 static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
   if constexpr (kTeams == kWide && NV <= fwd_most_sub<VEC>()) {
-    if constexpr (sizeof(T) == 2 && VEC > 1)
+    if constexpr (sizeof(T) == 2 && VEC > 1 && NV <= 5)   // (three stages of two wider rows each do not fit)
       if (t.groups > 1) return ln_fwd_teams_launch<T, VEC, NV, kGrouped>(a, t, smem, s);
     if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, kNarrow>(a, t, smem, s);
   }
-  if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
-  return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV, kTeams>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
+  if constexpr (kTeams == kWide && 2 * NV <= fwd_most_sub<VEC>()) {
+    return fail(kErrUnsupported, "bxl_layernorm_fwd: no team of several warps has rows this narrow");
+  } else {
+    if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
+    return launch_kernel("ln_fwd_teams_kernel launch", ln_fwd_teams_kernel<T, VEC, NV, kTeams>, dim3(team_blocks(t, smem <= kSmemHalf ? 2 : 1)), dim3(kTeamThreads), smem, s, 1, a, t);
+  }
 }
 template <class T, int VEC>
 static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
@@ -918,15 +922,19 @@ static int ln_bwd_teams_launch(const LnArgs& a, const LnTeams& t, int blocks, in
       if (t.groups > 1) return ln_bwd_teams_launch<T, VEC, NV, kGrouped>(a, t, blocks, smem, s);
     if (t.TL <= 32) return ln_bwd_teams_launch<T, VEC, NV, kNarrow>(a, t, blocks, smem, s);
   }
-  if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
-  return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV, kTeams>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
+  if constexpr (kTeams == kWide && 2 * NV <= (VEC == 4 && sizeof(T) == 2 ? 6 : bwd_most<VEC>())) {
+    return fail(kErrUnsupported, "bxl_layernorm_bwd: no team of several warps has rows this narrow");
+  } else {
+    if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
+    return launch_kernel("ln_bwd_teams_kernel launch", ln_bwd_teams_kernel<T, VEC, NV, kTeams>, dim3(blocks), dim3(kTeamThreads), smem, s, 1, a, t);
+  }
 }
 template <class T, int VEC>
 static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s) {
   LnTeams t = {};
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
-  constexpr int most = bwd_most<VEC>(), wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 8;
+  constexpr int most = bwd_most<VEC>(), wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 6;
   done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
                                          plan_teams(t, a, sizeof(T), VEC, 2, most, wide, 4ll * a.C, true, kSmemSm, nv, smem));
   if (!done) return kOk;
@@ -952,9 +960,7 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
     if (nv == 4) return ln_bwd_teams_launch<T, VEC, 4>(a, t, blocks, smem, s);
     if constexpr (VEC == 4) {
       if (nv == 5) return ln_bwd_teams_launch<T, VEC, 5>(a, t, blocks, smem, s);
-      if (nv == 6) return ln_bwd_teams_launch<T, VEC, 6>(a, t, blocks, smem, s);
-      if (nv == 7) return ln_bwd_teams_launch<T, VEC, 7>(a, t, blocks, smem, s);
-      return ln_bwd_teams_launch<T, VEC, 8>(a, t, blocks, smem, s);
+      return ln_bwd_teams_launch<T, VEC, 6>(a, t, blocks, smem, s);
     }
     return fail(kErrUnsupported, "bxl_layernorm_bwd: no kernel for %d vectors a thread", nv);
   }
