@@ -1404,9 +1404,10 @@ int repack_rows(const RowCopy& a, const RowCopy& b, cudaStream_t s) {
   return launch_kernel("repack_rows_kernel launch", repack_rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, oa, ob);
 }
 
+// Whether results or residual need the variants for rows of any alignment (and rows that repeat or overlap, as a broadcast residual's).
 static bool linear_ragged(const LinearProduct& q) {
   auto rows16 = [](const void* base, long long ld) { return aligned16(base) && ld % 8 == 0; };
-  return q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && !rows16(q.residual, q.ldr)) || (q.pre && !rows16(q.pre, q.ldp));
+  return q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && (!rows16(q.residual, q.ldr) || q.ldr < q.N)) || (q.pre && !rows16(q.pre, q.ldp));
 }
 static int linear_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(q.residual); }
 static bool linear_heavy(const LinearProduct& q) { return linear_ragged(q) || q.residual || q.pre; }

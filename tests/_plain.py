@@ -42,6 +42,10 @@ def within(got, want, bound, what):
     off = (got.double() - want).abs()
     limit = bound + HALF[t] * (want.abs() + bound) + TINY[t]
     bad = ~(off <= limit)  # NaN counts
+    # The largest finite value is (2 - 2 h) 2^e; from half a step above it on, (2 - h) 2^e, rounding gives infinity, as it has to: 60011 equal
+    # rows whose value is 1.34 add up to 80463, beyond the 65520 of fp16.
+    over = want.abs() + bound >= torch.finfo(t).max * (2 - HALF[t]) / (2 - 2 * HALF[t])
+    bad &= ~(over & (got.double() == want.sign() * float("inf")))
     if bad.any():
         i = int((off / limit).nan_to_num(float("inf")).argmax())
         raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} values off; worst at {i}: {got.flatten()[i].item()} is not "

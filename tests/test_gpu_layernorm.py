@@ -105,6 +105,14 @@ def test_units_of_several_rows(rows, c, dtype, param):
     _check(torch.cat([x, x], dim=1)[:, c:], w, b, dy)
 
 
+@pytest.mark.parametrize("rows,c", [(40, 1285), (4001, 320), (801, 1608), (1701, 643), (60011, 640)])
+def test_repeated_rows(rows, c):
+    cuda_or_skip()
+    x, w, b, dy = _inputs(rows, c, torch.float16)
+    _check(x[:1].expand_as(x), w, b, dy)
+    _check(x, w, b, dy[:1].expand_as(dy))
+
+
 @pytest.mark.parametrize("rows,c", [(40, 1285), (4001, 320), (801, 1608), (601, 4096), (1701, 643), (513, 20000)])
 def test_in_place(rows, c):
     cuda_or_skip()

@@ -144,6 +144,21 @@ def test_layouts(layout, m):
     _check_bwd(s, "none", None)
 
 
+@pytest.mark.parametrize("m,k,n", [(3, 320, 640), (140, 320, 640), (140, 72, 99), (20, 2048, 64), (3000, 64, 264)])
+def test_repeated_rows(m, k, n):
+    """Broadcast rows, one memory for all of them, in the place of every input that has rows."""
+    cuda_or_skip()
+    _lib, ops = _ops()
+    s = _inputs(m, k, n, torch.bfloat16)
+    one = {name: s[name][:1].expand_as(s[name]) for name in ("x", "residual", "dy")}
+    pre = _check_fwd({**s, "residual": one["residual"]}, "silu")
+    _check_fwd({**s, "x": one["x"]}, "gelu")
+    _check_bwd({**s, "dy": one["dy"]}, "silu", pre)
+    _check_bwd({**s, "x": one["x"], "dy": one["dy"]}, "none", None)
+    _check_bwd(s, "relu", pre[:1].expand_as(pre))
+    _lib.device_status()
+
+
 def test_empty_and_wanted():
     cuda_or_skip()
     _, ops = _ops()
