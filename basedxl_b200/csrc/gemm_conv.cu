@@ -1162,10 +1162,10 @@ static TileConfig choose_tiles(int tiles_m, int N, int num_kb, bool b_kn, int fo
   return best;
 }
 
-// The same model for one round of single CTAs.
-static double tiles_cost(int num_kb, int bn, bool heavy) {
+// The same model for one round of single CTAs (linear layers).
+static double tiles_cost(int num_kb, int bn) {
   const double kb_us = fmax(bn / 256.0 * 0.256, (16384.0 + bn * 128.0) / 139000.0);
-  return (num_kb * kb_us + (heavy ? 0.455 : 0.271) * (bn / 32.0) + 4.28) * (1.0 - 0.05 * bn / 256.0);
+  return (num_kb * kb_us + 0.455 * (bn / 32.0) + 4.28) * (1.0 - 0.05 * bn / 256.0);
 }
 // Of two launches in a row the second one's set-up runs beside the first.
 constexpr double kOverlapUs = 1.5;
@@ -1187,7 +1187,7 @@ template <bool kConv, bool kPair, bool kSplit, bool kTwo, int kLin>
 static int launch_one(const GemmParams& p, int num_units, cudaStream_t stream) {
   const int b_rows = kLin ? staged_cols(kPair ? p.bn / 2 : p.bn, p.b_kn) : kPair ? p.bn / 2 : p.bn;
   const int smem = p.stages * p.parts * (kABytes + b_rows * 128) + recv_bytes(p.bn, kSplit ? p.split : 1) + kSmemMisc +
-                   (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? ragged_bytes(kLin) : kLin ? out_bytes(p.residual) : 0);
+                   (p.ln_part ? kSmemLnExtra : 0) + (p.ragged ? ragged_bytes(kLin) : kLin ? out_bytes(p.residual && !kSplit) : 0);
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1409,13 +1409,18 @@ static bool linear_ragged(const LinearProduct& q) {
   auto rows16 = [](const void* base, long long ld) { return aligned16(base) && ld % 8 == 0; };
   return q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && (!rows16(q.residual, q.ldr) || q.ldr < q.N)) || (q.pre && !rows16(q.pre, q.ldp));
 }
-static int linear_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(q.residual); }
-static bool linear_heavy(const LinearProduct& q) { return linear_ragged(q) || q.residual || q.pre; }
+static int linear_extra(const LinearProduct& q, int split = 1) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(q.residual && split == 1); }
+// The choice of tiles does not look at the residual or the value before the activation: with them and without, the sums have the same
+// order and the result the same bits.  (A residual's buffers leave at least three stages.)  As epilogues go all of these are heavy: 64 x
+// 2304 x 128 10.1 us when products without either counted as light, 8.0 so.
+static int planned_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(false); }
 static int tiles_along(int n, int of) { return (int)(((long long)n + of - 1) / of); }
 static TileConfig linear_tiles(const LinearProduct& q) {
   const bool one = linear_ragged(q);   // no variant with pairs or splits
-  return choose_tiles(tiles_along(q.M, kBM), q.N, tiles_along(q.K, kBK), q.b_kn != 0, g_force_bn, one ? 1 : g_force_split, one ? 0 : g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0, linear_extra(q), 1,
-                      linear_heavy(q), true);
+  TileConfig tc = choose_tiles(tiles_along(q.M, kBM), q.N, tiles_along(q.K, kBK), q.b_kn != 0, g_force_bn, one ? 1 : g_force_split, one ? 0 : g_force_pair < 0 ? kDefaultPair : g_force_pair, 0.0,
+                               planned_extra(q), 1, true, true);
+  tc.stages = stages_for(tc.pair ? 2 * staged_cols(tc.bn / 2, q.b_kn) : staged_cols(tc.bn, q.b_kn), tc.split, tc.pair, linear_extra(q, tc.split), 1, tc.bn);
+  return tc;
 }
 static int linear_params(const LinearProduct& q, const TileConfig& tc, GemmParams& p) {
   int* st = device_status_ptr();
@@ -1519,8 +1524,8 @@ static Sliced sliced_within(const LinearProduct& q, int ctas) {
   const int kb = tiles_along(q.K, kBK);
   for (int bn = 64; bn <= 256; bn += 64) {
     const long long tiles = (long long)tiles_along(q.M, kBM) * tiles_along(q.N, bn);
-    if (tiles > ctas || stages_for(bn, 1, 0, linear_extra(q)) < 3) continue;
-    const double whole = tiles_cost(kb, bn, linear_heavy(q));
+    if (tiles > ctas || stages_for(bn, 1, 0, planned_extra(q)) < 3) continue;
+    const double whole = tiles_cost(kb, bn);
     if (whole < best.cost_us) best.bn = bn, best.slices = 1, best.tiles = (int)tiles, best.cost_us = whole;
     int s = (int)(ctas / tiles);
     s = s < kb / 2 ? s : kb / 2;
@@ -1528,7 +1533,7 @@ static Sliced sliced_within(const LinearProduct& q, int ctas) {
     if (s < 2) continue;
     const int per = (kb + s - 1) / s;
     s = (kb + per - 1) / per;
-    const double c = tiles_cost(per, bn, true) + 3.0 + part_bytes(q, s) / 2.0e6;   // the second launch reads what the first has left in L2
+    const double c = tiles_cost(per, bn) + 3.0 + part_bytes(q, s) / 2.0e6;   // the second launch reads what the first has left in L2
     if (s > 1 && c < best.cost_us) best.bn = bn, best.slices = s, best.tiles = (int)tiles, best.cost_us = c;
   }
   return best;
@@ -1573,7 +1578,7 @@ static const LinearPlan& plan_products(const LinearProduct* const* q, int n) {
   memset(&key, 0, sizeof(key));
   unsigned hash = 0;
   for (int i = 0; i < n; ++i) {
-    const int v[5] = {q[i]->M, q[i]->N, q[i]->K, q[i]->b_kn, (linear_ragged(*q[i]) ? 2 : 0) + (linear_heavy(*q[i]) ? 1 : 0) + (q[i]->residual ? 4 : 0)};
+    const int v[5] = {q[i]->M, q[i]->N, q[i]->K, q[i]->b_kn, (linear_ragged(*q[i]) ? 1 : 0) + (q[i]->residual ? 2 : 0)};
     for (int j = 0; j < 5; ++j) key.v[i][j] = v[j], hash = hash * 31u + (unsigned)v[j];
   }
   key.n = n, key.sms = sm_count(), key.bn = g_force_bn, key.split = g_force_split, key.pair = g_force_pair;

@@ -159,6 +159,19 @@ def test_repeated_rows(m, k, n):
     _lib.device_status()
 
 
+@pytest.mark.parametrize("m,k,n", [(68, 2240, 64), (16, 2752, 832), (820, 5032, 88), (517, 2759, 16), (11, 2189, 184), (4096, 320, 2560), (300, 640, 640), (5, 320, 64)])
+def test_same_bits_with_and_without(m, k, n):
+    """Neither keeping the value before the activation nor a residual of zeros changes the result."""
+    cuda_or_skip()
+    _, ops = _ops()
+    s = _inputs(m, k, n, torch.bfloat16)
+    y = ops.linear_act(s["x"], s["weight"], s["bias"], activation="silu")
+    zeros = torch.zeros_like(y)
+    assert torch.equal(ops.linear_act(s["x"], s["weight"], s["bias"], activation="silu", want_pre=True)[0], y)
+    assert torch.equal(ops.linear_act(s["x"], s["weight"], s["bias"], activation="silu", residual=zeros), y)
+    assert torch.equal(ops.linear_act(s["x"], s["weight"], s["bias"], activation="silu", residual=zeros, want_pre=True)[0], y)
+
+
 def test_empty_and_wanted():
     cuda_or_skip()
     _, ops = _ops()
