@@ -102,3 +102,36 @@ def test_layernorm(rows, c, dtype):
     f.check()
     g.check()
     _l.device_status()
+
+
+def test_two_streams_at_once():
+    """Calls of every operator on two streams beside one another give what they give one after the other."""
+    cuda_or_skip()
+    from basedxl_b200 import ops
+
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()
+        return [(rn(m, k), rn(n, k) * k**-0.5, rn(n), rn(m, n), rn(k)) for m, k, n in ((700, 1280, 640), (2500, 48, 40), (5, 320, 1280), (300, 321, 643))]
+
+    def step(sets):
+        out = []
+        for x, w, b, dy, gain in sets:
+            h, mean, rstd = ops.layernorm_fwd(x, gain, None, want_stats=True)
+            y, pre = ops.linear_act(h, w, b, activation="gelu", residual=dy, want_pre=True)
+            dh, dw, db = ops.linear_act_bwd(dy, h, w, pre, activation="gelu")
+            out += [y, dw, db, *ops.layernorm_bwd(dh, x, mean, rstd, gain)]
+        return out
+
+    sets = [inputs(1), inputs(2)]
+    want = [step(s) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for once in got[i]:
+            assert all(torch.equal(p, q) for p, q in zip(once, want[i]))
