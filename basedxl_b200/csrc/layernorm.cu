@@ -948,11 +948,12 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
     return ln_bwd_teams_launch<T, 1, 16>(a, t, blocks, smem, s);
   } else {
     // Vectors of 8 bytes where those of 16 would leave a sixth or more of the last ones' lanes idle (64M values of fp16: 640 columns 87.6 us
-    // with 16 bytes, 82.0 with 8; 1280 78.4 and 72.1).
+    // with 16 bytes, 82.0 with 8; 1280 78.4 and 72.1; 3436 x 13440, where both spill, 106 and 95).
     if constexpr (VEC == 8) {
       const int half = (a.C / 4 + t.TL - 1) / t.TL;
       if (half == 3) return ln_bwd_teams_launch<T, 4, 3>(a, t, blocks, smem, s);
       if (half == 5) return ln_bwd_teams_launch<T, 4, 5>(a, t, blocks, smem, s);
+      if (half == 7) return ln_bwd_teams_launch<T, 4, 7>(a, t, blocks, smem, s);
     }
     if (nv == 1) return ln_bwd_teams_launch<T, VEC, 1>(a, t, blocks, smem, s);
     if (nv == 2) return ln_bwd_teams_launch<T, VEC, 2>(a, t, blocks, smem, s);
