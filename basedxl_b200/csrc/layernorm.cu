@@ -378,7 +378,7 @@ struct TeamRing {
 // most of the other instructions); beyond three, weight and bias do not fit in registers beside them and are read from shared
 // memory.  64M values of fp16, at most three vectors / up to eight: 1280 columns 51.7 / 45.1 us, 1608 75 / 46.0, 4096 62 / 46.1.
 template <int VEC, int NV>
-__host__ __device__ constexpr bool fwd_params_shared() { return VEC == 8 && NV > 3; }
+__host__ __device__ constexpr bool fwd_params_shared() { return VEC == 1 ? NV > 16 : VEC == 8 && NV > 3; }
 // Bound by memory: 65536 x 1280 fp16 58 us (5.8 TB/s, 89 % of a copy's rate), 50000 x 1280 fp32 90 us (5.7 TB/s).
 template <class T, int VEC, int NV, int kTeams>
 __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_teams_kernel(const LnArgs a, const LnTeams t) {
@@ -833,7 +833,7 @@ static int team_blocks(const LnTeams& t, int per_sm) {
 
 // Vectors a thread holds in teams of up to a warp (eight of 16-bit values spill there: 2048 columns 52.4 us, with seven 46.6).
 template <int VEC>
-constexpr int fwd_most_sub() { return VEC == 1 ? 12 : VEC == 8 ? 7 : 6; }
+constexpr int fwd_most_sub() { return VEC == 1 ? 24 : VEC == 8 ? 7 : 6; }
 template <class T, int VEC, int NV, int kTeams = kWide>
 static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
   if constexpr (kTeams == kWide && NV <= fwd_most_sub<VEC>()) {
@@ -841,7 +841,7 @@ static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cuda
       if (t.groups > 1) return ln_fwd_teams_launch<T, VEC, NV, kGrouped>(a, t, smem, s);
     if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, kNarrow>(a, t, smem, s);
   }
-  if constexpr (kTeams == kWide && 2 * NV <= fwd_most_sub<VEC>()) {
+  if constexpr (kTeams == kWide && 2 * NV <= (VEC == 1 ? 12 : fwd_most_sub<VEC>())) {
     return fail(kErrUnsupported, "bxl_layernorm_fwd: no team of several warps has rows this narrow");
   } else {
     if (int rc = allow_smem<ln_fwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
@@ -853,11 +853,19 @@ static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
   LnTeams t = {};
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C);
-  constexpr int sub = fwd_most_sub<VEC>(), most = VEC == 8 ? 8 : sub, wide = VEC == 1 ? 16 : 8;
-  const long long params = VEC == 8 ? 8ll * a.C : 0;
-  done = (VEC > 1 || close) &&
-         (plan_teams(t, a, sizeof(T), VEC, 1, sub, most, params, false, kSmemSm, nv, smem) || plan_teams(t, a, sizeof(T), VEC, 1, sub, wide, params, false, kSmemSm, nv, smem));
-  if (done && nv * VEC <= 8) plan_teams(t, a, sizeof(T), VEC, 1, sub, most, params, false, kSmemHalf, nv, smem);   // two blocks an SM
+  constexpr int sub = fwd_most_sub<VEC>(), most = VEC == 8 ? 8 : sub, wide = 8;
+  const long long params = VEC == 4 ? 0 : 8ll * a.C;
+  // Single values: up to 24 a thread where every team has eight units or more, else 12 for more teams (100000 x 643 fp16 104 us with 12,
+  // 88 with 24; 4099 x 1285 fp32 12.4 and 13.8), or what the widest rows need (5000 x 12001: without a ring 234 us, 88 so).
+  auto plan = [&](int narrow, int wider, long long room) { return plan_teams(t, a, sizeof(T), VEC, 1, narrow, wider, params, false, room, nv, smem); };
+  int narrow = sub, wider = most;
+  done = (VEC > 1 || close) && plan(narrow, wider, kSmemSm);
+  if (VEC == 1 && done && t.units < 8ll * sm_count() * (t.TL > 32 ? kTeamThreads / t.TL : kTeamWarps)) {
+    narrow = wider = 12;
+    if (!plan(narrow, wider, kSmemSm)) narrow = wider = sub, plan(narrow, wider, kSmemSm);
+  }
+  if (VEC == 4 && !done) wider = wide, done = plan(narrow, wider, kSmemSm);
+  if (done && nv * VEC <= 8) plan(narrow, wider, kSmemHalf);   // two blocks an SM
   if (!done) return kOk;
   t.one_copy = close || t.rows == 1;
   if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_fwd: no device status word");
@@ -865,7 +873,9 @@ static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
     if (nv <= 4) return ln_fwd_teams_launch<T, 1, 4>(a, t, smem, s);
     if (nv <= 8) return ln_fwd_teams_launch<T, 1, 8>(a, t, smem, s);
     if (nv <= 12) return ln_fwd_teams_launch<T, 1, 12>(a, t, smem, s);
-    return ln_fwd_teams_launch<T, 1, 16>(a, t, smem, s);
+    if (nv <= 16) return ln_fwd_teams_launch<T, 1, 16>(a, t, smem, s);
+    if (nv <= 20) return ln_fwd_teams_launch<T, 1, 20>(a, t, smem, s);
+    return ln_fwd_teams_launch<T, 1, 24>(a, t, smem, s);
   } else {
     if (nv == 1) return ln_fwd_teams_launch<T, VEC, 1>(a, t, smem, s);
     if (nv == 2) return ln_fwd_teams_launch<T, VEC, 2>(a, t, smem, s);
@@ -912,17 +922,19 @@ static int ln_fwd(const LnArgs& a, bool vec, cudaStream_t s) {
   return launch_kernel("ln_fwd_long_kernel launch", ln_fwd_long_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, s, 1, a);
 }
 
-// Vectors a thread holds: 24 values of 16 bits or 16 of fp32 (8192 x 5120: 96 us with 24, 86 with 16); wider rows spill.
-template <int VEC>
-constexpr int bwd_most() { return VEC == 1 ? 12 : VEC == 8 ? 3 : 4; }
+// Vectors a thread holds: 24 values of 16 bits or 16 of fp32 (8192 x 5120: 96 us with 24, 86 with 16); wider rows spill.  Single values: 16 of
+// 16 bits (38611 x 1819 fp16 165 us with 12, 125 with 16), 12 of fp32; 24 in rows that are wider than that, spilling (5000 x 12001 fp16
+// 330 us without a ring, 180 so).
+template <class T, int VEC>
+constexpr int bwd_most() { return VEC == 1 ? (sizeof(T) == 2 ? 16 : 12) : VEC == 8 ? 3 : 4; }
 template <class T, int VEC, int NV, int kTeams = kWide>
 static int ln_bwd_teams_launch(const LnArgs& a, const LnTeams& t, int blocks, int smem, cudaStream_t s) {
-  if constexpr (kTeams == kWide && NV <= (VEC == 4 && sizeof(T) == 2 ? 5 : bwd_most<VEC>())) {
+  if constexpr (kTeams == kWide && NV <= (VEC == 4 && sizeof(T) == 2 ? 5 : bwd_most<T, VEC>())) {
     if constexpr (sizeof(T) == 2 && VEC > 1)
       if (t.groups > 1) return ln_bwd_teams_launch<T, VEC, NV, kGrouped>(a, t, blocks, smem, s);
     if (t.TL <= 32) return ln_bwd_teams_launch<T, VEC, NV, kNarrow>(a, t, blocks, smem, s);
   }
-  if constexpr (kTeams == kWide && 2 * NV <= (VEC == 4 && sizeof(T) == 2 ? 6 : bwd_most<VEC>())) {
+  if constexpr (kTeams == kWide && 2 * NV <= (VEC == 4 && sizeof(T) == 2 ? 6 : bwd_most<T, VEC>())) {
     return fail(kErrUnsupported, "bxl_layernorm_bwd: no team of several warps has rows this narrow");
   } else {
     if (int rc = allow_smem<ln_bwd_teams_kernel<T, VEC, NV, kTeams>>(kSmemSm)) return rc;
@@ -934,7 +946,7 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
   LnTeams t = {};
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
-  constexpr int most = bwd_most<VEC>(), wide = VEC == 1 ? 16 : VEC == 8 ? 4 : 6;
+  constexpr int most = bwd_most<T, VEC>(), wide = VEC == 1 ? 24 : VEC == 8 ? 4 : 6;
   done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
                                          plan_teams(t, a, sizeof(T), VEC, 2, most, wide, 4ll * a.C, true, kSmemSm, nv, smem));
   if (!done) return kOk;
@@ -945,7 +957,9 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
     if (nv <= 4) return ln_bwd_teams_launch<T, 1, 4>(a, t, blocks, smem, s);
     if (nv <= 8) return ln_bwd_teams_launch<T, 1, 8>(a, t, blocks, smem, s);
     if (nv <= 12) return ln_bwd_teams_launch<T, 1, 12>(a, t, blocks, smem, s);
-    return ln_bwd_teams_launch<T, 1, 16>(a, t, blocks, smem, s);
+    if (nv <= 16) return ln_bwd_teams_launch<T, 1, 16>(a, t, blocks, smem, s);
+    if (nv <= 20) return ln_bwd_teams_launch<T, 1, 20>(a, t, blocks, smem, s);
+    return ln_bwd_teams_launch<T, 1, 24>(a, t, blocks, smem, s);
   } else {
     // Vectors of 8 bytes where those of 16 would leave a sixth or more of the last ones' lanes idle (64M values of fp16: 640 columns 87.6 us
     // with 16 bytes, 82.0 with 8; 1280 78.4 and 72.1; 3436 x 13440, where both spill, 106 and 95).

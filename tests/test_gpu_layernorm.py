@@ -105,6 +105,13 @@ def test_units_of_several_rows(rows, c, dtype, param):
     _check(torch.cat([x, x], dim=1)[:, c:], w, b, dy)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,c", [(19003, 643), (19001, 601), (38003, 301), (76003, 131), (9601, 1285), (5003, 1819), (600, 12001), (2401, 9001)])
+def test_many_rows_of_any_length(rows, c, dtype):
+    cuda_or_skip()
+    _check(*_inputs(rows, c, dtype))
+
+
 @pytest.mark.parametrize("rows,c", [(40, 1285), (4001, 320), (801, 1608), (1701, 643), (60011, 640)])
 def test_repeated_rows(rows, c):
     cuda_or_skip()
