@@ -376,7 +376,8 @@ struct TeamRing {
 
 // Rows of 16-bit values take up to eight vectors a thread, so that few warps share a row (sums across warps, waits and refills are
 // most of the other instructions); beyond three, weight and bias do not fit in registers beside them and are read from shared
-// memory.  64M values of fp16, at most three vectors / up to eight: 1280 columns 51.7 / 45.1 us, 1608 75 / 46.0, 4096 62 / 46.1.
+// memory.  64M values of fp16, at most three vectors / up to eight: 1280 columns 51.7 / 45.1 us, 1608 75 / 46.0, 4096 62 / 46.1.  (Rows
+// of single values: beyond 16 of them.)
 template <int VEC, int NV>
 __host__ __device__ constexpr bool fwd_params_shared() { return VEC == 1 ? NV > 16 : VEC == 8 && NV > 3; }
 // Bound by memory: 65536 x 1280 fp16 58 us (5.8 TB/s, 89 % of a copy's rate), 50000 x 1280 fp32 90 us (5.7 TB/s).
