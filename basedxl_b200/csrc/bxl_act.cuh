@@ -4,8 +4,9 @@
 // silu, quick_gelu and gelu with tanh are z sigmoid(u), since (1 + tanh(u / 2)) / 2 = sigmoid(u); they take the fast
 // exponential and reciprocal, whose errors are 2^-21 of the value, far below the 2^-12 of an fp16 result.  gelu with erf takes
 // the normal distribution's tail below, to 1e-7.  Factors that stand beside a vanishing one are clamped, so that infinite
-// pre-activations give the limits (0 and z; derivatives 0 and 1; to 2^-50, as sigmoids end at 2^-60) and not 0 * inf; the
-// clamps pass NaN on.
+// pre-activations give the limits (0 and z; derivatives 0 and 1; to 2^-50, as sigmoids end at 2^-60) and not 0 * inf.  A NaN
+// reaches the result through other factors: what goes into a reciprocal, which a pair shares, never holds one (min_num), as it would
+// make the neighbouring column NaN too.
 #pragma once
 #include "bxl_types.cuh"
 
@@ -31,6 +32,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// ... and the number, where `a` is NaN
+__device__ __forceinline__ float min_num(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ float magnitude(float a) { return fabsf(a); }
 __device__ __forceinline__ float if_negative(float z, float a, float b) { return z < 0.f ? a : b; }
 // ... and of pairs, for what has no instruction for two
@@ -42,7 +45,7 @@ __device__ __forceinline__ float if_negative(float z, float a, float b) { return
 BXL_ON_PAIRS(exp2_approx)
 BXL_ON_PAIRS(magnitude)
 #undef BXL_ON_PAIRS
-// Both reciprocals of a pair from that of the product, which must not overflow: one special-function instruction instead of two.
+// Both reciprocals of a pair from that of the product, which must be finite: one special-function instruction instead of two.
 __device__ __forceinline__ F2 rcp_approx(F2 a) {
   const float2 u = split(a);
   const float r = rcp_approx(u.x * u.y);
@@ -51,6 +54,10 @@ __device__ __forceinline__ F2 rcp_approx(F2 a) {
 __device__ __forceinline__ F2 min_nan(F2 a, float b) {
   const float2 u = split(a);
   return f2(min_nan(u.x, b), min_nan(u.y, b));
+}
+__device__ __forceinline__ F2 min_num(F2 a, float b) {
+  const float2 u = split(a);
+  return f2(min_num(u.x, b), min_num(u.y, b));
 }
 __device__ __forceinline__ F2 max_nan(F2 a, float b) {
   const float2 u = split(a);
@@ -61,20 +68,21 @@ __device__ __forceinline__ F2 if_negative(F2 z, F2 a, F2 b) {
   return f2(if_negative(u.x, v.x, w.x), if_negative(u.y, v.y, w.y));
 }
 
-// Phi(-a) of the normal distribution, a >= 0, by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26: with
-// t = 1 / (1 + p y), erfc(y) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-y^2) + error, |error| <= 1.5e-7, at y = a / sqrt(2).
-// One reciprocal and one exponential, which the density takes too (`e` = exp(-a^2 / 2)).
+// Phi(-|z|) of the normal distribution, `a` = |z| up to a bound beyond which it vanishes, by Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26: with t = 1 / (1 + p y), erfc(y) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-y^2) + error,
+// |error| <= 1.5e-7, at y = a / sqrt(2).
+// One reciprocal and one exponential, which the density takes too (`e` = exp(-z^2 / 2)).
 template <class F>
-__device__ __forceinline__ F normal_tail(F a, F& e) {
+__device__ __forceinline__ F normal_tail(F z, F a, F& e) {
   const F t = rcp_approx(fma(splat<F>(0.3275911f * 0.70710678118654752f), a, splat<F>(1.f)));
-  e = exp2_approx(mul(mul(a, a), splat<F>(-0.72134752044448170f)));   // log2(e) / 2
+  e = exp2_approx(mul(mul(z, z), splat<F>(-0.72134752044448170f)));   // log2(e) / 2
   F p = fma(t, splat<F>(0.5f * 1.061405429f), splat<F>(0.5f * -1.453152027f));
   p = fma(t, p, splat<F>(0.5f * 1.421413741f));
   p = fma(t, p, splat<F>(0.5f * -0.284496736f));
   p = fma(t, p, splat<F>(0.5f * 0.254829592f));
   return mul(mul(p, t), e);
 }
-// exp(-u) of sigmoid(u) = 1 / (1 + exp(-u)), at most 2^60, so that the product of two divisors does not overflow
+// exp(-u) of sigmoid(u) = 1 / (1 + exp(-u)), at most 2^60 (and that of a NaN), so that the product of two divisors is finite
 template <int ACT, class F>
 __device__ __forceinline__ F exp_minus_argument(F z) {
   constexpr float kLog2e = 1.4426950408889634f;
@@ -83,7 +91,7 @@ __device__ __forceinline__ F exp_minus_argument(F z) {
   else if constexpr (ACT == BXL_ACT_QUICK_GELU) u = mul(z, splat<F>(-1.702f * kLog2e));
   else  // gelu with tanh: u = 2 sqrt(2 / pi) (z + 0.044715 z^3)
     u = mul(z, fma(mul(z, z), splat<F>(-0.07135481627260025f * kLog2e), splat<F>(-1.5957691216057308f * kLog2e)));
-  return exp2_approx(min_nan(u, 60.f));
+  return exp2_approx(min_num(u, 60.f));
 }
 
 template <int ACT, class F>
@@ -94,9 +102,9 @@ __device__ __forceinline__ F act_value(F z) {
     return max_nan(z, 0.f);
   } else if constexpr (ACT == BXL_ACT_GELU) {
     // z Phi(z) = max(z, 0) - |z| Phi(-|z|): nothing cancels on either side
-    const F a = min_nan(magnitude(z), 1e3f);
+    const F a = min_num(magnitude(z), 1e3f);
     F e;
-    const F q = normal_tail(a, e);
+    const F q = normal_tail(z, a, e);
     return fma(mul(a, splat<F>(-1.f)), q, max_nan(z, 0.f));
   } else {
     return mul(max_nan(z, -1e3f), rcp_approx(add(exp_minus_argument<ACT>(z), splat<F>(1.f))));
@@ -113,9 +121,9 @@ __device__ __forceinline__ F act_slope(F z) {
     return add(zero, if_negative(mul(z, splat<F>(-1.f)), splat<F>(1.f), splat<F>(0.f)));
   } else if constexpr (ACT == BXL_ACT_GELU) {
     // Phi(z) + z phi(z): of s = Phi(-a) - a phi(a) it is s on the left and 1 - s on the right
-    const F a = min_nan(magnitude(z), 1e3f);
+    const F a = min_num(magnitude(z), 1e3f);
     F e;
-    const F q = normal_tail(a, e);
+    const F q = normal_tail(z, a, e);
     const F s = fma(mul(a, splat<F>(-0.3989422804014327f)), e, q);
     return if_negative(z, s, fma(s, splat<F>(-1.f), splat<F>(1.f)));
   } else {

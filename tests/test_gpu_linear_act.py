@@ -215,6 +215,40 @@ def test_infinite_and_missing_values(act, m):
         assert torch.equal(y[2:], ops.linear_act(s["x"], w, None, activation=act)[2:])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,k,n", [(2, 64, 48), (64, 64, 48), (300, 64, 48), (300, 64, 45), (60, 3528, 24), (1000, 64, 512)])
+def test_a_missing_value_stays_in_its_column(m, k, n, act, dtype):
+    """A NaN in one element of the bias, in a row of the weight or in one element of ``pre``: every other column of the results, and
+    every other row of ``dweight``, is what it is without."""
+    cuda_or_skip()
+    _lib, ops = _ops()
+    s = _inputs(m, k, n, dtype)
+    nan, lost = float("nan"), [3, 10, 17]
+    rest = [j for j in range(n) if j not in lost]
+    w, b = s["weight"].clone(), s["bias"].clone()
+    b[3] = b[10] = nan
+    w[17, k // 2] = nan
+    want = _plain.linear(s["x"], s["weight"], s["bias"], act, None)
+    y, pre = ops.linear_act(s["x"], w, b, activation=act, want_pre=True)
+    assert y[:, lost].isnan().all() and pre[:, lost].isnan().all()
+    _plain.within(y[:, rest], want[0][:, rest], want[1][:, rest], "y")
+    _plain.within(pre[:, rest], want[2][:, rest], want[3][:, rest], "pre")
+    if act == "none":   # its backward pass takes no pre
+        return
+    pre = ops.linear_act(s["x"], s["weight"], s["bias"], activation=act, want_pre=True)[1]
+    want = _plain.linear_grad(s["dy"], s["x"], s["weight"], pre, act)
+    bad = pre.clone()
+    bad[0, 3] = bad[m - 1, 10] = bad[0, 17] = nan
+    dx, dw, db = ops.linear_act_bwd(s["dy"], s["x"], s["weight"], bad, act)
+    assert dx[[0, m - 1]].isnan().all() and dw[lost].isnan().all() and db[lost].isnan().all()
+    if m > 2:
+        _plain.within(dx[1 : m - 1], want[0][1 : m - 1], want[1][1 : m - 1], "dx")
+    _plain.within(dw[rest], want[2][rest], want[3][rest], "dweight")
+    _plain.within(db[rest], want[4][rest], want[5][rest], "dbias")
+    _lib.device_status()
+
+
 def test_out_and_neighbours():
     """``out`` may be the residual; nothing behind the last row is written."""
     cuda_or_skip()
