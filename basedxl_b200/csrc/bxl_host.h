@@ -88,9 +88,12 @@ struct LinearProduct {
   int act, bf16, M, N, K;
 };
 // One product, or two (n = 2) that do not depend on one another.  *launches grows by the kernels enqueued.  The workspace's size goes
-// by everything in the products but A and B.
+// by everything in the products but A and B; its address need only be 16-byte aligned.
 long long linear_workspace(const LinearProduct* const* q, int n);
 int linear_products(const LinearProduct* const* q, int n, void* workspace, int* launches, cudaStream_t stream);
+// Partial sums are stored 32 bytes at a time, at a 32-byte boundary of a workspace that is 16-byte aligned and this much larger.
+constexpr long long kPartSlack = 16;
+inline float* part_base(void* workspace) { return reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 31) & ~static_cast<uintptr_t>(31)); }
 // Copies the rows of up to two 16-bit matrices to rows ld_dst (a multiple of 8) apart; dst null = nothing to copy.
 struct RowCopy {
   const void* src;

@@ -1607,13 +1607,13 @@ long long linear_workspace(const LinearProduct* const* q, int n) {
   const LinearPlan& plan = plan_products(q, n);
   long long bytes = 0;
   for (int i = 0; i < n; ++i) bytes += part_bytes(*q[i], plan.slices(i));
-  return bytes;
+  return bytes ? bytes + kPartSlack : 0;
 }
 
 int linear_products(const LinearProduct* const* q, int n, void* workspace, int* launches, cudaStream_t stream) {
   const LinearPlan plan = plan_products(q, n);
   const bool bf16 = q[0]->bf16;
-  float* part[2] = {static_cast<float*>(workspace), static_cast<float*>(workspace)};
+  float* part[2] = {part_base(workspace), part_base(workspace)};
   if (n == 2) part[1] += part_bytes(*q[0], plan.slices(0)) / 4;
   if (plan.together) {
     GemmTwo two;

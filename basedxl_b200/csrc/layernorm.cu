@@ -1038,7 +1038,8 @@ extern "C" int bxl_layernorm_fwd(const void* x, long long ldx, const void* weigh
 
 extern "C" long long bxl_layernorm_bwd_workspace_bytes(long long rows, int C) {
   if (rows <= 0 || C <= 0) return 0;
-  return ln_bwd_blocks(rows) * 2ll * C * (long long)sizeof(float);
+  const long long bytes = ln_bwd_blocks(rows) * 2ll * C * (long long)sizeof(float);
+  return bytes ? bytes + kPartSlack : 0;
 }
 
 extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
@@ -1061,7 +1062,7 @@ extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, 
   }
   LnArgs a = {};
   a.x = x, a.dy = dy, a.y = dx, a.ldx = ldx, a.lddy = lddy, a.ldy = lddx, a.weight = weight;
-  a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.part = params ? static_cast<float*>(workspace) : nullptr;
+  a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.part = params ? part_base(workspace) : nullptr;
   a.rows = rows, a.C = C, a.param_f32 = param_dtype == BXL_F32, a.inv_c = 1.f / (float)C;
   const bool vec = rows_of_vectors(x, ldx, C, b) && rows_of_vectors(dy, lddy, C, b) && rows_of_vectors(dx, lddx, C, b) && al16(weight);
   cudaStream_t s = (cudaStream_t)stream;

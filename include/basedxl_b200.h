@@ -170,7 +170,7 @@ int bxl_gemm_ragged_f16(const void* A, long long lda, const void* B, long long l
  * (written ones apart).  Operands of the tensor cores that the copy engine cannot read (rows not 16-byte aligned) are first
  * copied to the workspace.  dz is rounded to `dtype` between its two products; sums have a fixed order.
  * Written operands overlap nothing else of the call, except that y may be the residual.
- * bxl_linear_act_*_workspace_bytes reads all fields but the workspace.  *launches (or NULL): kernels
+ * bxl_linear_act_*_workspace_bytes reads all fields but the workspace, which is 16-byte aligned.  *launches (or NULL): kernels
  * enqueued.  Few tiles and a long sum are shared among CTAs by parts of it, joined in a fixed order by a second kernel.
  * The forward pass replaces bxl_gemm_f16 and the activation around it; no counterpart of the backward pass in the
  * reference, which only runs inference. */
@@ -354,7 +354,7 @@ int bxl_layernorm_fwd(const void* x, long long ldx, const void* weight, const vo
 /* Its gradients, given those of y: with h = (x - mean) rstd and g = dy weight,
  *   dx = rstd (g - mean(g) - h mean(g h)),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
  * dweight, dbias [C] of type `param_dtype`, either may be NULL; with both NULL, or a workspace of no bytes
- * (few rows, one kernel instead of two), the workspace may be NULL.  The sums are formed in fp32 in a fixed order: the same call gives the same bits.  dx overlaps neither x nor dy. */
+ * (few rows, one kernel instead of two), the workspace may be NULL; else it is 16-byte aligned.  The sums are formed in fp32 in a fixed order: the same call gives the same bits.  dx overlaps neither x nor dy. */
 long long bxl_layernorm_bwd_workspace_bytes(long long rows, int C);
 int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
                       const void* weight, void* dx, long long lddx, void* dweight, void* dbias, long long rows, int C, int dtype,

@@ -135,3 +135,27 @@ def test_two_streams_at_once():
     for i in range(2):
         for once in got[i]:
             assert all(torch.equal(p, q) for p, q in zip(once, want[i]))
+
+
+class _Shifted(_Arena):
+    """The workspace lies 16 bytes behind a 32-byte boundary."""
+
+    def __init__(self, sizes):
+        super().__init__({name: n + 16 if name == "workspace" else n for name, n in sizes.items()})
+        if "workspace" in self.at:
+            self.at["workspace"] = (self.at["workspace"][0] + 16, sizes["workspace"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("m,k,n", LINEAR)
+def test_linear_layers_any_workspace(m, k, n, dtype, monkeypatch):
+    """16-byte alignment is all that the workspace needs."""
+    monkeypatch.setitem(globals(), "_Arena", _Shifted)
+    test_linear_layers(m, k, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("rows,c", NORM + [(530, 8192), (530, 12288), (530, 6152)])
+def test_layernorm_any_workspace(rows, c, dtype, monkeypatch):
+    monkeypatch.setitem(globals(), "_Arena", _Shifted)
+    test_layernorm(rows, c, dtype)

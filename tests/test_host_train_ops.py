@@ -202,3 +202,12 @@ def test_c_linear_act_bwd_refuses(kw):
 def test_workspace_of_the_forward_pass(kw, nbytes):
     """Copies only of operands whose rows are not 16-byte aligned, and none for a few rows."""
     assert _lib.load().bxl_linear_act_fwd_workspace_bytes(_linear(**kw)) == nbytes
+
+
+def test_workspace_leaves_room_to_align():
+    """Partial sums are stored 32 bytes at a time: 16 bytes more than they take, for a 32-byte boundary in a workspace that is 16-byte aligned."""
+    l = _lib.load()
+    sliced = l.bxl_linear_act_fwd_workspace_bytes(_linear(M=60, N=24, K=3528, ldx=3528, ldw=3528, ldy=24))
+    assert sliced > 60 * 32 * 4 * 2 and sliced % 32 == 16
+    sums = l.bxl_layernorm_bwd_workspace_bytes(600, 8192)
+    assert sums > 2 * 8192 * 4 and sums % 32 == 16 and l.bxl_layernorm_bwd_workspace_bytes(5, 8192) == 0
