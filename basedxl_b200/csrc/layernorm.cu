@@ -289,10 +289,12 @@ __device__ __forceinline__ bool team_sum(float (&v)[K], const LnTeams& t, const 
   add_lanes<K>(v, 1);
   return failed;
 }
-// s / C, exact where the quotient is (equal values have that value as their mean): a product and one correction.
+// s / C, exact where the quotient is (equal values have that value as their mean): a product and one correction, which an infinite sum
+// does without.
 __device__ __forceinline__ float mean_of(float s, const LnArgs& a) {
   const float m = s * a.inv_c;
-  return fmaf(fmaf(-m, static_cast<float>(a.C), s), a.inv_c, m);
+  const float exact = fmaf(fmaf(-m, static_cast<float>(a.C), s), a.inv_c, m);
+  return fabsf(m) < INFINITY ? exact : m;
 }
 // A vector of fp32 parameters in shared memory: quarters of 16 bytes of neighbouring vectors lie side by side (two
 // planes for VEC = 8), so that a warp's reads meet no bank twice.

@@ -311,3 +311,24 @@ def _plain_grad(x, w, b, dy):
     leaves = [t.double().requires_grad_() for t in (x, w, b)]
     y = torch.nn.functional.layer_norm(leaves[0], w.shape, leaves[1], leaves[2], EPS)
     return torch.autograd.grad(y, leaves, dy.double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("rows,c", [(20, 320), (4001, 320), (801, 1608), (1701, 643), (60011, 640), (513, 20000)])
+def test_mean_of_infinite_rows(rows, c, dtype):
+    """The mean of a row is infinite where its sum is, for few rows and for many; its other results are NaN, other rows as they were."""
+    cuda_or_skip()
+    _lib, ops = _ops()
+    x, w, b, _ = _inputs(rows, c, dtype)
+    clean = ops.layernorm_fwd(x, w, b, EPS, want_stats=True)
+    x = x.clone()
+    inf = float("inf")
+    x[3, 5], x[7, 0], x[rows - 1, c - 1], x[9, 1], x[9, 2] = inf, -inf, inf, inf, -inf
+    y, mean, rstd = ops.layernorm_fwd(x, w, b, EPS, want_stats=True)
+    assert mean[3] == inf and mean[7] == -inf and mean[rows - 1] == inf and mean[9].isnan()
+    hit = [3, 7, 9, rows - 1]
+    assert y[hit].isnan().all() and rstd[hit].isnan().all()
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[hit] = False
+    assert all(torch.equal(p[rest], q[rest]) for p, q in zip((y, mean, rstd), clean))
+    _lib.device_status()
