@@ -353,7 +353,7 @@ __device__ __forceinline__ void load_bias(const GemmParams& p, int nb, BiasChunk
   const T* from = reinterpret_cast<const T*>(p.bias) + nb;
   if (p.bias_vec && nb + 32 <= p.N) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) b.u[q] = __ldg(reinterpret_cast<const uint4*>(from) + q);
+    for (int q = 0; q < 4; ++q) b.u[q] = reinterpret_cast<const uint4*>(from)[q];
   } else {
     uint32_t w[16];
 #pragma unroll
@@ -1296,6 +1296,8 @@ struct RepackOperand {
   long long ld, ld_dst; // elements
   int rows, cols;
 };
+// (Plain loads: the read-only path is for what nothing writes while the kernel's blocks run, and they already do while the preceding
+// kernel writes its results.)
 __device__ __forceinline__ void repack_vector(const RepackOperand& o, long long i) {
   const int vecs = static_cast<int>(o.ld_dst / 8);
   const long long r = i / vecs;
@@ -1308,10 +1310,10 @@ __device__ __forceinline__ void repack_vector(const RepackOperand& o, long long 
     if ((reinterpret_cast<uintptr_t>(s) & 2u) == 0) {
       const uint32_t* q = reinterpret_cast<const uint32_t*>(s);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = __ldg(q + j);
+      for (int j = 0; j < 4; ++j) w[j] = q[j];
     } else {
       const uint32_t* q = reinterpret_cast<const uint32_t*>(s + 1);
-      const uint32_t a = __ldg(s), b = __ldg(q), e = __ldg(q + 1), f = __ldg(q + 2), g = __ldg(s + 7);
+      const uint32_t a = s[0], b = q[0], e = q[1], f = q[2], g = s[7];
       w[0] = a | (b << 16), w[1] = __funnelshift_r(b, e, 16), w[2] = __funnelshift_r(e, f, 16), w[3] = (f >> 16) | (g << 16);
     }
     *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);

@@ -85,7 +85,9 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32) few_rows_kernel(const FewRo
       for (int j = 0; j < 8; ++j) {
         const int k = i * 32 + 4 * j + q;
         u.v[j] = 0;
-        if (decltype(all)::value || k < p.K) asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(u.v[j]) : "l"(row + k));   // volatile: all of them before the first use
+        // volatile: all of them before the first use.  (Not the read-only path: the preceding kernel may write x and W while this one's
+        // blocks already wait for it.)
+        if (decltype(all)::value || k < p.K) asm volatile("ld.global.u16 %0, [%1];" : "=h"(u.v[j]) : "l"(row + k));
       }
       return u;
     }

@@ -249,6 +249,31 @@ def test_a_missing_value_stays_in_its_column(m, k, n, act, dtype):
     _lib.device_status()
 
 
+@pytest.mark.parametrize("m,k,n", [(4, 1003, 2400), (8, 640, 2400), (8, 65, 1280), (40, 1003, 640), (40, 640, 640)])
+def test_inputs_of_the_kernel_before(m, k, n):
+    """Rows and bias that the calls right before have written, over values that an earlier call of the same layer has read."""
+    cuda_or_skip()
+    _, ops = _ops()
+    w, wb = _inputs(m, k, n, torch.float16)["weight"], _inputs(1, k, n, torch.float16, 7)["weight"]
+    xs = [_inputs(m, k, n, torch.float16, seed)["x"] for seed in range(20)]
+    want = []
+    for x in xs:
+        y = ops.layernorm_fwd(x)
+        b = ops.linear_act(x[0], wb)
+        torch.cuda.synchronize()
+        want.append(ops.linear_act(y, w, b, activation="silu"))
+        torch.cuda.synchronize()
+    x, b, got = torch.empty_like(xs[0]), torch.empty(n, device="cuda", dtype=torch.float16), []
+    for _ in range(5):
+        for v in xs:
+            x.copy_(v)
+            ops.linear_act(x, w, b, activation="silu")
+            ops.linear_act(x[0], wb, out=b)
+            ops.layernorm_fwd(x, out=x)
+            got.append(ops.linear_act(x, w, b, activation="silu"))
+    assert all(torch.equal(p, q) for p, q in zip(got, want * 5))
+
+
 def test_out_and_neighbours():
     """``out`` may be the residual; nothing behind the last row is written."""
     cuda_or_skip()
