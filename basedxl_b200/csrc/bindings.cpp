@@ -99,6 +99,12 @@ void apart(const char* who, const Tensor& out, const char* what, const Tensor* o
   TORCH_CHECK_VALUE(may_be_it && a == b && other->is_contiguous(), who, ": out overlaps ", what);
 }
 
+// A tensor that has been written to counts as changed: its new version is by what autograd and this package's caches (K/V of the
+// conditioning, packed weights) see it.
+void written(const Tensor& out) {
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // The library, set up for the current device (through _lib.lib(), once per device).
 void ensure_device(int dev) {
   static bool ready[64] = {};
@@ -184,6 +190,7 @@ PyObject* layernorm_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     finish(bxl_layernorm_fwd(r.p, r.ld, w.ptr(), b.ptr(), y.mutable_data_ptr(), c, stats ? mean.mutable_data_ptr<float>() : nullptr,
                              stats ? rstd.mutable_data_ptr<float>() : nullptr, rows, (int)c, dt, pt, (float)eps, c10::cuda::getCurrentCUDAStream().stream()),
            1);
+    if (into) written(y);
   }
   return stats ? wrap3(y, mean, rstd) : wrap(y);
   END_HANDLE_TH_ERRORS
@@ -282,6 +289,7 @@ PyObject* linear_act(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int launches = 0;
     const int rc = bxl_linear_act_fwd(&a, &launches, c10::cuda::getCurrentCUDAStream().stream());
     finish(rc, launches);
+    if (into) written(y);
   }
   if (!want_pre) return wrap(y);
   PyObject* r = PyTuple_New(2);

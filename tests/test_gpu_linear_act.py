@@ -410,3 +410,34 @@ def test_mixed_devices_are_refused():
 
 def out_of(x):
     return torch.zeros(x.shape[0], 6, dtype=x.dtype)
+
+
+def test_out_has_a_new_version():
+    """What is written into ``out`` counts as a change: autograd refuses a graph that needs the values before, and cross-attention projects
+    its conditioning again."""
+    cuda_or_skip()
+    _, ops = _ops()
+    from basedxl_b200.layers import Attention
+
+    x, w = _inputs(77, 64, 64, torch.float16)["x"][None], _inputs(1, 64, 64, torch.float16, 3)["weight"]
+    calls = (lambda out: ops.layernorm_fwd(x, out=out), lambda out: ops.linear_act(x, w, out=out))
+    for call in calls:
+        out = x.clone()
+        leaf = torch.ones_like(out).requires_grad_()
+        product = leaf * out
+        call(out)
+        assert out._version == 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+        with torch.inference_mode():
+            call(torch.empty_like(x))
+    assert ops.layernorm_fwd(x[:, :0], out=torch.empty_like(x)[:, :0])._version == 0
+
+    layer = Attention(128, 2, 64).half().cuda()   # its context is 64 wide
+    for call in calls:
+        ctx = x.clone()
+        with torch.no_grad():
+            first = layer.context_kv(ctx).clone()
+            call(ctx)
+            kv = layer.context_kv(ctx).clone()
+            assert not torch.equal(kv, first) and torch.equal(kv, layer.context_kv(ctx.clone()))
