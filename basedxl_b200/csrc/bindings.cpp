@@ -10,6 +10,7 @@
 #include <string>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -99,6 +100,11 @@ void apart(const char* who, const Tensor& out, const char* what, const Tensor* o
   TORCH_CHECK_VALUE(may_be_it && a == b && other->is_contiguous(), who, ": out overlaps ", what);
 }
 
+// As PyTorch's own functions: what is written to it would be missing from the graph that autograd records.
+void writable(const char* who, const Tensor& out) {
+  TORCH_CHECK_VALUE(out.is_contiguous(), who, ": out must be contiguous");
+  TORCH_CHECK_VALUE(!(out.requires_grad() && at::GradMode::is_enabled()), who, ": out requires a gradient, which is not recorded here");
+}
 // A tensor that has been written to counts as changed: its new version is by what autograd and this package's caches (K/V of the
 // conditioning, packed weights) see it.
 void written(const Tensor& out) {
@@ -173,7 +179,7 @@ PyObject* layernorm_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   TORCH_CHECK_VALUE(!w || !b || w->scalar_type() == b->scalar_type(), who, ": weight and bias must share a type");
   if (into) {
     same(who, "out", *into.t, x.sizes(), type);
-    TORCH_CHECK_VALUE(into->is_contiguous(), who, ": out must be contiguous");
+    writable(who, *into.t);
     apart(who, *into.t, "x", &x, true), apart(who, *into.t, "weight", w.t, false), apart(who, *into.t, "bias", b.t, false);
   }
   same_device(who, {w.t, b.t, into.t}, x);
@@ -264,7 +270,7 @@ PyObject* linear_act(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (res) same(who, "residual", *res.t, sizes, type);
   if (into) {
     same(who, "out", *into.t, sizes, type);
-    TORCH_CHECK_VALUE(into->is_contiguous(), who, ": out must be contiguous");
+    writable(who, *into.t);
     apart(who, *into.t, "x", &x, false), apart(who, *into.t, "weight", &w, false), apart(who, *into.t, "bias", b.t, false), apart(who, *into.t, "residual", res.t, true);
   }
   same_device(who, {&w, b.t, res.t, into.t}, x);

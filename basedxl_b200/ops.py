@@ -264,7 +264,8 @@ def _activation(name, activation) -> int:
 
 def linear_act(x, weight, bias=None, activation=None, residual=None, out=None, want_pre: bool = False):
     """``act(x[..., K] @ weight[N, K]^T + bias) + residual`` in one product, fp16 or bf16, any extents; ``activation`` is one of
-    ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``, and overlaps no other input) receives the result.
+    ``ACTIVATIONS``.  ``out`` (contiguous; it may be ``residual``, and overlaps no other input) receives the result.  Nothing is
+    recorded for autograd.
     ``want_pre`` also returns the value before the activation, rounded to the type of ``x``: the input of
     :func:`linear_act_bwd`."""
     return _lib.native().linear_act(x, weight, bias, _activation("linear_act", activation), residual, out, bool(want_pre))
@@ -489,7 +490,7 @@ def layernorm(x, gamma, beta, eps):
 def layernorm_fwd(x, weight=None, bias=None, eps: float = 1e-5, out=None, want_stats: bool = False):
     """LayerNorm over the last axis of ``x`` (fp16, bf16 or fp32, any width); ``weight`` and ``bias`` in its type or in
     fp32, either may be absent.  ``out`` (which may be ``x``) receives the result.  ``want_stats`` also returns the
-    rows' fp32 ``mean`` and ``rstd``, the input of :func:`layernorm_bwd`."""
+    rows' fp32 ``mean`` and ``rstd``, the input of :func:`layernorm_bwd`.  Nothing is recorded for autograd."""
     return _lib.native().layernorm_fwd(x, weight, bias, eps, out, bool(want_stats))
 
 

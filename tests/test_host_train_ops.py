@@ -211,3 +211,13 @@ def test_workspace_leaves_room_to_align():
     assert sliced > 60 * 32 * 4 * 2 and sliced % 32 == 16
     sums = l.bxl_layernorm_bwd_workspace_bytes(600, 8192)
     assert sums > 2 * 8192 * 4 and sums % 32 == 16 and l.bxl_layernorm_bwd_workspace_bytes(5, 8192) == 0
+
+
+def test_out_that_requires_a_gradient_is_refused():
+    """As PyTorch refuses it: what is written would be missing from the graph.  Without grad mode there is none."""
+    for call in (lambda out: ops.layernorm_fwd(_z(5, 8), out=out), lambda out: ops.linear_act(_z(5, 4), _z(8, 4), out=out)):
+        leaf = _z(5, 8).requires_grad_()
+        assert "out requires a gradient" in _refused(call, out=leaf) and "out requires a gradient" in _refused(call, out=leaf * 2)
+        with torch.no_grad():
+            assert HOST in _refused(call, out=leaf)
+        assert HOST in _refused(call, out=leaf.detach())
