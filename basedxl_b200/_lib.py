@@ -83,6 +83,7 @@ SIGNATURES = {
     "bxl_layernorm_fwd": (_i, [_vp, _ll, _vp, _vp, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _f, _vp]),
     "bxl_layernorm_bwd_workspace_bytes": (_ll, [_ll, _i]),
     "bxl_layernorm_bwd": (_i, [_vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _vp, _ll, _vp]),
+    "bxl_layernorm_bwd_launches": (_i, []),
     "bxl_geglu_f16": (_i, [_vp, _vp, _ll, _i, _vp]),
     "bxl_cfg_euler_step": (_i, [_vp, _vp, _vp, _ll, _f, _f, _f, _vp]),
 }

@@ -227,10 +227,10 @@ PyObject* layernorm_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const Rows rd(dy), rx(x);
     const int64_t bytes = want_dw || want_db ? bxl_layernorm_bwd_workspace_bytes(rows, (int)c) : 0;
     const Tensor ws = bytes ? empty({bytes}, at::kByte, x.device()) : Tensor();
-    finish(bxl_layernorm_bwd(rd.p, rd.ld, rx.p, rx.ld, mean.const_data_ptr<float>(), rstd.const_data_ptr<float>(), w.ptr(), dx.mutable_data_ptr(), c,
-                             want_dw ? dw.mutable_data_ptr() : nullptr, want_db ? db.mutable_data_ptr() : nullptr, rows, (int)c, type_of(type), type_of(param),
-                             bytes ? ws.mutable_data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream().stream()),
-           bytes ? 2 : 1);
+    const int rc = bxl_layernorm_bwd(rd.p, rd.ld, rx.p, rx.ld, mean.const_data_ptr<float>(), rstd.const_data_ptr<float>(), w.ptr(), dx.mutable_data_ptr(), c,
+                                     want_dw ? dw.mutable_data_ptr() : nullptr, want_db ? db.mutable_data_ptr() : nullptr, rows, (int)c, type_of(type), type_of(param),
+                                     bytes ? ws.mutable_data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream().stream());
+    finish(rc, bxl_layernorm_bwd_launches());
   } else {
     if (want_dw) dw.zero_();
     if (want_db) db.zero_();

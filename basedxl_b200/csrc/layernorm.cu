@@ -992,6 +992,7 @@ static int ln_bwd_small(const LnArgs& a, bool vec, void* dweight, void* dbias, c
   if (vec) return launch_kernel("ln_bwd_small_kernel launch", ln_bwd_small_kernel<T, P, V>, grid, dim3(kSmallThreads), 0, s, 1, a, dw, db);
   return launch_kernel("ln_bwd_small_kernel launch", ln_bwd_small_kernel<T, P, 1>, grid, dim3(kSmallThreads), 0, s, 1, a, dw, db);
 }
+static thread_local int g_bwd_launches = 0;
 template <class T>
 static int ln_bwd(const LnArgs& a, bool vec, int& blocks, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
@@ -1004,6 +1005,7 @@ static int ln_bwd(const LnArgs& a, bool vec, int& blocks, cudaStream_t s) {
   if (!a.part) return kOk;
   const long long shares = a.rows < 64 ? a.rows : 64;
   blocks = (int)shares;
+  ++g_bwd_launches;
   return launch_kernel("ln_bwd_columns_kernel launch", ln_bwd_columns_kernel<T>, dim3((a.C + 255) / 256, (unsigned)shares), dim3(256), 0, s, 1, a);
 }
 
@@ -1044,6 +1046,8 @@ extern "C" long long bxl_layernorm_bwd_workspace_bytes(long long rows, int C) {
   return bytes ? bytes + kPartSlack : 0;
 }
 
+extern "C" int bxl_layernorm_bwd_launches(void) { return g_bwd_launches; }
+
 extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
                                  const void* weight, void* dx, long long lddx, void* dweight, void* dbias, long long rows, int C, int dtype,
                                  int param_dtype, void* workspace, long long workspace_bytes, void* stream) {
@@ -1068,6 +1072,7 @@ extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, 
   a.rows = rows, a.C = C, a.param_f32 = param_dtype == BXL_F32, a.inv_c = 1.f / (float)C;
   const bool vec = rows_of_vectors(x, ldx, C, b) && rows_of_vectors(dy, lddy, C, b) && rows_of_vectors(dx, lddx, C, b) && al16(weight);
   cudaStream_t s = (cudaStream_t)stream;
+  g_bwd_launches = 1;
   if (!ln_bwd_blocks(rows)) {
     a.part = nullptr;
     if (dtype == BXL_F32) return ln_bwd_small<float, float>(a, vec, dweight, dbias, s);
@@ -1079,5 +1084,6 @@ extern "C" int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, 
   else if (dtype == BXL_BF16) rc = ln_bwd<__nv_bfloat16>(a, vec, blocks, s);
   else rc = ln_bwd<float>(a, vec, blocks, s);
   if (rc || !params) return rc;
+  ++g_bwd_launches;
   return sum_partials(a.part, blocks, 2ll * C, C, dweight, dbias, param_dtype, s);
 }

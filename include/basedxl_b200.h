@@ -359,6 +359,8 @@ long long bxl_layernorm_bwd_workspace_bytes(long long rows, int C);
 int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
                       const void* weight, void* dx, long long lddx, void* dweight, void* dbias, long long rows, int C, int dtype,
                       int param_dtype, void* workspace, long long workspace_bytes, void* stream);
+/* Kernels that the calling thread's last successful bxl_layernorm_bwd has enqueued (one to three). */
+int bxl_layernorm_bwd_launches(void);
 /* out[rows,F] = h[:, :F] * gelu(h[:, F:]) for h[rows,2F] (exact erf GELU). */
 int bxl_geglu_f16(const void* h, void* out, long long rows, int F, void* stream);
 

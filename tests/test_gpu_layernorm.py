@@ -332,3 +332,18 @@ def test_mean_of_infinite_rows(rows, c, dtype):
     rest[hit] = False
     assert all(torch.equal(p[rest], q[rest]) for p, q in zip((y, mean, rstd), clean))
     _lib.device_status()
+
+
+@pytest.mark.parametrize("rows,c,apart,kernels", [(5, 97, True, 1), (600, 97, True, 3), (600, 96, False, 2), (600, 20000, False, 3), (513, 11600, False, 3)])
+def test_counted_launches(rows, c, apart, kernels):
+    """One kernel for few rows, two with the column sums, three where the rows have no ring; one without column sums."""
+    cuda_or_skip()
+    _lib, ops = _ops()
+    x = torch.randn(rows, c + 3, device="cuda")[:, 1 : c + 1]
+    x = x if apart else x.contiguous()
+    w = torch.ones(c, device="cuda")
+    _, mean, rstd = ops.layernorm_fwd(x, w, want_stats=True)
+    for want, n in (({}, kernels), ({"want_dbias": False}, kernels), ({"want_dweight": False, "want_dbias": False}, 1)):
+        before = _lib.launches
+        ops.layernorm_bwd(x, x, mean, rstd, w, **want)
+        assert _lib.launches - before == n
