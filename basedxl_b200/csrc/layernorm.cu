@@ -790,9 +790,10 @@ static bool back_to_back(const void* base, long long ld, int C) { return al16(ba
 
 constexpr long long kSmemSm = 227 * 1024, kSmemHalf = kSmemSm / 2 - 1024;   // of an SM; a block's where two share one
 // Fills `t` for rows of `mats` matrices and threads of at most `most` vectors (`most_sub` in teams of up to a warp); false where rows of this size do not fit.
-// `params`: bytes of shared memory for the parameters; `sums`: whether the block's column sums meet in the rings at the end;
+// `grouped`: up to how many vectors a thread there are kernels that take several rows of a team as one unit (others would leave out all
+// but the first).  `params`: bytes of shared memory for the parameters; `sums`: whether the block's column sums meet in the rings at the end;
 // `room`: shared memory of a block.  NV of the kernel: t.nv.
-static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats, int most_sub, int most, long long params, bool sums, long long room, int& nv,
+static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats, int most_sub, int most, int grouped, long long params, bool sums, long long room, int& nv,
                        int& smem) {
   const long long row = a.C * (long long)elem, n = a.C / vec;
   if (a.rows > INT_MAX) return false;
@@ -812,7 +813,7 @@ static bool plan_teams(LnTeams& t, const LnArgs& a, int elem, int vec, int mats,
   // 64 93.5 -> 80.7 us, 100000 x 640 80.0 -> 77.6; fp32 and rows that are not 16-byte aligned gain nothing (65536 x 320 fp32 29.7, 32.3).
   t.TL = TL, t.per = TL < 32 ? 32 / TL : 1, t.groups = 1;
   const long long grid_teams = (long long)teams * sm_count() * (room < kSmemSm ? 2 : 1);
-  while (elem == 2 && vec > 1 && TL <= 32 && t.groups < 8 && stages_of(2ll * t.groups * t.per) >= (mats == 1 ? 3 : 2) &&
+  while (elem == 2 && vec > 1 && TL <= 32 && nv <= grouped && t.groups < 8 && stages_of(2ll * t.groups * t.per) >= (mats == 1 ? 3 : 2) &&
          a.rows >= 6 * grid_teams * 2 * t.groups * t.per)
     t.groups *= 2;
   t.rows = t.per * t.groups, t.units = (uint32_t)((a.rows + t.rows - 1) / t.rows);
@@ -837,10 +838,11 @@ static int team_blocks(const LnTeams& t, int per_sm) {
 // Vectors a thread holds in teams of up to a warp (eight of 16-bit values spill there: 2048 columns 52.4 us, with seven 46.6).
 template <int VEC>
 constexpr int fwd_most_sub() { return VEC == 1 ? 24 : VEC == 8 ? 7 : 6; }
+constexpr int kFwdGrouped = 5;   // (three stages of two wider rows each do not fit)
 template <class T, int VEC, int NV, int kTeams = kWide>
 static int ln_fwd_teams_launch(const LnArgs& a, const LnTeams& t, int smem, cudaStream_t s) {
   if constexpr (kTeams == kWide && NV <= fwd_most_sub<VEC>()) {
-    if constexpr (sizeof(T) == 2 && VEC > 1 && NV <= 5)   // (three stages of two wider rows each do not fit)
+    if constexpr (sizeof(T) == 2 && VEC > 1 && NV <= kFwdGrouped)
       if (t.groups > 1) return ln_fwd_teams_launch<T, VEC, NV, kGrouped>(a, t, smem, s);
     if (t.TL <= 32) return ln_fwd_teams_launch<T, VEC, NV, kNarrow>(a, t, smem, s);
   }
@@ -860,7 +862,7 @@ static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
   const long long params = VEC == 4 ? 0 : 8ll * a.C;
   // Single values: up to 24 a thread where every team has eight units or more, else 12 for more teams (100000 x 643 fp16 104 us with 12,
   // 88 with 24; 4099 x 1285 fp32 12.4 and 13.8), or what the widest rows need (5000 x 12001: without a ring 234 us, 88 so).
-  auto plan = [&](int narrow, int wider, long long room) { return plan_teams(t, a, sizeof(T), VEC, 1, narrow, wider, params, false, room, nv, smem); };
+  auto plan = [&](int narrow, int wider, long long room) { return plan_teams(t, a, sizeof(T), VEC, 1, narrow, wider, kFwdGrouped, params, false, room, nv, smem); };
   int narrow = sub, wider = most;
   done = (VEC > 1 || close) && plan(narrow, wider, kSmemSm);
   if (VEC == 1 && done && t.units < 8ll * sm_count() * (t.TL > 32 ? kTeamThreads / t.TL : kTeamWarps)) {
@@ -868,7 +870,7 @@ static int ln_fwd_teams(const LnArgs& a, bool& done, cudaStream_t s) {
     if (!plan(narrow, wider, kSmemSm)) narrow = wider = sub, plan(narrow, wider, kSmemSm);
   }
   if (VEC == 4 && !done) wider = wide, done = plan(narrow, wider, kSmemSm);
-  if (done && nv * VEC <= 8) plan(narrow, wider, kSmemHalf);   // two blocks an SM
+  if (done && nv * VEC <= 8 && !plan(narrow, wider, kSmemHalf)) plan(narrow, wider, kSmemSm);   // two blocks an SM
   if (!done) return kOk;
   t.one_copy = close || t.rows == 1;
   if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_fwd: no device status word");
@@ -950,8 +952,8 @@ static int ln_bwd_teams(const LnArgs& a, bool& done, int& blocks, cudaStream_t s
   int nv = 0, smem = 0;
   const bool close = back_to_back(a.x, a.ldx, a.C) && back_to_back(a.dy, a.lddy, a.C);
   constexpr int most = bwd_most<T, VEC>(), wide = VEC == 1 ? 24 : VEC == 8 ? 4 : 6;
-  done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
-                                         plan_teams(t, a, sizeof(T), VEC, 2, most, wide, 4ll * a.C, true, kSmemSm, nv, smem));
+  done = (VEC > 1 || close) && (plan_teams(t, a, sizeof(T), VEC, 2, most, most, most, 4ll * a.C, true, kSmemSm, nv, smem) ||
+                                         plan_teams(t, a, sizeof(T), VEC, 2, most, wide, most, 4ll * a.C, true, kSmemSm, nv, smem));
   if (!done) return kOk;
   t.one_copy = close || t.rows == 1;
   if (!(t.dev_status = device_status_ptr())) return fail(kErrCuda, "bxl_layernorm_bwd: no device status word");

@@ -347,3 +347,10 @@ def test_counted_launches(rows, c, apart, kernels):
         before = _lib.launches
         ops.layernorm_bwd(x, x, mean, rstd, w, **want)
         assert _lib.launches - before == n
+
+
+@pytest.mark.parametrize("rows,c", [(30011, 1280), (30011, 1408), (30011, 1792)])
+def test_many_rows_of_five_to_seven_vectors(rows, c):
+    """Enough rows for units of several, at the widths up to which a warp's threads hold a row."""
+    cuda_or_skip()
+    _check(*_inputs(rows, c, torch.float16))
