@@ -778,10 +778,11 @@ static int allow_smem(int bytes) {
   return kOk;
 }
 constexpr int kLnMaxC = 1 << 30;   // column indices, and a step past the last one, are ints
-// Blocks of the backward pass, at most: each leaves one row of column sums.
+// Rows of column sums that the backward pass leaves, at most: one per block of the teams (one an SM), or per share of ln_bwd_columns_kernel.
+constexpr int kColumnShares = 64;
 static long long ln_bwd_blocks(long long rows) {
   if (rows <= kSmallRows) return 0;
-  const long long most = sm_count() * 2ll;
+  const long long most = sm_count() > kColumnShares ? sm_count() : kColumnShares;
   return rows < most ? rows : most;
 }
 
@@ -1005,7 +1006,7 @@ static int ln_bwd(const LnArgs& a, bool vec, int& blocks, cudaStream_t s) {
   if (int rc = launch_kernel("ln_bwd_long_kernel launch", ln_bwd_long_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(1024), 0, s, 1, a))
     return rc;
   if (!a.part) return kOk;
-  const long long shares = a.rows < 64 ? a.rows : 64;
+  const long long shares = a.rows < kColumnShares ? a.rows : kColumnShares;
   blocks = (int)shares;
   ++g_bwd_launches;
   return launch_kernel("ln_bwd_columns_kernel launch", ln_bwd_columns_kernel<T>, dim3((a.C + 255) / 256, (unsigned)shares), dim3(256), 0, s, 1, a);

@@ -221,3 +221,11 @@ def test_out_that_requires_a_gradient_is_refused():
         with torch.no_grad():
             assert HOST in _refused(call, out=leaf)
         assert HOST in _refused(call, out=leaf.detach())
+
+
+def test_workspace_of_the_backward_norm():
+    """One row of sums for each of at most 148 blocks (the SMs of the device; the library counts 148 without one)."""
+    l = _lib.load()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148
+    for rows in (513, 4096, 1 << 40):
+        assert l.bxl_layernorm_bwd_workspace_bytes(rows, 640) == sms * 2 * 640 * 4 + 16
