@@ -1569,10 +1569,10 @@ static LinearPlan make_plan(const LinearProduct* const* q, int n) {
   }
   return plan;
 }
-// A plan goes by extents, layouts and alignment alone and takes 2 to 4 us to make: the last ones of this thread are kept, under all
-// that they go by.
+// A plan goes by extents, layouts and alignment, and by the device (its SMs, the clusters that it holds at a time), and takes 2 to 4 us
+// to make: the last ones of this thread are kept, under all that they go by.
 struct PlanKey {
-  int v[2][5], n, sms, bn, split, pair;
+  int v[2][5], n, device, bn, split, pair;
   bool operator==(const PlanKey& o) const { return memcmp(this, &o, sizeof(o)) == 0; }
 };
 static const LinearPlan& plan_products(const LinearProduct* const* q, int n) {
@@ -1583,7 +1583,8 @@ static const LinearPlan& plan_products(const LinearProduct* const* q, int n) {
     const int v[5] = {q[i]->M, q[i]->N, q[i]->K, q[i]->b_kn, (linear_ragged(*q[i]) ? 1 : 0) + (q[i]->residual ? 2 : 0)};
     for (int j = 0; j < 5; ++j) key.v[i][j] = v[j], hash = hash * 31u + (unsigned)v[j];
   }
-  key.n = n, key.sms = sm_count(), key.bn = g_force_bn, key.split = g_force_split, key.pair = g_force_pair;
+  if (cudaGetDevice(&key.device) != cudaSuccess) key.device = -1;
+  key.n = n, key.bn = g_force_bn, key.split = g_force_split, key.pair = g_force_pair;
   struct Entry {
     PlanKey key;
     LinearPlan plan;
