@@ -2,8 +2,10 @@
 // a time.
 //
 // silu, quick_gelu and gelu with tanh are z sigmoid(u), since (1 + tanh(u / 2)) / 2 = sigmoid(u); they take the fast
-// exponential and reciprocal, whose errors are 2^-21 of the value, far below the 2^-12 of an fp16 result.  gelu with erf takes
-// the normal distribution's tail below, to 1e-7.  Factors that stand beside a vanishing one are clamped, so that infinite
+// exponential (2^-22 of its value) and reciprocal (2^-23).  With the roundings of 1 + exp(-u) and of the pair's products (4 2^-24) that is at
+// most 2^-20 of the value, and |u| 2^-22 more on the left, where the value follows exp(u): the argument is rounded up to four times.
+// At the clamp, |u| = 41.6, it comes to 2^-16.6; half a step of an fp16 result is 2^-11.  Beyond, the bound is absolute, as is that of
+// gelu with erf, which takes the normal distribution's tail below: |z| 1e-7.  Factors that stand beside a vanishing one are clamped, so that infinite
 // pre-activations give the limits (0 and z; derivatives 0 and 1; to 2^-50, as sigmoids end at 2^-60) and not 0 * inf.  A NaN
 // reaches the result through other factors: what goes into a reciprocal, which a pair shares, never holds one (min_num), as it would
 // make the neighbouring column NaN too.

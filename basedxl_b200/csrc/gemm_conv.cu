@@ -1412,9 +1412,10 @@ static bool linear_ragged(const LinearProduct& q) {
   return q.N % 8 || !rows16(q.C, q.ldc) || (q.residual && (!rows16(q.residual, q.ldr) || q.ldr < q.N)) || (q.pre && !rows16(q.pre, q.ldp));
 }
 static int linear_extra(const LinearProduct& q, int split = 1) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(q.residual && split == 1); }
-// The choice of tiles does not look at the residual or the value before the activation: with them and without, the sums have the same
-// order and the result the same bits.  (A residual's buffers leave at least three stages.)  As epilogues go all of these are heavy: 64 x
-// 2304 x 128 10.1 us when products without either counted as light, 8.0 so.
+// The choice of tiles does not look at a residual of aligned rows or the value before the activation: with them and without, the sums
+// have the same order and the result the same bits.  A residual (rows that repeat, overlap or are not 16-byte aligned) or a `pre`
+// that makes the product ragged takes that variant's tiles, and may give others.  (A residual's buffers leave at least three stages.)
+// As epilogues go all of these are heavy: 64 x 2304 x 128 10.1 us when products without either counted as light, 8.0 so.
 static int planned_extra(const LinearProduct& q) { return linear_ragged(q) ? ragged_bytes(1) : out_bytes(false); }
 static int tiles_along(int n, int of) { return (int)(((long long)n + of - 1) / of); }
 static TileConfig linear_tiles(const LinearProduct& q) {

@@ -132,6 +132,9 @@ static int few_rows(const FewRows& p, bool vec, cudaStream_t s) {
 
 // ---- backward: dz and its column sums ----------------------------------------------------------
 // Block (x, y): 32 * VEC columns, the y-th share of the rows, a row per warp.  Sums are taken of dz before it is rounded.
+// dz is rounded to the operands' type, as PyTorch does between its own operators: the tensor cores multiply 16-bit values.  dx and dW are
+// off by 1.4 times as much as with a dz kept in 32 bits (bf16 2.3e-3 for 1.7e-3 of their norm, fp16 2.9e-4 for 2.1e-4), half of
+// it the rounding of the results themselves; dz in two 16-bit parts would double the work of both products.
 struct DzArgs {
   const void *dy, *pre;
   void* dz;                 // null: not stored

@@ -354,7 +354,8 @@ int bxl_layernorm_fwd(const void* x, long long ldx, const void* weight, const vo
 /* Its gradients, given those of y: with h = (x - mean) rstd and g = dy weight,
  *   dx = rstd (g - mean(g) - h mean(g h)),  dweight = sum over rows of dy h,  dbias = sum over rows of dy.
  * dweight, dbias [C] of type `param_dtype`, either may be NULL; with both NULL, or a workspace of no bytes
- * (few rows, one kernel instead of two), the workspace may be NULL; else it is 16-byte aligned.  The sums are formed in fp32 in a fixed order: the same call gives the same bits.  dx overlaps neither x nor dy. */
+ * (few rows, one kernel instead of two), the workspace may be NULL; else it is 16-byte aligned.  The sums are formed in fp32 in
+ * a fixed order: the same call gives the same bits.  dx overlaps neither x nor dy. */
 long long bxl_layernorm_bwd_workspace_bytes(long long rows, int C);
 int bxl_layernorm_bwd(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
                       const void* weight, void* dx, long long lddx, void* dweight, void* dbias, long long rows, int C, int dtype,
