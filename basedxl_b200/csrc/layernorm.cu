@@ -382,7 +382,7 @@ struct TeamRing {
 // of single values: beyond 16 of them.)
 template <int VEC, int NV>
 __host__ __device__ constexpr bool fwd_params_shared() { return VEC == 1 ? NV > 16 : VEC == 8 && NV > 3; }
-// Bound by memory: 65536 x 1280 fp16 58 us (5.8 TB/s, 89 % of a copy's rate), 50000 x 1280 fp32 90 us (5.7 TB/s).
+// Bound by memory: 65536 x 1280 fp16 58 us (5.8 TB/s, 89 % of a copy's rate; 61 on a slower GPU), 50000 x 1280 fp32 90 us (5.7 TB/s).
 template <class T, int VEC, int NV, int kTeams>
 __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_teams_kernel(const LnArgs a, const LnTeams t) {
   constexpr bool kSub = kTeams != kWide;
@@ -482,8 +482,8 @@ __global__ void __launch_bounds__(kTeamThreads, NV * VEC <= 8 ? 2 : 1) ln_fwd_te
 }
 
 // ---- backward --------------------------------------------------------------------------------
-// fp32 rows are bound by memory (8192 x 5120 76 us without the column sums' second launch, 6.6 TB/s), 16-bit ones by issue slots (58 to 60 %
-// of them taken, by 16 warps an SM: the sums' registers allow no more): 50000 x 1280 71 us, 5.4 TB/s; 32768 x 640 27 us and 4.7 for
+// fp32 rows are bound by memory (8192 x 5120 76 us without the column sums' second launch, 6.6 TB/s), 16-bit ones by the 16 warps an SM that
+// the sums' registers allow (58 to 60 % of the issue slots taken): 50000 x 1280 71 us, 5.4 TB/s; 32768 x 640 27 us and 4.7 for
 // the second launch.
 template <class T, int VEC, int NV, int kTeams>
 __global__ void __launch_bounds__(kTeamThreads, 1) ln_bwd_teams_kernel(const LnArgs a, const LnTeams t) {

@@ -53,7 +53,7 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
 // multiply-adds instead the widening of x bounds it: 31.6, 8.9 and 3.0 us (one row of 2560 x 10240 10.5).
 // Any other rows are loaded value by value, lane 4 g + q the values q, q + 4 .. q + 28, which is bound by the number of loads: 8 x 2051 x
 // 8193 20.9 us, 4 x 1748 x 4672 12.3 (54.7 and 16.3 with a lane per value of K and fused multiply-adds; rows turned in shared memory 21.8
-// and 10.3, but the small calls slower).
+// and 10.3, but the small calls slower); 8 x 8193 x 2051 35 alone, 95 to 104 in a stream of such calls.
 constexpr int kFewMaxWarps = 8;
 template <class T, bool kVec>
 __global__ void __launch_bounds__(kFewMaxWarps * 32) few_rows_kernel(const FewRows p) {
